@@ -57,6 +57,17 @@ class PvCfg(ctypes.Structure):
     ]
 
 
+class MoeCfg(ctypes.Structure):
+    """gplk_moe_cfg (include/gplk.h)."""
+
+    _fields_ = [(name, _p) for name in ("x", "router", "gate", "up", "down", "sf_gate", "sf_up", "sf_down",
+                                        "alpha_gate", "alpha_up", "alpha_down", "y", "ids", "weights",
+                                        "workspace")] + [
+        ("workspace_bytes", _sz),
+        *[(name, _i) for name in ("T", "E", "top", "D", "F", "ldx", "ldy", "renormalise", "dtype")],
+    ]
+
+
 def lib() -> ctypes.CDLL:
     """Load libgplk.so (building it first if this checkout has nvcc and no
     library yet). Raises if it cannot be loaded."""
@@ -96,6 +107,12 @@ def lib() -> ctypes.CDLL:
             getattr(L, nm).argtypes = [_p, _p, _p, _i, _i, _i, _p]
     L.gplk_selftest_wait_timeout.restype = _i
     L.gplk_selftest_wait_timeout.argtypes = [ctypes.c_ulonglong, _p, _p]
+    L.gplk_gemv_nvfp4.restype = _i
+    L.gplk_gemv_nvfp4.argtypes = [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _i, _p]
+    L.gplk_moe_nvfp4.restype = _i
+    L.gplk_moe_nvfp4.argtypes = [ctypes.POINTER(MoeCfg), _p]
+    L.gplk_moe_nvfp4_workspace_bytes.restype = _sz
+    L.gplk_moe_nvfp4_workspace_bytes.argtypes = [_i, _i, _i, _i, _i]
     L.gplk_nvfp4_sf_bytes.restype = _sz
     L.gplk_nvfp4_sf_bytes.argtypes = [_i, _i]
     if hasattr(L, "gplk_powervirus_launch"):
@@ -220,6 +237,113 @@ def gemm_nvfp4_tn(A, B, SFA, SFB, D, K: int, alpha, stream=None) -> None:
     assert A.shape[1] * 2 == K and B.shape[1] * 2 == K and D.numel() == M * N
     _check("gplk_gemm_nvfp4_tn", lib().gplk_gemm_nvfp4_tn(_ptr(A), _ptr(B), _ptr(SFA), _ptr(SFB), _ptr(D),
                                                             M, N, K, _ptr(alpha), _stream(stream)))
+
+
+# ------------------------------------------------------------ a few tokens with NVFP4 weights
+
+MAX_TOKENS = 32
+
+
+def _act_dtype(t) -> int:
+    """GPLK_DTYPE_* of a tensor of activations (-1: neither)."""
+    import torch
+
+    return 0 if t.dtype == torch.bfloat16 else 1 if t.dtype == torch.float16 else -1
+
+
+def _need(fn: str, *conds) -> None:
+    """The checks a pointer cannot carry: shapes, types, devices."""
+    if not all(conds):
+        raise GplkError(fn, 1)
+
+
+def _rows(t) -> tuple[int, int, int]:
+    """(rows, columns, leading dimension) of a 2-D tensor with contiguous rows."""
+    r, c = t.shape
+    return r, c, t.stride(0) if r > 1 else max(c, 1)
+
+
+def _on(dev, fn: str, *tensors):
+    """Raises unless every tensor is on CUDA device `dev`; a context in which
+    that device is the current one."""
+    import contextlib
+
+    import torch
+
+    _need(fn, dev.type == "cuda", *[t.device == dev for t in tensors])
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, stream=None) -> None:
+    """Y = alpha * X @ w.T (+ residual) for up to 32 rows of activations.
+    X: (T, K), Y and residual: (T, N), all bf16 or all f16, rows contiguous and
+    any distance apart; residual may be Y. W: (N, K/2) packed E2M1 and SF its
+    scale bytes, as gemm_nvfp4_tn and operands.quantize_nvfp4 have them;
+    alpha: 1-element float32 tensor, the matrix scale."""
+    import torch
+
+    fn, dt = "gplk_gemv_nvfp4", _act_dtype(X)
+    _need(fn, X.dim() == 2, Y.dim() == 2, W.dim() == 2)
+    T, K, ldx = _rows(X)
+    T2, N, ldy = _rows(Y)
+    _need(fn, dt >= 0, Y.dtype == X.dtype, T2 == T, W.shape[0] == N, W.shape[1] * 2 == K, W.dtype == torch.uint8,
+          W.is_contiguous(), SF.dtype == torch.uint8, SF.is_contiguous(), alpha.dtype == torch.float32,
+          alpha.numel() == 1, K < 2 or X.stride(1) == 1, N < 2 or Y.stride(1) == 1,
+          SF.numel() >= nvfp4_sf_bytes(N, K))
+    ldr, rp = 0, None
+    if residual is not None:
+        _need(fn, residual.shape == Y.shape, residual.dtype == X.dtype, N < 2 or residual.stride(1) == 1,
+              residual.device == X.device)
+        ldr, rp = _rows(residual)[2], residual.data_ptr()
+    with _on(X.device, fn, W, SF, Y, alpha):
+        _check(fn, lib().gplk_gemv_nvfp4(_ptr(X), _ptr(W), _ptr(SF), _ptr(Y), rp, T, N, K, ldx, ldy, ldr, _ptr(alpha),
+                                         dt, _stream(stream)))
+
+
+def moe_nvfp4_workspace_bytes(T: int, E: int, top: int, D: int, F: int) -> int:
+    return int(lib().gplk_moe_nvfp4_workspace_bytes(T, E, top, D, F))
+
+
+def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = True, workspace="auto",
+              stream=None) -> None:
+    """A mixture-of-experts layer (gplk_moe_nvfp4) for up to 32 tokens.
+    X, Y: (T, D), bf16 or f16, rows contiguous and any distance apart;
+    router: (E, D) of the same type. gate, up, down: (W, SF, alpha) with W
+    (E, F, D/2), (E, F, D/2), (E, D, F/2) packed E2M1, SF (E, bytes) the scale
+    bytes of each expert's matrix and alpha (E,) float32. ids: (T, top) int32
+    and weights: (T, top) float32 receive each token's experts and their
+    weights. workspace: "auto" (from torch's allocator, on the call's stream),
+    or a uint8 CUDA tensor of moe_nvfp4_workspace_bytes that no overlapping
+    call uses."""
+    import torch
+
+    fn, dt = "gplk_moe_nvfp4", _act_dtype(X)
+    _need(fn, X.dim() == 2, Y.dim() == 2, router.dim() == 2, ids.dim() == 2)
+    T, D, ldx = _rows(X)
+    T2, D2, ldy = _rows(Y)
+    E, top = router.shape[0], ids.shape[1]
+    F = gate[0].shape[1] if gate[0].dim() == 3 else 0
+    _need(fn, dt >= 0, Y.dtype == X.dtype, (T2, D2) == (T, D), X.stride(1) == 1, Y.stride(1) == 1,
+          router.shape[1] == D, router.dtype == X.dtype, router.is_contiguous(), ids.dtype == torch.int32,
+          ids.shape[0] == T, ids.is_contiguous(), weights.shape == ids.shape, weights.dtype == torch.float32,
+          weights.is_contiguous())
+    for (w, sf, alpha), rows, k in ((gate, F, D), (up, F, D), (down, D, F)):
+        _need(fn, tuple(w.shape) == (E, rows, k // 2), w.dtype == torch.uint8, w.is_contiguous(),
+              sf.dtype == torch.uint8, sf.is_contiguous(), sf.numel() == E * nvfp4_sf_bytes(rows, k),
+              alpha.dtype == torch.float32, alpha.is_contiguous(), alpha.numel() == E)
+    with _on(X.device, fn, router, *gate, *up, *down, Y, ids, weights):
+        if isinstance(workspace, str):
+            # A fresh block of the caching allocator, in the stream's own pool:
+            # concurrent calls and captured graphs never share it.
+            with torch.cuda.stream(stream) if stream is not None else torch.cuda.stream(None):
+                workspace = torch.empty(max(1, moe_nvfp4_workspace_bytes(T, E, top, D, F)), dtype=torch.uint8,
+                                        device=X.device)
+        _need(fn, workspace.device == X.device, workspace.is_contiguous())
+        c = MoeCfg(_ptr(X), _ptr(router), _ptr(gate[0]), _ptr(up[0]), _ptr(down[0]), _ptr(gate[1]), _ptr(up[1]),
+                   _ptr(down[1]), _ptr(gate[2]), _ptr(up[2]), _ptr(down[2]), _ptr(Y), _ptr(ids), _ptr(weights),
+                   _ptr(workspace), workspace.numel() * workspace.element_size(), T, E, top, D, F, ldx, ldy,
+                   int(bool(renormalise)), dt)
+        _check(fn, lib().gplk_moe_nvfp4(ctypes.byref(c), _stream(stream)))
 
 
 # ------------------------------------------------------------ dense tensor-core GEMMs

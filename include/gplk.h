@@ -131,6 +131,70 @@ int gplk_gemm_nvfp4_tn(const uint8_t *A, const uint8_t *B, const uint8_t *SFA,
  * a K extent of k elements. */
 size_t gplk_nvfp4_sf_bytes(int rows, int k);
 
+/* ------------------------------------------------------------ a few tokens with NVFP4 weights
+ * These entry points have no counterpart in the reference, whose GEMM rungs
+ * are square. They are the narrow formats' other shape: a few activation
+ * rows against all of the weights, bound by HBM instead of the tensor cores.
+ * Activations are 16-bit, in one of two types: */
+#define GPLK_DTYPE_BF16 0
+#define GPLK_DTYPE_F16 1
+
+/* Y[t][n] = (*alpha) * sum_k X[t][k] * sf[n, k/16] * w[n, k]  (+ R[t][n])
+ * for T tokens (0 <= T <= 32) and N outputs. W (N rows of K/2 bytes) and SF
+ * (gplk_nvfp4_sf_bytes(N, K) bytes) are what gplk_gemm_nvfp4_tn takes as an
+ * operand; scales in the layout's padding do not
+ * affect the result. X, Y and R are
+ * row-major, of type `dtype`, with leading dimensions ldx >= K, ldy >= N and
+ * ldr >= N in elements. R may be NULL, and may be Y itself (Y is then
+ * updated in place); X must not overlap Y. Sums are FP32; each output is
+ * rounded once. alpha is a device pointer to the weights' per-tensor scale.
+ * Requires K % 64 == 0 and 16-byte aligned W and SF; X, Y and R may have any
+ * alignment and leading dimension (rows of X on 16-byte boundaries load
+ * fastest). The result does not depend on other calls or on timing: equal
+ * inputs give equal bits. */
+int gplk_gemv_nvfp4(const void *X, const uint8_t *W, const uint8_t *SF, void *Y, const void *R, int T,
+                    int N, int K, int ldx, int ldy, int ldr, const float *alpha, int dtype,
+                    cudaStream_t stream);
+
+/* A mixture-of-experts layer for T tokens (0 <= T <= 32):
+ *   logits = router x;  p = softmax(logits) over the E experts;  the `top`
+ *   experts of largest p, in that order, the lower index first among equals;
+ *   their p divided by its sum if renormalise != 0
+ *   h_e = silu(alpha_gate[e] * gate_e x) * (alpha_up[e] * up_e x)
+ *   y   = sum over the chosen e of p_e * alpha_down[e] * down_e h_e
+ * router is E x D row-major in the activations' type. gate and up hold E
+ * NVFP4 matrices of F rows by D, down E of D rows by F, one after another
+ * (F * D / 2 bytes each); sf_* their scales, gplk_nvfp4_sf_bytes(F, D) or
+ * (D, F) bytes per expert; alpha_* one FP32 per expert. Weights of experts
+ * that no token chose are not read. Logits, softmax, h and every sum are
+ * FP32. Requires D % 64 == 0, F % 64 == 0, E <= 512, top <= min(E, 16),
+ * E * F and E * D below 2^31; x, y and router in any alignment.
+ * x must not overlap y.
+ * The workspace (gplk_moe_nvfp4_workspace_bytes, 16-byte aligned, any
+ * content) serves one call at a time: calls that can overlap on the GPU
+ * need one each. */
+typedef struct {
+    const void *x;             /* T rows of D, leading dimension ldx */
+    const void *router;        /* E x D */
+    const uint8_t *gate, *up;  /* E x F x D / 2 */
+    const uint8_t *down;       /* E x D x F / 2 */
+    const uint8_t *sf_gate, *sf_up, *sf_down;
+    const float *alpha_gate, *alpha_up, *alpha_down; /* E each */
+    void *y;                   /* T rows of D, leading dimension ldy */
+    int32_t *ids;              /* T x top, or NULL: the chosen experts */
+    float *weights;            /* T x top, or NULL: their weights */
+    void *workspace;
+    size_t workspace_bytes;
+    int T, E, top, D, F;
+    int ldx, ldy;              /* elements */
+    int renormalise;
+    int dtype;
+} gplk_moe_cfg;
+
+/* Bytes of workspace of one call; 0 for sizes gplk_moe_nvfp4 refuses. */
+size_t gplk_moe_nvfp4_workspace_bytes(int T, int E, int top, int D, int F);
+int gplk_moe_nvfp4(const gplk_moe_cfg *cfg, cudaStream_t stream);
+
 /* ------------------------------------------------------------ dense tensor-core GEMMs
  * C = A * B in the reference's cublasGemmEx layout: every matrix column-major,
  * no transposes, alpha = 1, beta = 0:
