@@ -2,12 +2,52 @@
 //   y[t][n] = alpha * sum_k x[t][k] * sf[n][k / 16] * w[n][k]  (+ r[t][n])
 // with E2M1 weights and UE4M3 scales in the layout gplk_gemm_nvfp4_tn reads,
 // 16-bit activations and FP32 sums, rounded once to the activations' type.
+// The main loop here (stream_kernel) also runs the experts' products of
+// gplk_moe_nvfp4.cu.
+//
+// What bounds it: every weight is read once for 2 T operations, so HBM. A
+// B200 reads 46 weights per SM and clock; decoding them on the CUDA cores
+// takes about that many issue slots (one warp per row with FP32 FMAs measured
+// 0.56 TB/s at one token, 16384 x 8192). So the weights are not decoded at all:
+// they go from HBM through TMA to the block-scaled tensor-core MMA
+// (kind::mxf4nvf4), codes and scales as they lie, and the activations are
+// brought to its operand format instead, exactly enough to count as 16-bit:
+//
+//   Within a 16-group of a token, 2^b the power of two at or below its largest
+//   magnitude, x is rounded to a multiple of 2^b / 8192 and written in
+//   balanced base-8 digits  x = 2^b * sum_p d_p / 2 * 8^-p,  p = 0..4,
+//   d_0 in -4..4, the others in -4..3. Every d / 2 is an E2M1 value, so digit p
+//   of all of k is one E2M1 row ("plane") of the MMA's B operand, and 2^b,
+//   relative to the token's largest magnitude 2^A, is the group's UE4M3 scale.
+//   Five planes keep 15 bits: an activation is off by at most 2^-14 of its
+//   group's largest magnitude (2^-28 of the token's, in groups 2^14 below
+//   it), where BF16 itself is off by 2^-9 of each value. The accumulator
+//   column of each (token, plane) is exact products in FP32 sums; the epilogue
+//   adds 8^-p times the planes' columns.
+//
+// So T tokens are an MMA of N = 5 T columns (padded to 8), at most 160 of the
+// 256 an instruction takes, whose time at T = 32 is still below the time HBM
+// needs for the weights.
+//
+// Layout of the work. A block owns 128 weight rows (the MMA's M) and a slice
+// of K; blocks of a cluster share the rows, split K, and add their partial
+// sums in rank order through distributed shared memory, so the bits do not
+// depend on timing. Two blocks share an SM: one's start and end hide behind
+// the other's stream.
+//   warp 0      TMA producer: 128 rows x 128 bytes of codes and up to 2 KiB of
+//               scales per stage (256 elements of K) into a ring
+//   warp 1      owns TMEM; one thread copies the scales to TMEM and issues
+//               one MMA per 64 elements of K
+//   warps 2..9  convert the same 256 elements of every token into the stage's
+//               B rows and scales (a warp per token and stage); warps 2..5
+//               then read the accumulator, and all warps add the slices
+// Every mbarrier wait is bounded, as everywhere in this library.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp4.h>
-#include <cuda_fp8.h>
 
 #include <climits>
+#include <cstring>
+#include <type_traits>
 
 #include "gplk_ptx.cuh"
 
@@ -15,89 +55,588 @@ namespace gplk {
 namespace fewtok {
 
 constexpr int kMaxTokens = 32;
+constexpr int kMaxExperts = 512;
+constexpr int kMaxTop = 16;
+constexpr int kPlanes = 5;
+constexpr int kConvWarps = 8;
+constexpr int kThreads = 64 + 32 * kConvWarps;
+constexpr int kTileRows = 128;
+constexpr int kStageK = 256;                    // elements of K per stage
+constexpr uint32_t kWBytes = kTileRows * 128;   // codes of a stage
+constexpr uint32_t kSfaBytes = 4 * 512;         // scales of a stage
+constexpr int kMaxStages = 8;
+constexpr uint32_t kDigitBias = 4u * (1u + 8u + 64u + 512u + 4096u);
 
-template <typename T>
-__device__ __forceinline__ float to_f32(T v) {
-    if constexpr (sizeof(T) == 4) return (float)v;
-    else return static_cast<float>(v);
-}
+enum class Mode { Gemv, GateUp, Down };
+
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
     return static_cast<T>(v);
 }
 
-// Byte offset of the scale of 16-group g of row r (see gplk_nvfp4_sf_bytes).
-__device__ __forceinline__ size_t sf_offset(size_t r, int g, int kblocks4) {
-    return ((r >> 7) * (size_t)kblocks4 + (size_t)(g >> 2)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + (g & 3);
-}
-
-__device__ __forceinline__ float sf_value(uint8_t b) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
-}
-
-// Dot products of one weight row with up to 8 activation rows, over the
-// 16-groups of one warp's lanes; the warp's sums end in every lane.
-template <typename XT>
-__device__ __forceinline__ void row_dots(const uint8_t* w, const uint8_t* sf, size_t row, int K, const XT* const* x,
-                                         int nx, float (&acc)[8]) {
-    const int kb4 = (K + 63) / 64;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
-    for (int g = (int)lane_id(); g < K / 16; g += 32) {
-        const uint2 c = *reinterpret_cast<const uint2*>(w + row * (size_t)(K / 2) + (size_t)g * 8);
-        const float s = sf_value(sf[sf_offset(row, g, kb4)]);
-        float v[16];
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-            const uint8_t byte = (uint8_t)((b < 4 ? c.x : c.y) >> (8 * (b & 3)));
-            const __half2 h = __half2(__nv_cvt_fp4x2_to_halfraw2(byte, __NV_E2M1));
-            v[2 * b] = __low2float(h) * s;
-            v[2 * b + 1] = __high2float(h) * s;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < nx) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) acc[i] = fmaf(v[j], to_f32(x[i][g * 16 + j]), acc[i]);
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int o = 16; o; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-}
-
-struct GemvParams {
-    const void* X;
-    const uint8_t* W;
-    const uint8_t* SF;
-    void* Y;
-    const void* R;
-    const float* alpha;
-    int T, N, K, ldx, ldy, ldr;
+// ---------------------------------------------------------------- routing tables (MoE)
+// Written by the route kernel into the layer's workspace.
+struct Route {
+    int n_active;
+    int active[kMaxExperts];                    // chosen experts, ascending
+    int count[kMaxExperts];                     // tokens of active expert a
+    int16_t list[kMaxExperts][kMaxTokens];      // their slots (token * top + rank), ascending
+    int16_t slot[kMaxExperts][kMaxTokens];      // slot of token t with active expert a, or -1
 };
 
-template <typename XT>
-__global__ void __launch_bounds__(256) gemv_simple_kernel(const GemvParams p) {
-    const int n = blockIdx.x * 8 + (int)warp_id_uniform();
-    const int t0 = blockIdx.y * 8;
-    if (n >= p.N) return;
-    const int nx = min(8, p.T - t0);
-    const XT* x[8];
-    for (int i = 0; i < 8; ++i) x[i] = static_cast<const XT*>(p.X) + (size_t)(t0 + min(i, nx - 1)) * p.ldx;
-    float acc[8];
-    row_dots<XT>(p.W, p.SF, (size_t)n, p.K, x, nx, acc);
-    const float alpha = *p.alpha;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < nx && lane_id() == (uint32_t)i) {
-            float v = acc[i] * alpha;
-            if (p.R) v += to_f32(static_cast<const XT*>(p.R)[(size_t)(t0 + i) * p.ldr + n]);
-            static_cast<XT*>(p.Y)[(size_t)(t0 + i) * p.ldy + n] = from_f32<XT>(v);
-        }
+struct Params {
+    const void* X;       // activations (Gemv, GateUp: 16-bit rows; Down: FP32 h rows by slot)
+    const uint8_t* sf0;  // scales: W, gate or down
+    const uint8_t* sf1;  // GateUp: up
+    const float* alpha0; // Gemv: one; GateUp: gate's, per expert
+    const float* alpha1; // GateUp: up's
+    const float* alpha2; // GateUp: down's, folded into h
+    void* Y;             // Gemv, Down: T rows; GateUp: FP32 h rows by slot
+    const void* R;
+    const Route* route;
+    const float* weights;  // MoE: per slot
+    int T, N, K, ldx, ldy, ldr;
+    int x_vec;           // rows of X are 16-byte aligned
+    int top;
+    int tiles;           // 128-row tiles of one matrix
+    int k_stages;        // stages of one matrix row
+    int kblocks;         // K / 64
+    int split;           // slices of K
+    int nb;              // accumulator columns for T tokens
+    int stages;          // ring depth
+    uint32_t stage_bytes, sfb_bytes;
+    uint32_t tmem_cols, sf_col0, sf_slot;
+};
+
+struct Control {
+    uint64_t full[kMaxStages];
+    uint64_t empty[kMaxStages];
+    uint64_t acc_full;
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort;
+    uint32_t amax[kMaxTokens];  // bits of the largest magnitude in this block's slice
+    int16_t slot[kMaxTokens];   // GateUp: slots of the block's tokens
+};
+
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
 }
 
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Eight consecutive activations of one lane.
+template <typename XT>
+__device__ __forceinline__ void load_raw(const XT* x, bool vec, uint4 (&r)[2]) {
+    if constexpr (sizeof(XT) == 4) {
+        r[0] = *reinterpret_cast<const uint4*>(x);
+        r[1] = *reinterpret_cast<const uint4*>(x + 4);
+    } else if (vec) {
+        r[0] = *reinterpret_cast<const uint4*>(x);
+    } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+        r[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+template <typename XT>
+__device__ __forceinline__ void widen(const uint4 (&r)[2], float (&v)[8]) {
+    const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+    if constexpr (sizeof(XT) == 4) {
+        const uint32_t w1[4] = {r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __uint_as_float(w[i]);
+            v[4 + i] = __uint_as_float(w1[i]);
+        }
+    } else if constexpr (std::is_same<XT, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
+            v[2 * i] = __low2float(h);
+            v[2 * i + 1] = __high2float(h);
+        }
+    }
+}
+
+// Bits of the largest magnitude. Integer order is magnitude order, with
+// infinity and then NaN above every finite number.
+__device__ __forceinline__ uint32_t max_bits(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
+}
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// Exponent A of a token's largest magnitude. Below 2^-100 the anchor stays
+// there: what is then lost is below 2^-127, FP32's own subnormal range.
+__device__ __forceinline__ int anchor_of(uint32_t amax_bits) { return max((int)(amax_bits >> 23) - 127, -100); }
+
+// Eight nibbles of biased digits (0..7 for -4..3; 8 for the top digit's 4) to
+// E2M1 codes of d / 2: magnitude |d| in the low three bits, sign above.
+template <bool TOP>
+__device__ __forceinline__ uint32_t digit_codes(uint32_t w) {
+    uint32_t m = ~(w >> 2);  // 1 in the nibbles of negative digits
+    if constexpr (TOP) m &= ~(w >> 3);
+    m &= 0x11111111u;
+    uint32_t c = ((w ^ (m * 3u)) & 0x33333333u) + m * 9u;  // negative: 8 | (3 - w) + 1
+    if constexpr (TOP) c |= (w >> 1) & 0x44444444u;
+    return c;
+}
+
+// One token's 256 elements of a stage, eight per lane: planes 5 t .. 5 t + 4
+// of the stage's B rows (128-byte swizzled, K-major) and the 16 groups'
+// scales. `on` is false for lanes beyond K, whose blocks no MMA reads.
+__device__ __forceinline__ void convert(const float (&v)[8], int anchor, int t, bool on, uint8_t* b_rows,
+                                        uint8_t* sfb, uint32_t lane) {
+    uint32_t m = max_bits(v);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));  // the other half of the 16-group
+    const int b = max((int)(m >> 23) - 127, anchor - 14);
+    const float scale = __uint_as_float((uint32_t)(13 - b + 127) << 23);
+    // x * scale is at most 2^14 in magnitude; adding 1.5 * 2^23 rounds it to an
+    // integer, and the bias makes every digit non-negative.
+    constexpr float kMagic = 12582912.0f + (float)kDigitBias;
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__fmaf_rn(v[i], scale, kMagic));
+    uint32_t q[4];  // elements i and i + 4: nibbles i and i + 4 of a word are 16 bits apart
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = __byte_perm(u[i], u[i + 4], 0x5410);
+    if (!on) return;
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+        const int sh = 3 * (kPlanes - 1 - p);
+        const uint32_t mask = p == 0 ? 0x000F000Fu : 0x00070007u;
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= ((q[i] >> sh) & mask) << (4 * i);
+        w = p == 0 ? digit_codes<true>(w) : digit_codes<false>(w);
+        const uint32_t r = (uint32_t)(kPlanes * t + p);
+        *reinterpret_cast<uint32_t*>(b_rows + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
+                                     (lane & 3) * 4) = w;
+        if ((lane & 1) == (uint32_t)(p & 1))
+            sfb[(r >> 7) * 2048 + (lane >> 3) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((lane >> 1) & 3)] =
+                (uint8_t)((b - anchor + 15) << 3);
+    }
+}
+
+// A token without a part in the stage's expert: zero digits, scale 1.
+__device__ __forceinline__ void convert_zero(int t, uint8_t* b_rows, uint8_t* sfb, uint32_t lane) {
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+        const uint32_t r = (uint32_t)(kPlanes * t + p);
+        *reinterpret_cast<uint32_t*>(b_rows + (r >> 3) * 1024 + (r & 7) * 128 + lane * 4) = 0u;
+        if ((lane & 1) == (uint32_t)(p & 1))
+            sfb[(r >> 7) * 2048 + (lane >> 3) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((lane >> 1) & 3)] = 0x38;
+    }
+}
+
+__device__ __forceinline__ uint32_t pad8(uint32_t n) { return (n + 7) & ~7u; }
+
+template <Mode M, typename XT, typename YT>
+__global__ void __launch_bounds__(kThreads, 2)
+    stream_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1, const Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    Control& sm = *reinterpret_cast<Control*>(ring + (size_t)p.stages * p.stage_bytes);
+    const uint32_t warp = warp_id_uniform();
+    const uint32_t lane = lane_id();
+    const int rank = (int)cluster_ctarank();
+    const int csize = (M == Mode::GateUp ? 2 : 1) * p.split;
+    const int cid = (int)blockIdx.x / csize;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(&sm.full[i], 1 + kConvWarps);
+            mbar_init(&sm.empty[i], 1);
+        }
+        mbar_init(&sm.acc_full, 1);
+        mbar_init(&sm.drain, 1);
+        sm.abort = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tm0);
+        if (M == Mode::GateUp) tma_prefetch_desc(&tm1);
+    }
+    if (threadIdx.x < kMaxTokens) sm.amax[threadIdx.x] = 0;
+    if (warp == 1) {
+        tmem_alloc(&sm.tmem_base, p.tmem_cols);
+        tmem_relinquish();
+    }
+    // The set-up above may overlap the previous kernel's tail; nothing below
+    // touches global memory before that kernel has completed.
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // This block's rows, tokens and stages.
+    int tile = cid, slice = rank, expert = 0, ntok = p.T, total = p.k_stages;
+    bool second = false;  // GateUp: the `up` half of the cluster
+    if constexpr (M == Mode::GateUp) {
+        const int a = cid / p.tiles;
+        tile = cid % p.tiles;
+        second = rank >= p.split;
+        slice = second ? rank - p.split : rank;
+        if (a < p.route->n_active) {
+            expert = p.route->active[a];
+            ntok = p.route->count[a];
+            if (threadIdx.x < (unsigned)ntok) sm.slot[threadIdx.x] = p.route->list[a][threadIdx.x];
+        } else {
+            ntok = 0;
+            total = 0;
+        }
+    } else if constexpr (M == Mode::Down) {
+        total = p.route->n_active * p.k_stages;
+    }
+    const int first = (int)((long long)total * slice / p.split);
+    const int nst = (int)((long long)total * (slice + 1) / p.split) - first;
+    const uint32_t nb = M == Mode::GateUp ? pad8((uint32_t)(kPlanes * ntok)) : (uint32_t)p.nb;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0, issued_mask = 0, issued_parity = 0;
+            bool ok = true;
+            const CUtensorMap* tm = second ? &tm1 : &tm0;
+            const size_t sf_matrix = (size_t)p.tiles * (size_t)p.kblocks * 512;
+            for (int i = 0; i < nst; ++i) {
+                if (!mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, 0x0601)) {
+                    ok = false;
+                    break;
+                }
+                int kb = first + i;
+                if constexpr (M == Mode::Down) {
+                    expert = p.route->active[kb / p.k_stages];
+                    kb %= p.k_stages;
+                }
+                const uint32_t sf_bytes = 512u * (uint32_t)min(4, p.kblocks - 4 * kb);
+                uint8_t* st = ring + (size_t)stage * p.stage_bytes;
+                const uint8_t* sf = (second ? p.sf1 : p.sf0) + (size_t)expert * sf_matrix +
+                                    ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
+                mbar_arrive_expect_tx(&sm.full[stage], kWBytes + sf_bytes);
+                tma_load_2d(st, tm, &sm.full[stage], kb * 128, expert * p.N + tile * kTileRows);
+                bulk_load(st + kWBytes + (size_t)p.nb * 128, sf, sf_bytes, &sm.full[stage]);
+                issued_mask |= 1u << stage;
+                issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (!ok || *(volatile int*)&sm.abort) {
+                // Drain: every issued copy must land before the block exits.
+                int dummy = 0;
+                for (int s2 = 0; s2 < p.stages; ++s2)
+                    if (issued_mask & (1u << s2))
+                        mbar_wait(&sm.full[s2], (issued_parity >> s2) & 1u, &dummy, 0x0602, 100000000ull);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0 && nst > 0) {
+            const uint32_t idesc = idesc_nvf4(kTileRows, (int)nb);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int i = 0; i < nst; ++i) {
+                if (!mbar_wait(&sm.full[stage], phase, &sm.abort, 0x0611)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const int kb = M == Mode::Down ? (first + i) % p.k_stages : first + i;
+                const int nblk = min(4, p.kblocks - 4 * kb);
+                const uint32_t a_addr = smem_u32(ring) + (uint32_t)stage * p.stage_bytes;
+                const uint32_t b_addr = a_addr + kWBytes;
+                const uint32_t sfa_addr = b_addr + (uint32_t)p.nb * 128;
+                const uint32_t sfb_addr = sfa_addr + kSfaBytes;
+                const uint32_t sf_col = tmem + p.sf_col0 + (uint32_t)stage * p.sf_slot;
+                // A: K-block j at sf_col + 4 j. B: K-block j, 128-row half h at
+                // sf_col + 16 + 8 j + 4 h (two halves), or sf_col + 16 + 4 j.
+                const uint32_t bstep = p.sf_slot > 32 ? 8u : 4u;
+                for (int j = 0; j < nblk; ++j) {
+                    tmem_cp_32x128b_warpx4(sf_col + 4 * j, smem_desc(sfa_addr + 512 * j, 0, 128, 0));
+                    tmem_cp_32x128b_warpx4(sf_col + 16 + bstep * j, smem_desc(sfb_addr + 512 * j, 0, 128, 0));
+                    if (bstep == 8u)
+                        tmem_cp_32x128b_warpx4(sf_col + 20 + 8 * j, smem_desc(sfb_addr + 2048 + 512 * j, 0, 128, 0));
+                }
+                for (int j = 0; j < nblk; ++j)
+                    mma_nvf4(tmem, desc_kmajor_sw128(a_addr + 32 * j), desc_kmajor_sw128(b_addr + 32 * j), idesc,
+                             sf_col + 4 * j, sf_col + 16 + bstep * j, (i | j) != 0);
+                tc_commit(&sm.empty[stage]);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (ok) tc_commit(&sm.acc_full);
+            // Every MMA issued by this thread completes before TMEM is freed.
+            tc_commit(&sm.drain);
+            int dummy = 0;
+            mbar_wait(&sm.drain, 0, &dummy, 0x0613, 100000000ull);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------ activations
+        const int w = (int)warp - 2;
+        // Lane's eight elements of token t in stage i; false: none.
+        auto load = [&](int i, int t, uint4 (&r)[2]) -> bool {
+            int kb = first + i, row = t;
+            if constexpr (M == Mode::Down) {
+                row = p.route->slot[kb / p.k_stages][t];
+                kb %= p.k_stages;
+            } else if constexpr (M == Mode::GateUp) {
+                row = sm.slot[t] / p.top;
+            }
+            const int k = kb * kStageK + (int)lane * 8;
+            r[0] = r[1] = make_uint4(0, 0, 0, 0);
+            if (row < 0) return false;
+            if (k < p.K) load_raw(static_cast<const XT*>(p.X) + (size_t)row * p.ldx + k, p.x_vec != 0, r);
+            return true;
+        };
+        // Largest magnitude of each token over the block's slice.
+        const int units = nst * ntok;
+        for (int u0 = w; u0 < units; u0 += 4 * kConvWarps) {
+            uint4 r[4][2];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int u = u0 + c * kConvWarps;
+                r[c][0] = r[c][1] = make_uint4(0, 0, 0, 0);
+                if (u < units) load(u / ntok, u % ntok, r[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int u = u0 + c * kConvWarps;
+                float v[8];
+                widen<XT>(r[c], v);
+                const uint32_t m = __reduce_max_sync(0xffffffffu, max_bits(v));
+                if (lane == 0 && u < units) atomicMax(&sm.amax[u % ntok], m);
+            }
+        }
+        named_sync(1, 32 * kConvWarps);
+        // Stage i: this warp converts tokens t = w - i (mod 8), so one token's
+        // stages rotate over the warps. The next unit's elements are loaded
+        // before the current one's are converted.
+        int ni = 0, nt = w & 7;
+        auto settle = [&]() {
+            while (nt >= ntok && ni < nst) {
+                ++ni;
+                nt = (w - ni) & 7;
+            }
+        };
+        uint4 next[2];
+        bool next_on = false;
+        settle();
+        if (ni < nst) next_on = load(ni, nt, next);
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int i = 0; i < nst; ++i) {
+            if (!mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, 0x0621)) break;
+            __syncwarp();
+            uint8_t* b_rows = ring + (size_t)stage * p.stage_bytes + kWBytes;
+            uint8_t* sfb = b_rows + (size_t)p.nb * 128 + kSfaBytes;
+            const int kb = M == Mode::Down ? (first + i) % p.k_stages : first + i;
+            const bool in_k = kb * kStageK + (int)lane * 8 < p.K;
+            for (int t = (w - i) & 7; t < ntok; t += kConvWarps) {
+                float v[8];
+                widen<XT>(next, v);
+                const bool on = next_on;
+                nt += kConvWarps;
+                settle();
+                if (ni < nst) next_on = load(ni, nt, next);
+                if (M != Mode::Down || on) convert(v, anchor_of(sm.amax[t]), t, in_k, b_rows, sfb, lane);
+                else convert_zero(t, b_rows, sfb, lane);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.full[stage]);
+            if (++stage == p.stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        __syncwarp();
+        // ------------------------------------------------------------ partial sums
+        // Warps 2..5: a thread reads its row's columns, adds the planes and
+        // leaves the slice's sum in shared memory (the ring's first stage, whose
+        // last use the accumulator barrier has seen complete).
+        if (w < 4) {
+            float* part = reinterpret_cast<float*>(ring);
+            const uint32_t quarter = warp & 3u;
+            const int row = (int)(quarter * 32 + lane);
+            const float alpha = M == Mode::Gemv ? __ldg(p.alpha0)
+                                : M == Mode::GateUp ? __ldg((second ? p.alpha1 : p.alpha0) + expert)
+                                                    : 1.0f;
+            if (nst > 0) {
+                mbar_wait(&sm.acc_full, 0, &sm.abort, 0x0631);
+                __syncwarp();
+                tc_fence_after();
+                for (int t0 = 0; t0 < ntok; t0 += 8) {
+                    uint32_t c[5][8];
+#pragma unroll
+                    for (int i = 0; i < 5; ++i)
+                        tmem_ld_32x32b_x8(tmem + ((quarter * 32u) << 16) + (uint32_t)(kPlanes * t0 + 8 * i), c[i]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (t0 + i >= ntok) continue;
+                        auto col = [&](int n) { return __uint_as_float(c[n >> 3][n & 7]); };
+                        float s = col(5 * i + 4);
+#pragma unroll
+                        for (int q = 3; q >= 0; --q) s = __fmaf_rn(s, 0.125f, col(5 * i + q));
+                        const uint32_t mb = sm.amax[t0 + i];
+                        s = s * alpha * __uint_as_float((uint32_t)(anchor_of(mb) - 8 + 127) << 23);
+                        if (mb >= kInfBits) s = __uint_as_float(0x7FC00000u);
+                        part[(t0 + i) * kTileRows + row] = s;
+                    }
+                }
+                tc_fence_before();
+            } else {
+                for (int t = 0; t < ntok; ++t) part[t * kTileRows + row] = 0.0f;
+            }
+        }
+    }
+    __syncwarp();
+    cluster_sync();
+
+    // ---------------------------------------------------------------- slices
+    // The cluster's blocks share the rows out; slices add in rank order.
+    {
+        const int rows = kTileRows / csize;
+        const uint32_t base = smem_u32(ring);
+        for (int i = (int)threadIdx.x; i < ntok * rows; i += kThreads) {
+            const int t = i / rows, r = rank * rows + i % rows;
+            const int n = tile * kTileRows + r;
+            if (n >= p.N) continue;
+            const uint32_t off = base + (uint32_t)(t * kTileRows + r) * 4u;
+            float s = 0.0f;
+            for (int c = 0; c < p.split; ++c) s += ld_cluster_f32(mapa_shared(off, (uint32_t)c));
+            if constexpr (M == Mode::Gemv) {
+                if (p.R) s += static_cast<float>(static_cast<const YT*>(p.R)[(size_t)t * p.ldr + n]);
+                static_cast<YT*>(p.Y)[(size_t)t * p.ldy + n] = from_f32<YT>(s);
+            } else if constexpr (M == Mode::GateUp) {
+                float u = 0.0f;
+                for (int c = 0; c < p.split; ++c) u += ld_cluster_f32(mapa_shared(off, (uint32_t)(p.split + c)));
+                const int slot = sm.slot[t];
+                const float c = p.weights[slot] * __ldg(p.alpha2 + expert);
+                static_cast<float*>(p.Y)[(size_t)slot * p.ldy + n] = s / (1.0f + expf(-s)) * u * c;
+            } else {
+                static_cast<YT*>(p.Y)[(size_t)t * p.ldy + n] = from_f32<YT>(s);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // no block leaves while another may read its sums
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, p.tmem_cols);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
 static inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// Accumulator columns, ring depth and TMEM for T tokens. Up to 25 tokens (128
+// columns) two blocks share an SM, each with half of its shared memory and
+// 256 TMEM columns; above, the second 128 rows of B scales and the larger
+// stages leave room for one.
+struct Shape {
+    int per_sm;
+    size_t smem;
+};
+
+static Shape set_shape(Params& p) {
+    p.nb = (kPlanes * p.T + 7) & ~7;
+    const bool wide = p.nb > 128;
+    p.sfb_bytes = wide ? 4096 : 2048;
+    p.stage_bytes = kWBytes + (uint32_t)p.nb * 128 + kSfaBytes + p.sfb_bytes;
+    const size_t overhead = 1024 + ((sizeof(Control) + 127) & ~(size_t)127);
+    // 228 KiB per SM, 1 KiB of it reserved per block.
+    const size_t room = (wide ? 227 * 1024 : (228 * 1024 - 2 * 1024) / 2) - overhead;
+    p.stages = (int)(room / p.stage_bytes);
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    p.sf_col0 = ((uint32_t)p.nb + 15) & ~15u;
+    p.sf_slot = wide ? 48 : 32;
+    p.tmem_cols = wide ? 512 : 256;
+    return {wide ? 1 : 2, (size_t)p.stages * p.stage_bytes + overhead};
+}
+
+// Slices of K: the split whose waves of blocks, each as long as its stages and
+// about two more for its start and end, take the fewest stage times. `units`
+// blocks would run without a split, each of `stages` stages.
+static int choose_split(double units, double stages, int max_split, int slots) {
+    int best = 1;
+    double best_cost = 0;
+    for (int s = 1; s <= max_split; s *= 2) {
+        if (s > 1 && stages < s) break;
+        const double waves = (double)(long long)((units * s + slots - 1) / slots);
+        const double cost = waves * ((stages + s - 1) / s + 2.0);
+        if (s == 1 || cost < best_cost) {
+            best = s;
+            best_cost = cost;
+        }
+    }
+    return best;
+}
+
+template <Mode M, typename XT, typename YT>
+static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const Params& p, size_t smem, int clusters,
+                         cudaStream_t stream) {
+    auto kernel = stream_kernel<M, XT, YT>;
+    static thread_local uint64_t configured = 0;  // bit per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GPLK_STATUS_CUDA_ERROR;
+    if (!(configured & (1ull << dev))) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
+            return GPLK_STATUS_LAUNCH_FAIL;
+        configured |= 1ull << dev;
+    }
+    const int csize = (M == Mode::GateUp ? 2 : 1) * p.split;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * csize));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)csize;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return launch_status(cudaLaunchKernelEx(&cfg, kernel, tm0, tm1, p));
+}
+
+// Tensor map of `rows` weight rows of K / 2 bytes, boxes of 128 rows x 128 bytes.
+static int encode_weights(CUtensorMap* map, const uint8_t* W, uint64_t rows, int K) {
+    return encode_tmap_2d_u8(map, W, (uint64_t)K / 2, rows, (uint64_t)K / 2, 128, kTileRows);
+}
 
 }  // namespace fewtok
 }  // namespace gplk
@@ -111,15 +650,37 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     if (dtype != GPLK_DTYPE_BF16 && dtype != GPLK_DTYPE_F16) return GPLK_STATUS_BAD_ARG;
     if (T == 0 || N == 0) return GPLK_STATUS_OK;
     if (K == 0 || K % 64 != 0 || ldx < K || ldy < N || (R && ldr < N)) return GPLK_STATUS_BAD_ARG;
+    if (N > INT_MAX / 8) return GPLK_STATUS_BAD_ARG;  // N / 128 tiles of 8 slices fit a grid
     if (!X || !W || !SF || !Y || !alpha) return GPLK_STATUS_BAD_ARG;
     if (!aligned16(W) || !aligned16(SF) || !aligned(X, 2) || !aligned(Y, 2) || !aligned(R, 2) || !aligned(alpha, 4))
         return GPLK_STATUS_BAD_ARG;
     DeviceInfo d;
-    const int st = require_sm100(&d);
+    int st = require_sm100(&d);
     if (st != GPLK_STATUS_OK) return st;
-    const GemvParams p{X, W, SF, Y, R, alpha, T, N, K, ldx, ldy, ldr};
-    const dim3 grid((unsigned)(((long)N + 7) / 8), (unsigned)((T + 7) / 8));
-    if (dtype == GPLK_DTYPE_BF16) gemv_simple_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(p);
-    else gemv_simple_kernel<__half><<<grid, 256, 0, stream>>>(p);
-    return launch_status(cudaGetLastError());
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.X = X;
+    p.sf0 = SF;
+    p.alpha0 = alpha;
+    p.Y = Y;
+    p.R = R;
+    p.T = T;
+    p.N = N;
+    p.K = K;
+    p.ldx = ldx;
+    p.ldy = ldy;
+    p.ldr = ldr;
+    p.x_vec = aligned16(X) && (T == 1 || ldx % 8 == 0);
+    p.tiles = (N + kTileRows - 1) / kTileRows;
+    p.k_stages = (K + kStageK - 1) / kStageK;
+    p.kblocks = K / 64;
+    const Shape s = set_shape(p);
+    if (s.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
+    p.split = choose_split(p.tiles, p.k_stages, 8, s.per_sm * d.sm_count);
+    CUtensorMap tm;
+    st = encode_weights(&tm, W, (uint64_t)N, K);
+    if (st != GPLK_STATUS_OK) return st;
+    return dtype == GPLK_DTYPE_BF16
+               ? launch_stream<Mode::Gemv, __nv_bfloat16, __nv_bfloat16>(tm, tm, p, s.smem, p.tiles, stream)
+               : launch_stream<Mode::Gemv, __half, __half>(tm, tm, p, s.smem, p.tiles, stream);
 }

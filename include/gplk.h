@@ -148,7 +148,7 @@ size_t gplk_nvfp4_sf_bytes(int rows, int k);
  * ldr >= N in elements. R may be NULL, and may be Y itself (Y is then
  * updated in place); X must not overlap Y. Sums are FP32; each output is
  * rounded once. alpha is a device pointer to the weights' per-tensor scale.
- * Requires K % 64 == 0 and 16-byte aligned W and SF; X, Y and R may have any
+ * Requires K % 64 == 0, N < 2^28 and 16-byte aligned W and SF; X, Y and R may have any
  * alignment and leading dimension (rows of X on 16-byte boundaries load
  * fastest). The result does not depend on other calls or on timing: equal
  * inputs give equal bits. */
@@ -168,7 +168,7 @@ int gplk_gemv_nvfp4(const void *X, const uint8_t *W, const uint8_t *SF, void *Y,
  * (D, F) bytes per expert; alpha_* one FP32 per expert. Weights of experts
  * that no token chose are not read. Logits, softmax, h and every sum are
  * FP32. Requires D % 64 == 0, F % 64 == 0, E <= 512, top <= min(E, 16),
- * E * F and E * D below 2^31; x, y and router in any alignment.
+ * E * F and E * D below 2^28; x, y and router in any alignment.
  * x must not overlap y.
  * The workspace (gplk_moe_nvfp4_workspace_bytes, 16-byte aligned, any
  * content) serves one call at a time: calls that can overlap on the GPU
