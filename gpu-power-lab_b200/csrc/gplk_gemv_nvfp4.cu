@@ -126,6 +126,17 @@ __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[
                  : "memory");
 }
 
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e != 0;
+}
+
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -355,8 +366,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        if (lane == 0 && nst > 0) {
+        // The whole warp runs the loop, so addresses and descriptors stay in
+        // uniform registers, and one elected lane issues.
+        if (nst > 0) {
             const uint32_t idesc = idesc_nvf4(kTileRows, (int)nb);
+            const uint32_t bstep = p.sf_slot > 32 ? 8u : 4u;
+            const uint64_t op_desc = desc_kmajor_sw128(0), sf_desc = smem_desc(0, 0, 128, 0);
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -365,35 +380,50 @@ __global__ void __launch_bounds__(kThreads, 2)
                     ok = false;
                     break;
                 }
+                __syncwarp();
                 tc_fence_after();
                 const int kb = M == Mode::Down ? (first + i) % p.k_stages : first + i;
                 const int nblk = min(4, p.kblocks - 4 * kb);
                 const uint32_t a_addr = smem_u32(ring) + (uint32_t)stage * p.stage_bytes;
-                const uint32_t b_addr = a_addr + kWBytes;
-                const uint32_t sfa_addr = b_addr + (uint32_t)p.nb * 128;
-                const uint32_t sfb_addr = sfa_addr + kSfaBytes;
+                const uint32_t sfa_addr = a_addr + kWBytes + (uint32_t)p.nb * 128;
+                const uint64_t a_desc = op_desc + (a_addr >> 4), b_desc = a_desc + (kWBytes >> 4);
+                const uint64_t sfa_desc = sf_desc + (sfa_addr >> 4), sfb_desc = sfa_desc + (kSfaBytes >> 4);
                 const uint32_t sf_col = tmem + p.sf_col0 + (uint32_t)stage * p.sf_slot;
                 // A: K-block j at sf_col + 4 j. B: K-block j, 128-row half h at
                 // sf_col + 16 + 8 j + 4 h (two halves), or sf_col + 16 + 4 j.
-                const uint32_t bstep = p.sf_slot > 32 ? 8u : 4u;
-                for (int j = 0; j < nblk; ++j) {
-                    tmem_cp_32x128b_warpx4(sf_col + 4 * j, smem_desc(sfa_addr + 512 * j, 0, 128, 0));
-                    tmem_cp_32x128b_warpx4(sf_col + 16 + bstep * j, smem_desc(sfb_addr + 512 * j, 0, 128, 0));
-                    if (bstep == 8u)
-                        tmem_cp_32x128b_warpx4(sf_col + 20 + 8 * j, smem_desc(sfb_addr + 2048 + 512 * j, 0, 128, 0));
+                auto scales = [&](int j) {
+                    tmem_cp_32x128b_warpx4(sf_col + 4 * j, sfa_desc + 32 * j);
+                    tmem_cp_32x128b_warpx4(sf_col + 16 + bstep * j, sfb_desc + 32 * j);
+                    if (bstep == 8u) tmem_cp_32x128b_warpx4(sf_col + 20 + 8 * j, sfb_desc + 128 + 32 * j);
+                };
+                auto product = [&](int j) {
+                    mma_nvf4(tmem, a_desc + 2 * j, b_desc + 2 * j, idesc, sf_col + 4 * j, sf_col + 16 + bstep * j,
+                             (i | j) != 0);
+                };
+                if (elect_one()) {
+                    if (nblk == 4) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) scales(j);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) product(j);
+                    } else {
+                        for (int j = 0; j < nblk; ++j) scales(j);
+                        for (int j = 0; j < nblk; ++j) product(j);
+                    }
+                    tc_commit(&sm.empty[stage]);
                 }
-                for (int j = 0; j < nblk; ++j)
-                    mma_nvf4(tmem, desc_kmajor_sw128(a_addr + 32 * j), desc_kmajor_sw128(b_addr + 32 * j), idesc,
-                             sf_col + 4 * j, sf_col + 16 + bstep * j, (i | j) != 0);
-                tc_commit(&sm.empty[stage]);
+                __syncwarp();
                 if (++stage == p.stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
             }
-            if (ok) tc_commit(&sm.acc_full);
-            // Every MMA issued by this thread completes before TMEM is freed.
-            tc_commit(&sm.drain);
+            if (elect_one()) {
+                if (ok) tc_commit(&sm.acc_full);
+                // Every MMA issued completes before TMEM is freed.
+                tc_commit(&sm.drain);
+            }
+            __syncwarp();
             int dummy = 0;
             mbar_wait(&sm.drain, 0, &dummy, 0x0613, 100000000ull);
         }
