@@ -59,7 +59,6 @@ constexpr int kMaxExperts = 512;
 constexpr int kMaxTop = 16;
 constexpr int kPlanes = 5;
 constexpr int kConvWarps = 8;
-constexpr int kThreads = 64 + 32 * kConvWarps;
 constexpr int kTileRows = 128;
 constexpr int kStageK = 256;                    // elements of K per stage
 constexpr uint32_t kWBytes = kTileRows * 128;   // codes of a stage
@@ -95,6 +94,9 @@ struct Params {
     const void* R;
     const Route* route;
     const float* weights;  // MoE: per slot
+    const uint8_t* image;  // Image kernels: the converted activations, by stage
+    const uint32_t* amax;  // bits of each token's largest magnitude, or NULL: this kernel finds its slice's
+    uint32_t* amax_out;    // GateUp: h's, by token
     int T, N, K, ldx, ldy, ldr;
     int x_vec;           // rows of X are 16-byte aligned
     int top;
@@ -117,6 +119,7 @@ struct Control {
     int abort;
     uint32_t amax[kMaxTokens];  // bits of the largest magnitude in this block's slice
     int16_t slot[kMaxTokens];   // GateUp: slots of the block's tokens
+    uint8_t dirty[kMaxStages][kMaxTokens];  // Down: the ring slot holds digits of that token
 };
 
 __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -262,8 +265,11 @@ __device__ __forceinline__ void convert_zero(int t, uint8_t* b_rows, uint8_t* sf
 
 __device__ __forceinline__ uint32_t pad8(uint32_t n) { return (n + 7) & ~7u; }
 
-template <Mode M, typename XT, typename YT>
-__global__ void __launch_bounds__(kThreads, 2)
+template <bool IMAGE>
+constexpr int kThreads = IMAGE ? 64 + 128 : 64 + 32 * kConvWarps;
+
+template <Mode M, typename XT, typename YT, bool IMAGE>
+__global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     stream_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
-            mbar_init(&sm.full[i], 1 + kConvWarps);
+            mbar_init(&sm.full[i], IMAGE ? 1 : 1 + kConvWarps);
             mbar_init(&sm.empty[i], 1);
         }
         mbar_init(&sm.acc_full, 1);
@@ -291,9 +297,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         tmem_alloc(&sm.tmem_base, p.tmem_cols);
         tmem_relinquish();
     }
-    // The set-up above may overlap the previous kernel's tail; nothing below
-    // touches global memory before that kernel has completed.
-    pdl_wait();
+    // The set-up above may overlap the previous kernel's tail. The conversion
+    // kernel that an Image kernel follows let it start only once every kernel
+    // before the two had completed, so weights may be read at once; what that
+    // kernel wrote is read behind its own pdl_wait(). Elsewhere nothing below
+    // touches global memory before the previous kernel has completed.
+    if constexpr (!IMAGE) pdl_wait();
     pdl_launch_dependents();
 
     // This block's rows, tokens and stages.
@@ -331,11 +340,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             bool ok = true;
             const CUtensorMap* tm = second ? &tm1 : &tm0;
             const size_t sf_matrix = (size_t)p.tiles * (size_t)p.kblocks * 512;
-            for (int i = 0; i < nst; ++i) {
-                if (!mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, 0x0601)) {
-                    ok = false;
-                    break;
-                }
+            const uint32_t image_bytes = IMAGE ? (uint32_t)p.nb * 128 + p.sfb_bytes : 0u;
+            auto load_weights = [&](int i) {
                 int kb = first + i;
                 if constexpr (M == Mode::Down) {
                     expert = p.route->active[kb / p.k_stages];
@@ -345,15 +351,43 @@ __global__ void __launch_bounds__(kThreads, 2)
                 uint8_t* st = ring + (size_t)stage * p.stage_bytes;
                 const uint8_t* sf = (second ? p.sf1 : p.sf0) + (size_t)expert * sf_matrix +
                                     ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
-                mbar_arrive_expect_tx(&sm.full[stage], kWBytes + sf_bytes);
+                mbar_arrive_expect_tx(&sm.full[stage], kWBytes + sf_bytes + image_bytes);
                 tma_load_2d(st, tm, &sm.full[stage], kb * 128, expert * p.N + tile * kTileRows);
-                bulk_load(st + kWBytes + (size_t)p.nb * 128, sf, sf_bytes, &sm.full[stage]);
+                bulk_load(st + kWBytes, sf, sf_bytes, &sm.full[stage]);
                 issued_mask |= 1u << stage;
                 issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+            };
+            auto load_image = [&](int i) {
+                bulk_load(ring + (size_t)stage * p.stage_bytes + kWBytes + kSfaBytes,
+                          p.image + (size_t)(first + i) * image_bytes, image_bytes, &sm.full[stage]);
+            };
+            auto advance = [&]() {
                 if (++stage == p.stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
+            };
+            // An Image kernel fills the ring with weights before it waits for
+            // the conversion.
+            int head = 0;
+            if constexpr (IMAGE) {
+                head = min(nst, p.stages);
+                for (int i = 0; i < head; ++i, ++stage) load_weights(i);
+                stage = 0;
+                pdl_wait();
+                for (int i = 0; i < head; ++i) {
+                    load_image(i);
+                    advance();
+                }
+            }
+            for (int i = head; i < nst; ++i) {
+                if (!mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, 0x0601)) {
+                    ok = false;
+                    break;
+                }
+                load_weights(i);
+                if constexpr (IMAGE) load_image(i);
+                advance();
             }
             if (!ok || *(volatile int*)&sm.abort) {
                 // Drain: every issued copy must land before the block exits.
@@ -385,9 +419,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 const int kb = M == Mode::Down ? (first + i) % p.k_stages : first + i;
                 const int nblk = min(4, p.kblocks - 4 * kb);
                 const uint32_t a_addr = smem_u32(ring) + (uint32_t)stage * p.stage_bytes;
-                const uint32_t sfa_addr = a_addr + kWBytes + (uint32_t)p.nb * 128;
-                const uint64_t a_desc = op_desc + (a_addr >> 4), b_desc = a_desc + (kWBytes >> 4);
-                const uint64_t sfa_desc = sf_desc + (sfa_addr >> 4), sfb_desc = sfa_desc + (kSfaBytes >> 4);
+                const uint64_t a_desc = op_desc + (a_addr >> 4), b_desc = a_desc + ((kWBytes + kSfaBytes) >> 4);
+                const uint64_t sfa_desc = sf_desc + ((a_addr + kWBytes) >> 4);
+                const uint64_t sfb_desc = sfa_desc + ((kSfaBytes + (uint32_t)p.nb * 128) >> 4);
                 const uint32_t sf_col = tmem + p.sf_col0 + (uint32_t)stage * p.sf_slot;
                 // A: K-block j at sf_col + 4 j. B: K-block j, 128-row half h at
                 // sf_col + 16 + 8 j + 4 h (two halves), or sf_col + 16 + 4 j.
@@ -429,9 +463,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         __syncwarp();
     } else {
-        // ------------------------------------------------------------ activations
         const int w = (int)warp - 2;
-        // Lane's eight elements of token t in stage i; false: none.
+        if constexpr (IMAGE) {
+            pdl_wait();
+            if (w == 0) sm.amax[lane] = (int)lane < p.T ? p.amax[lane] : 0u;
+            named_sync(1, 128);
+        } else {
+        // ------------------------------------------------------------ activations
+        // Unit u = i * tokens + t, token t in stage i, is warp u % 8's. A lane
+        // holds eight elements of it; false: the token has none in the stage.
         auto load = [&](int i, int t, uint4 (&r)[2]) -> bool {
             int kb = first + i, row = t;
             if constexpr (M == Mode::Down) {
@@ -446,66 +486,132 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (k < p.K) load_raw(static_cast<const XT*>(p.X) + (size_t)row * p.ldx + k, p.x_vec != 0, r);
             return true;
         };
-        // Largest magnitude of each token over the block's slice.
-        const int units = nst * ntok;
-        for (int u0 = w; u0 < units; u0 += 4 * kConvWarps) {
-            uint4 r[4][2];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int u = u0 + c * kConvWarps;
-                r[c][0] = r[c][1] = make_uint4(0, 0, 0, 0);
-                if (u < units) load(u / ntok, u % ntok, r[c]);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int u = u0 + c * kConvWarps;
-                float v[8];
-                widen<XT>(r[c], v);
-                const uint32_t m = __reduce_max_sync(0xffffffffu, max_bits(v));
-                if (lane == 0 && u < units) atomicMax(&sm.amax[u % ntok], m);
-            }
-        }
-        named_sync(1, 32 * kConvWarps);
-        // Stage i: this warp converts tokens t = w - i (mod 8), so one token's
-        // stages rotate over the warps. The next unit's elements are loaded
-        // before the current one's are converted.
-        int ni = 0, nt = w & 7;
-        auto settle = [&]() {
-            while (nt >= ntok && ni < nst) {
-                ++ni;
-                nt = (w - ni) & 7;
+        struct Unit {
+            int i, t;
+        };
+        const int step_i = ntok > 0 ? kConvWarps / ntok : 0, step_t = ntok > 0 ? kConvWarps % ntok : 0;
+        auto next_unit = [&](Unit& u) {
+            u.i += step_i;
+            u.t += step_t;
+            if (u.t >= ntok) {
+                u.t -= ntok;
+                ++u.i;
             }
         };
-        uint4 next[2];
-        bool next_on = false;
-        settle();
-        if (ni < nst) next_on = load(ni, nt, next);
-        int stage = 0;
-        uint32_t phase = 0;
-        for (int i = 0; i < nst; ++i) {
-            if (!mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, 0x0621)) break;
-            __syncwarp();
-            uint8_t* b_rows = ring + (size_t)stage * p.stage_bytes + kWBytes;
-            uint8_t* sfb = b_rows + (size_t)p.nb * 128 + kSfaBytes;
+        const Unit first_unit = {ntok > 0 ? w / ntok : 0, ntok > 0 ? w % ntok : 0};
+        const int units = nst * ntok;
+        auto b_rows_of = [&](int st) { return ring + (size_t)st * p.stage_bytes + kWBytes + kSfaBytes; };
+        auto in_k = [&](int i) {
             const int kb = M == Mode::Down ? (first + i) % p.k_stages : first + i;
-            const bool in_k = kb * kStageK + (int)lane * 8 < p.K;
-            for (int t = (w - i) & 7; t < ntok; t += kConvWarps) {
-                float v[8];
-                widen<XT>(next, v);
-                const bool on = next_on;
-                nt += kConvWarps;
-                settle();
-                if (ni < nst) next_on = load(ni, nt, next);
-                if (M != Mode::Down || on) convert(v, anchor_of(sm.amax[t]), t, in_k, b_rows, sfb, lane);
-                else convert_zero(t, b_rows, sfb, lane);
+            return kb * kStageK + (int)lane * 8 < p.K;
+        };
+        auto keep_max = [&](const uint4 (&r)[2], int t, bool valid) {
+            float v[8];
+            widen<XT>(r, v);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, max_bits(v));
+            if (lane == 0 && valid) atomicMax(&sm.amax[t], m);
+        };
+        // A slice of at most four units per warp that the ring holds whole
+        // stays in registers between the search for the largest magnitude
+        // and the conversion.
+        bool done = false;
+        if constexpr (M == Mode::Gemv) {
+            constexpr int kHeld = 4;
+            if (nst <= p.stages && units <= kHeld * kConvWarps) {
+                uint4 r[kHeld][2];
+                Unit u = first_unit;
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c, next_unit(u))
+                    if (u.i < nst) load(u.i, u.t, r[c]);
+                u = first_unit;
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c, next_unit(u))
+                    if (u.i < nst) keep_max(r[c], u.t, true);
+                named_sync(1, 32 * kConvWarps);
+                u = first_unit;
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c, next_unit(u)) {
+                    if (u.i >= nst) continue;
+                    float v[8];
+                    widen<XT>(r[c], v);
+                    uint8_t* b_rows = b_rows_of(u.i);
+                    convert(v, anchor_of(sm.amax[u.t]), u.t, in_k(u.i), b_rows, b_rows + (size_t)p.nb * 128, lane);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0)
+                    for (int i = 0; i < nst; ++i) mbar_arrive(&sm.full[i]);
+                done = true;
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.full[stage]);
-            if (++stage == p.stages) {
-                stage = 0;
-                phase ^= 1u;
+        }
+        if (!done) {
+            if (p.amax) {
+                if (w == 0 && (int)lane < ntok)
+                    sm.amax[lane] = p.amax[M == Mode::GateUp ? sm.slot[lane] / p.top : (int)lane];
+            } else {
+                Unit u = first_unit;
+                for (int u0 = w; u0 < units; u0 += 4 * kConvWarps) {
+                    uint4 r[4][2];
+                    int t[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c, next_unit(u)) {
+                        t[c] = u.t;
+                        r[c][0] = r[c][1] = make_uint4(0, 0, 0, 0);
+                        if (u.i < nst) load(u.i, u.t, r[c]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) keep_max(r[c], t[c], u0 + c * kConvWarps < units);
+                }
             }
+            if constexpr (M == Mode::Down) {
+                for (int i = w * 32 + (int)lane; i < kMaxStages * kMaxTokens; i += 32 * kConvWarps)
+                    (&sm.dirty[0][0])[i] = 1;
+            }
+            named_sync(1, 32 * kConvWarps);
+            // Two units' elements are on their way while one is converted.
+            Unit cur = first_unit, ahead = first_unit;
+            uint4 r0[2], r1[2];
+            bool on0 = false, on1 = false;
+            if (ahead.i < nst) on0 = load(ahead.i, ahead.t, r0);
+            next_unit(ahead);
+            if (ahead.i < nst) on1 = load(ahead.i, ahead.t, r1);
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int i = 0; i < nst; ++i) {
+                if (!mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, 0x0621)) break;
+                __syncwarp();
+                uint8_t* b_rows = b_rows_of(stage);
+                uint8_t* sfb = b_rows + (size_t)p.nb * 128;
+                const bool inside = in_k(i);
+                while (cur.i == i) {
+                    const int t = cur.t;
+                    float v[8];
+                    widen<XT>(r0, v);
+                    const bool on = on0;
+                    r0[0] = r1[0];
+                    r0[1] = r1[1];
+                    on0 = on1;
+                    next_unit(cur);
+                    next_unit(ahead);
+                    if (ahead.i < nst) on1 = load(ahead.i, ahead.t, r1);
+                    if (M != Mode::Down || on) {
+                        convert(v, anchor_of(sm.amax[t]), t, inside, b_rows, sfb, lane);
+                        if (M == Mode::Down && lane == 0) sm.dirty[stage][t] = 1;
+                    } else if (sm.dirty[stage][t]) {
+                        convert_zero(t, b_rows, sfb, lane);
+                        __syncwarp();
+                        if (lane == 0) sm.dirty[stage][t] = 0;
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.full[stage]);
+                if (++stage == p.stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+        }
         }
         __syncwarp();
         // ------------------------------------------------------------ partial sums
@@ -556,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     {
         const int rows = kTileRows / csize;
         const uint32_t base = smem_u32(ring);
-        for (int i = (int)threadIdx.x; i < ntok * rows; i += kThreads) {
+        for (int i = (int)threadIdx.x; i < ntok * rows; i += kThreads<IMAGE>) {
             const int t = i / rows, r = rank * rows + i % rows;
             const int n = tile * kTileRows + r;
             if (n >= p.N) continue;
@@ -571,7 +677,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int c = 0; c < p.split; ++c) u += ld_cluster_f32(mapa_shared(off, (uint32_t)(p.split + c)));
                 const int slot = sm.slot[t];
                 const float c = p.weights[slot] * __ldg(p.alpha2 + expert);
-                static_cast<float*>(p.Y)[(size_t)slot * p.ldy + n] = s / (1.0f + expf(-s)) * u * c;
+                const float h = s / (1.0f + expf(-s)) * u * c;
+                static_cast<float*>(p.Y)[(size_t)slot * p.ldy + n] = h;
+                atomicMax(&p.amax_out[slot / p.top], __float_as_uint(h) & 0x7FFFFFFFu);
             } else {
                 static_cast<YT*>(p.Y)[(size_t)t * p.ldy + n] = from_f32<YT>(s);
             }
@@ -583,6 +691,73 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, p.tmem_cols);
+    }
+}
+
+// ---------------------------------------------------------------- conversion ahead of the products
+// Writes the B rows and scales of every stage as the ring holds them, a block
+// per token, so that the blocks of an Image kernel fetch them with one bulk
+// copy per stage instead of each converting all of the tokens again.
+constexpr int kImageThreads = 512;
+
+template <typename XT>
+__global__ void __launch_bounds__(kImageThreads)
+    image_kernel(const XT* X, uint8_t* image, uint32_t* amax, int K, int ldx, int x_vec, int nb, uint32_t sfb_bytes) {
+    __shared__ uint32_t top[kImageThreads / 32];
+    constexpr int kWarps = kImageThreads / 32, kHeld = 4;
+    const int t = blockIdx.x, warp = (int)warp_id_uniform();
+    const uint32_t lane = lane_id();
+    const int stages = (K + kStageK - 1) / kStageK;
+    // Only now may the products start, whose weight loads wait for no one:
+    // every earlier kernel has completed.
+    pdl_wait();
+    pdl_launch_dependents();
+    const XT* x = X + (size_t)t * ldx;
+    auto load = [&](int i, uint4 (&r)[2]) {
+        const int k = i * kStageK + (int)lane * 8;
+        r[0] = r[1] = make_uint4(0, 0, 0, 0);
+        if (k < K) load_raw(x + k, x_vec != 0, r);
+    };
+    uint4 held[kHeld][2];  // the first stages stay in registers
+    uint32_t m = 0;
+    for (int i0 = warp; i0 < stages; i0 += kHeld * kWarps) {
+        uint4 r[kHeld][2];
+#pragma unroll
+        for (int c = 0; c < kHeld; ++c) {
+            r[c][0] = r[c][1] = make_uint4(0, 0, 0, 0);
+            if (i0 + c * kWarps < stages) load(i0 + c * kWarps, r[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < kHeld; ++c) {
+            float v[8];
+            widen<XT>(r[c], v);
+            m = max(m, max_bits(v));
+            if (i0 == warp) {
+                held[c][0] = r[c][0];
+                held[c][1] = r[c][1];
+            }
+        }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) top[warp] = m;
+    __syncthreads();
+    m = __reduce_max_sync(0xffffffffu, lane < kWarps ? top[lane] : 0u);
+    if (threadIdx.x == 0) amax[t] = m;
+    const int anchor = anchor_of(m);
+    const size_t bytes = (size_t)nb * 128 + sfb_bytes;
+    auto emit = [&](int i, const uint4 (&r)[2]) {
+        float v[8];
+        widen<XT>(r, v);
+        uint8_t* b_rows = image + (size_t)i * bytes;
+        convert(v, anchor, t, i * kStageK + (int)lane * 8 < K, b_rows, b_rows + (size_t)nb * 128, lane);
+    };
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c)
+        if (warp + c * kWarps < stages) emit(warp + c * kWarps, held[c]);
+    for (int i = warp + kHeld * kWarps; i < stages; i += kWarps) {
+        uint4 r[2];
+        load(i, r);
+        emit(i, r);
     }
 }
 
@@ -633,10 +808,10 @@ static int choose_split(double units, double stages, int max_split, int slots) {
     return best;
 }
 
-template <Mode M, typename XT, typename YT>
+template <Mode M, typename XT, typename YT, bool IMAGE = false>
 static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const Params& p, size_t smem, int clusters,
                          cudaStream_t stream) {
-    auto kernel = stream_kernel<M, XT, YT>;
+    auto kernel = stream_kernel<M, XT, YT, IMAGE>;
     static thread_local uint64_t configured = 0;  // bit per device
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GPLK_STATUS_CUDA_ERROR;
@@ -648,7 +823,7 @@ static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const P
     const int csize = (M == Mode::GateUp ? 2 : 1) * p.split;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * csize));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kThreads<IMAGE>);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -668,12 +843,45 @@ static int encode_weights(CUtensorMap* map, const uint8_t* W, uint64_t rows, int
     return encode_tmap_2d_u8(map, W, (uint64_t)K / 2, rows, (uint64_t)K / 2, 128, kTileRows);
 }
 
+// Whether the activations are converted once, by a kernel of their own, or by
+// every block for itself.
+static bool use_image(int T, int K) { return (long long)T * K > 32768; }
+
+// Workspace of the converted activations: the stages' images, then the
+// tokens' largest magnitudes.
+static size_t image_bytes(const Params& p) { return (size_t)p.k_stages * ((size_t)p.nb * 128 + p.sfb_bytes); }
+
+template <typename XT>
+static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* workspace, cudaStream_t stream) {
+    if (!workspace) return launch_stream<Mode::Gemv, XT, XT>(tm, tm, p, s.smem, p.tiles, stream);
+    uint8_t* image = static_cast<uint8_t*>(workspace);
+    uint32_t* amax = reinterpret_cast<uint32_t*>(image + image_bytes(p));
+    const int st = launch_status(launch_pdl(image_kernel<XT>, dim3((unsigned)p.T), dim3(kImageThreads), 0, stream,
+                                            static_cast<const XT*>(p.X), image, amax, p.K, p.ldx, p.x_vec, p.nb,
+                                            p.sfb_bytes));
+    if (st != GPLK_STATUS_OK) return st;
+    p.image = image;
+    p.amax = amax;
+    return launch_stream<Mode::Gemv, XT, XT, true>(tm, tm, p, s.smem, p.tiles, stream);
+}
+
 }  // namespace fewtok
 }  // namespace gplk
 
+extern "C" size_t gplk_gemv_nvfp4_workspace_bytes(int T, int N, int K) {
+    using namespace gplk::fewtok;
+    if (T <= 0 || T > kMaxTokens || N <= 0 || K <= 0 || K % 64 != 0 || !use_image(T, K)) return 0;
+    Params p;
+    memset(&p, 0, sizeof(p));
+    p.T = T;
+    p.k_stages = (K + kStageK - 1) / kStageK;
+    set_shape(p);
+    return image_bytes(p) + sizeof(uint32_t) * kMaxTokens;
+}
+
 extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* SF, void* Y, const void* R, int T,
                                int N, int K, int ldx, int ldy, int ldr, const float* alpha, int dtype,
-                               cudaStream_t stream) {
+                               void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     using namespace gplk;
     using namespace gplk::fewtok;
     if (T < 0 || N < 0 || K < 0 || T > kMaxTokens) return GPLK_STATUS_BAD_ARG;
@@ -682,7 +890,8 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     if (K == 0 || K % 64 != 0 || ldx < K || ldy < N || (R && ldr < N)) return GPLK_STATUS_BAD_ARG;
     if (N > INT_MAX / 8) return GPLK_STATUS_BAD_ARG;  // N / 128 tiles of 8 slices fit a grid
     if (!X || !W || !SF || !Y || !alpha) return GPLK_STATUS_BAD_ARG;
-    if (!aligned16(W) || !aligned16(SF) || !aligned(X, 2) || !aligned(Y, 2) || !aligned(R, 2) || !aligned(alpha, 4))
+    if (!aligned16(W) || !aligned16(SF) || !aligned(X, 2) || !aligned(Y, 2) || !aligned(R, 2) || !aligned(alpha, 4) ||
+        !aligned16(workspace))
         return GPLK_STATUS_BAD_ARG;
     DeviceInfo d;
     int st = require_sm100(&d);
@@ -710,7 +919,8 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     CUtensorMap tm;
     st = encode_weights(&tm, W, (uint64_t)N, K);
     if (st != GPLK_STATUS_OK) return st;
-    return dtype == GPLK_DTYPE_BF16
-               ? launch_stream<Mode::Gemv, __nv_bfloat16, __nv_bfloat16>(tm, tm, p, s.smem, p.tiles, stream)
-               : launch_stream<Mode::Gemv, __half, __half>(tm, tm, p, s.smem, p.tiles, stream);
+    const size_t need = gplk_gemv_nvfp4_workspace_bytes(T, N, K);
+    void* ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;
+    return dtype == GPLK_DTYPE_BF16 ? launch_gemv<__nv_bfloat16>(p, s, tm, ws, stream)
+                                    : launch_gemv<__half>(p, s, tm, ws, stream);
 }

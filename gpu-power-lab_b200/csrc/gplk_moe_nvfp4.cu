@@ -27,14 +27,15 @@ using namespace fewtok;
 
 // Workspace: every part starts on a 256-byte boundary.
 struct Layout {
-    size_t route, logits, ids, weights, h, total;
+    size_t route, amax, logits, ids, weights, h, total;
 };
 
 static Layout layout(int T, int E, int top, int F) {
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     Layout l;
     l.route = 0;
-    l.logits = up(sizeof(Route));
+    l.amax = up(sizeof(Route));
+    l.logits = l.amax + up(2 * kMaxTokens * sizeof(uint32_t));
     l.ids = l.logits + up((size_t)T * E * 4);
     l.weights = l.ids + up((size_t)T * top * 4);
     l.h = l.weights + up((size_t)T * top * 4);
@@ -49,31 +50,72 @@ struct RouteParams {
     int* ids;
     float* weights;
     Route* route;
+    uint32_t* amax;  // bits of the largest magnitude of x, then of the weighted h, by token
     int T, E, top, D, ldx, renormalise;
+    int vec;  // rows of x and of the router are 16-byte aligned
 };
 
-// Router product: one block per expert and 8 tokens.
-template <typename XT>
-__global__ void __launch_bounds__(128) router_kernel(const RouteParams p) {
-    const int e = blockIdx.x, t0 = blockIdx.y * 8;
-    const int nx = min(8, p.T - t0);
+// Router product: a block per expert and up to 8 tokens, whose four warps
+// share out K. One more block per 8 tokens finds the tokens' largest
+// magnitudes, which anchor the conversion of x, and clears those of h.
+constexpr int kRouterThreads = 128;
+
+template <typename XT, int NX>
+__global__ void __launch_bounds__(kRouterThreads) router_kernel(const RouteParams p) {
+    const int e = blockIdx.x, t0 = blockIdx.y * NX;
+    const int nx = min(NX, p.T - t0);
+    const int warp = (int)warp_id_uniform();
+    const int lane = (int)lane_id();
     pdl_wait();
     pdl_launch_dependents();
-    const XT* r = static_cast<const XT*>(p.router) + (size_t)e * p.D;
     const XT* x = static_cast<const XT*>(p.x) + (size_t)t0 * p.ldx;
-    float acc[8] = {};
-    for (int k = threadIdx.x; k < p.D; k += 128) {
-        const float w = static_cast<float>(r[k]);
+    const bool vec = p.vec != 0;
+    if (e == p.E) {
+        for (int t = warp; t < nx; t += kRouterThreads / 32) {
+            uint32_t m = 0;
+            for (int k0 = lane * 8; k0 < p.D; k0 += 4 * 256) {
+                uint4 r[4][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < nx) acc[i] = fmaf(w, static_cast<float>(x[(size_t)i * p.ldx + k]), acc[i]);
+                for (int c = 0; c < 4; ++c) {
+                    r[c][0] = make_uint4(0, 0, 0, 0);
+                    if (k0 + 256 * c < p.D) load_raw(x + (size_t)t * p.ldx + k0 + 256 * c, vec, r[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float v[8];
+                    widen<XT>(r[c], v);
+                    m = max(m, max_bits(v));
+                }
+            }
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) p.amax[t0 + t] = m;
+            if (lane == 1) p.amax[kMaxTokens + t0 + t] = 0;
+        }
+        return;
     }
-    __shared__ float part[4][8];
+    const XT* r = static_cast<const XT*>(p.router) + (size_t)e * p.D;
+    float acc[NX] = {};
+    for (int k = (int)threadIdx.x * 8; k < p.D; k += kRouterThreads * 8) {
+        uint4 wr[2], xr[NX][2];
+        load_raw(r + k, vec, wr);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < NX; ++i) load_raw(x + (size_t)min(i, nx - 1) * p.ldx + k, vec, xr[i]);
+        float w[8];
+        widen<XT>(wr, w);
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+            float v[8];
+            widen<XT>(xr[i], v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[i] = fmaf(w[j], v[j], acc[i]);
+        }
+    }
+    __shared__ float part[4][NX];
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-        if (lane_id() == 0) part[threadIdx.x / 32][i] = acc[i];
+        if (lane == 0) part[warp][i] = acc[i];
     }
     __syncthreads();
     if (threadIdx.x < (unsigned)nx)
@@ -195,6 +237,8 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     r.ids = c.ids ? c.ids : reinterpret_cast<int*>(ws + l.ids);
     r.weights = c.weights ? c.weights : reinterpret_cast<float*>(ws + l.weights);
     r.route = reinterpret_cast<Route*>(ws + l.route);
+    r.amax = reinterpret_cast<uint32_t*>(ws + l.amax);
+    r.vec = aligned16(c.router) && aligned16(c.x) && (c.T == 1 || c.ldx % 8 == 0);
     r.T = c.T;
     r.E = c.E;
     r.top = c.top;
@@ -221,6 +265,8 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     g.Y = ws + l.h;
     g.route = r.route;
     g.weights = r.weights;
+    g.amax = r.amax;
+    g.amax_out = r.amax + kMaxTokens;
     g.T = c.T;
     g.N = c.F;
     g.K = c.D;
@@ -234,6 +280,7 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     const Shape gs = set_shape(g);
     Params o = g;
     o.X = g.Y;
+    o.amax = g.amax_out;
     o.sf0 = c.sf_down;
     o.Y = c.y;
     o.N = c.D;
@@ -255,7 +302,10 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     if (st == GPLK_STATUS_OK) st = encode_weights(&td, c.down, (uint64_t)c.E * c.D, c.F);
     if (st != GPLK_STATUS_OK) return st;
 
-    st = launch_status(launch_pdl(router_kernel<XT>, dim3(c.E, (c.T + 7) / 8), dim3(128), 0, stream, r));
+    auto router = [&](auto kernel, int nx) {
+        return launch_status(launch_pdl(kernel, dim3(c.E + 1, (c.T + nx - 1) / nx), dim3(kRouterThreads), 0, stream, r));
+    };
+    st = c.T == 1 ? router(router_kernel<XT, 1>, 1) : c.T <= 4 ? router(router_kernel<XT, 4>, 4) : router(router_kernel<XT, 8>, 8);
     if (st == GPLK_STATUS_OK)
         st = launch_status(launch_pdl(route_kernel, dim3(1), dim3(32 * kMaxTokens), 0, stream, r));
     if (st == GPLK_STATUS_OK)

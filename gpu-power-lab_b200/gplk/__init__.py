@@ -8,6 +8,7 @@ raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent.parent
@@ -108,7 +109,9 @@ def lib() -> ctypes.CDLL:
     L.gplk_selftest_wait_timeout.restype = _i
     L.gplk_selftest_wait_timeout.argtypes = [ctypes.c_ulonglong, _p, _p]
     L.gplk_gemv_nvfp4.restype = _i
-    L.gplk_gemv_nvfp4.argtypes = [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _i, _p]
+    L.gplk_gemv_nvfp4.argtypes = [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _i, _p, _sz, _p]
+    L.gplk_gemv_nvfp4_workspace_bytes.restype = _sz
+    L.gplk_gemv_nvfp4_workspace_bytes.argtypes = [_i, _i, _i]
     L.gplk_moe_nvfp4.restype = _i
     L.gplk_moe_nvfp4.argtypes = [ctypes.POINTER(MoeCfg), _p]
     L.gplk_moe_nvfp4_workspace_bytes.restype = _sz
@@ -244,62 +247,95 @@ def gemm_nvfp4_tn(A, B, SFA, SFB, D, K: int, alpha, stream=None) -> None:
 MAX_TOKENS = 32
 
 
+_act_dtypes: dict = {}
+
+
 def _act_dtype(t) -> int:
     """GPLK_DTYPE_* of a tensor of activations (-1: neither)."""
-    import torch
+    if not _act_dtypes:
+        import torch
 
-    return 0 if t.dtype == torch.bfloat16 else 1 if t.dtype == torch.float16 else -1
+        _act_dtypes.update({torch.bfloat16: 0, torch.float16: 1})
+    return _act_dtypes.get(t.dtype, -1)
 
 
-def _need(fn: str, *conds) -> None:
+def _need(fn: str, cond: bool) -> None:
     """The checks a pointer cannot carry: shapes, types, devices."""
-    if not all(conds):
+    if not cond:
         raise GplkError(fn, 1)
 
 
-def _rows(t) -> tuple[int, int, int]:
-    """(rows, columns, leading dimension) of a 2-D tensor with contiguous rows."""
-    r, c = t.shape
-    return r, c, t.stride(0) if r > 1 else max(c, 1)
-
-
-def _on(dev, fn: str, *tensors):
-    """Raises unless every tensor is on CUDA device `dev`; a context in which
-    that device is the current one."""
-    import contextlib
-
+def _fresh(nbytes: int, stream, device):
+    """A block of the caching allocator in the stream's own pool: calls that
+    overlap, and captured graphs, never share it."""
     import torch
 
-    _need(fn, dev.type == "cuda", *[t.device == dev for t in tensors])
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
-def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, stream=None) -> None:
+def _launch_on(index: int, stream, call) -> None:
+    """call(raw stream) with CUDA device `index` the current one. These calls
+    take microseconds: torch.cuda.current_stream() alone would take three."""
+    import torch
+
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _launch_on(index, stream, call)
+    if stream is None:
+        return call(torch._C._cuda_getCurrentRawStream(index))
+    if stream.device_index != index:
+        raise GplkError("stream of another device", 1)
+    call(stream.cuda_stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def gemv_nvfp4_workspace_bytes(T: int, N: int, K: int) -> int:
+    return int(lib().gplk_gemv_nvfp4_workspace_bytes(T, N, K))
+
+
+def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None) -> None:
     """Y = alpha * X @ w.T (+ residual) for up to 32 rows of activations.
     X: (T, K), Y and residual: (T, N), all bf16 or all f16, rows contiguous and
     any distance apart; residual may be Y. W: (N, K/2) packed E2M1 and SF its
     scale bytes, as gemm_nvfp4_tn and operands.quantize_nvfp4 have them;
-    alpha: 1-element float32 tensor, the matrix scale."""
+    alpha: 1-element float32 tensor, the matrix scale. workspace: "auto" (from
+    torch's allocator, on the call's stream), None (none: slower at most sizes),
+    or a uint8 CUDA tensor that no overlapping call uses."""
     import torch
 
-    fn, dt = "gplk_gemv_nvfp4", _act_dtype(X)
-    _need(fn, X.dim() == 2, Y.dim() == 2, W.dim() == 2)
-    T, K, ldx = _rows(X)
-    T2, N, ldy = _rows(Y)
-    _need(fn, dt >= 0, Y.dtype == X.dtype, T2 == T, W.shape[0] == N, W.shape[1] * 2 == K, W.dtype == torch.uint8,
-          W.is_contiguous(), SF.dtype == torch.uint8, SF.is_contiguous(), alpha.dtype == torch.float32,
-          alpha.numel() == 1, K < 2 or X.stride(1) == 1, N < 2 or Y.stride(1) == 1,
-          SF.numel() >= nvfp4_sf_bytes(N, K))
-    ldr, rp = 0, None
+    fn, L = "gplk_gemv_nvfp4", lib()
+    dt, u8, dev = _act_dtype(X), torch.uint8, X.get_device()
+    _need(fn, dt >= 0 and dev >= 0 and X.dim() == Y.dim() == W.dim() == 2)
+    (T, K), (T2, N), (rows, row_bytes) = X.shape, Y.shape, W.shape
+    (ldx, cx), (ldy, cy) = X.stride(), Y.stride()
+    _need(fn, T2 == T and rows == N and row_bytes * 2 == K and (cx == 1 or K < 2) and (cy == 1 or N < 2)
+          and Y.dtype == X.dtype and W.dtype == u8 and SF.dtype == u8 and alpha.dtype == torch.float32
+          and W.is_contiguous() and SF.is_contiguous() and alpha.numel() == 1
+          and SF.numel() >= -(-N // 128) * -(-K // 64) * 512
+          and W.get_device() == SF.get_device() == Y.get_device() == alpha.get_device() == dev)
+    ldr, rp, wp, wb = 0, None, None, 0
     if residual is not None:
-        _need(fn, residual.shape == Y.shape, residual.dtype == X.dtype, N < 2 or residual.stride(1) == 1,
-              residual.device == X.device)
-        ldr, rp = _rows(residual)[2], residual.data_ptr()
-    with _on(X.device, fn, W, SF, Y, alpha):
-        _check(fn, lib().gplk_gemv_nvfp4(_ptr(X), _ptr(W), _ptr(SF), _ptr(Y), rp, T, N, K, ldx, ldy, ldr, _ptr(alpha),
-                                         dt, _stream(stream)))
+        ldr, cr = residual.stride() if residual.dim() == 2 else (0, 0)
+        _need(fn, residual.shape == Y.shape and residual.dtype == X.dtype and (cr == 1 or N < 2)
+              and residual.get_device() == dev)
+        rp = residual.data_ptr()
+    if T < 2:  # one row has no distance to the next
+        ldx, ldy, ldr = K, N, N
+    if isinstance(workspace, str):
+        need = gemv_nvfp4_workspace_bytes(T, N, K)
+        workspace = _fresh(need, stream, X.device) if need else None
+    if workspace is not None:
+        _need(fn, workspace.get_device() == dev and workspace.is_contiguous())
+        wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _launch_on(dev, stream, lambda s: _check(fn, L.gplk_gemv_nvfp4(
+        X.data_ptr(), W.data_ptr(), SF.data_ptr(), Y.data_ptr(), rp, T, N, K, ldx, ldy, ldr, alpha.data_ptr(), dt, wp,
+        wb, s)))
 
 
+@functools.lru_cache(maxsize=4096)
 def moe_nvfp4_workspace_bytes(T: int, E: int, top: int, D: int, F: int) -> int:
     return int(lib().gplk_moe_nvfp4_workspace_bytes(T, E, top, D, F))
 
@@ -317,33 +353,34 @@ def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = Tr
     call uses."""
     import torch
 
-    fn, dt = "gplk_moe_nvfp4", _act_dtype(X)
-    _need(fn, X.dim() == 2, Y.dim() == 2, router.dim() == 2, ids.dim() == 2)
-    T, D, ldx = _rows(X)
-    T2, D2, ldy = _rows(Y)
+    fn, L = "gplk_moe_nvfp4", lib()
+    dt, u8, f32, dev = _act_dtype(X), torch.uint8, torch.float32, X.get_device()
+    (gw, gs, ga), (uw, us, ua), (dw, ds, da) = gate, up, down
+    _need(fn, dt >= 0 and dev >= 0 and X.dim() == Y.dim() == router.dim() == ids.dim() == 2 and gw.dim() == 3)
+    T, D = X.shape
     E, top = router.shape[0], ids.shape[1]
-    F = gate[0].shape[1] if gate[0].dim() == 3 else 0
-    _need(fn, dt >= 0, Y.dtype == X.dtype, (T2, D2) == (T, D), X.stride(1) == 1, Y.stride(1) == 1,
-          router.shape[1] == D, router.dtype == X.dtype, router.is_contiguous(), ids.dtype == torch.int32,
-          ids.shape[0] == T, ids.is_contiguous(), weights.shape == ids.shape, weights.dtype == torch.float32,
-          weights.is_contiguous())
-    for (w, sf, alpha), rows, k in ((gate, F, D), (up, F, D), (down, D, F)):
-        _need(fn, tuple(w.shape) == (E, rows, k // 2), w.dtype == torch.uint8, w.is_contiguous(),
-              sf.dtype == torch.uint8, sf.is_contiguous(), sf.numel() == E * nvfp4_sf_bytes(rows, k),
-              alpha.dtype == torch.float32, alpha.is_contiguous(), alpha.numel() == E)
-    with _on(X.device, fn, router, *gate, *up, *down, Y, ids, weights):
-        if isinstance(workspace, str):
-            # A fresh block of the caching allocator, in the stream's own pool:
-            # concurrent calls and captured graphs never share it.
-            with torch.cuda.stream(stream) if stream is not None else torch.cuda.stream(None):
-                workspace = torch.empty(max(1, moe_nvfp4_workspace_bytes(T, E, top, D, F)), dtype=torch.uint8,
-                                        device=X.device)
-        _need(fn, workspace.device == X.device, workspace.is_contiguous())
-        c = MoeCfg(_ptr(X), _ptr(router), _ptr(gate[0]), _ptr(up[0]), _ptr(down[0]), _ptr(gate[1]), _ptr(up[1]),
-                   _ptr(down[1]), _ptr(gate[2]), _ptr(up[2]), _ptr(down[2]), _ptr(Y), _ptr(ids), _ptr(weights),
-                   _ptr(workspace), workspace.numel() * workspace.element_size(), T, E, top, D, F, ldx, ldy,
-                   int(bool(renormalise)), dt)
-        _check(fn, lib().gplk_moe_nvfp4(ctypes.byref(c), _stream(stream)))
+    F = gw.shape[1]
+    (ldx, cx), (ldy, cy) = X.stride(), Y.stride()
+    _need(fn, Y.shape == X.shape and Y.dtype == X.dtype and cx == 1 and cy == 1 and router.shape[1] == D
+          and router.dtype == X.dtype and router.is_contiguous() and ids.dtype == torch.int32 and ids.shape[0] == T
+          and ids.is_contiguous() and weights.shape == ids.shape and weights.dtype == f32 and weights.is_contiguous()
+          and router.get_device() == Y.get_device() == ids.get_device() == weights.get_device() == dev)
+    up_shape, up_sf = (E, F, D // 2), E * -(-F // 128) * -(-D // 64) * 512
+    for w, sf, al, shape, n in ((gw, gs, ga, up_shape, up_sf), (uw, us, ua, up_shape, up_sf),
+                                (dw, ds, da, (E, D, F // 2), E * -(-D // 128) * -(-F // 64) * 512)):
+        _need(fn, w.shape == shape and w.dtype == u8 and sf.dtype == u8 and al.dtype == f32 and w.is_contiguous()
+              and sf.is_contiguous() and al.is_contiguous() and sf.numel() == n and al.numel() == E
+              and w.get_device() == sf.get_device() == al.get_device() == dev)
+    if T < 2:
+        ldx = ldy = D
+    if isinstance(workspace, str):
+        workspace = _fresh(max(1, moe_nvfp4_workspace_bytes(T, E, top, D, F)), stream, X.device)
+    _need(fn, workspace.get_device() == dev and workspace.is_contiguous())
+    c = MoeCfg(X.data_ptr(), router.data_ptr(), gw.data_ptr(), uw.data_ptr(), dw.data_ptr(), gs.data_ptr(),
+               us.data_ptr(), ds.data_ptr(), ga.data_ptr(), ua.data_ptr(), da.data_ptr(), Y.data_ptr(),
+               ids.data_ptr(), weights.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+               T, E, top, D, F, ldx, ldy, bool(renormalise), dt)
+    _launch_on(dev, stream, lambda s: _check(fn, L.gplk_moe_nvfp4(ctypes.byref(c), s)))
 
 
 # ------------------------------------------------------------ dense tensor-core GEMMs

@@ -154,7 +154,14 @@ size_t gplk_nvfp4_sf_bytes(int rows, int k);
  * inputs give equal bits. */
 int gplk_gemv_nvfp4(const void *X, const uint8_t *W, const uint8_t *SF, void *Y, const void *R, int T,
                     int N, int K, int ldx, int ldy, int ldr, const float *alpha, int dtype,
-                    cudaStream_t stream);
+                    void *workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* Bytes of workspace (16-byte aligned, any content) in which
+ * gplk_gemv_nvfp4 converts the activations once; 0 for sizes at which every
+ * block converts them for itself. With no workspace, or a smaller one, every
+ * block does so at any size, and the call takes longer. One workspace serves
+ * one call at a time. */
+size_t gplk_gemv_nvfp4_workspace_bytes(int T, int N, int K);
 
 /* A mixture-of-experts layer for T tokens (0 <= T <= 32):
  *   logits = router x;  p = softmax(logits) over the E experts;  the `top`
