@@ -66,7 +66,11 @@ constexpr uint32_t kSfaBytes = 4 * 512;         // scales of a stage
 constexpr int kMaxStages = 8;
 constexpr uint32_t kDigitBias = 4u * (1u + 8u + 64u + 512u + 4096u);
 
-enum class Mode { Gemv, GateUp, Down };
+// Gemv: all tokens against one matrix. GateUp: a chosen expert's tokens against
+// its gate and up matrices. Down: all tokens against every chosen expert's down
+// matrix, accumulated over the experts. DownPart: a chosen expert's tokens
+// against its down matrix.
+enum class Mode { Gemv, GateUp, Down, DownPart };
 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
@@ -77,8 +81,7 @@ __device__ __forceinline__ T from_f32(float v) {
 // Written by the route kernel into the layer's workspace.
 struct Route {
     int n_active;
-    int active[kMaxExperts];                    // chosen experts, ascending
-    int count[kMaxExperts];                     // tokens of active expert a
+    int head[kMaxExperts];                      // active expert a: its index | its tokens << 16, ascending; then 0
     int16_t list[kMaxExperts][kMaxTokens];      // their slots (token * top + rank), ascending
     int16_t slot[kMaxExperts][kMaxTokens];      // slot of token t with active expert a, or -1
 };
@@ -104,11 +107,33 @@ struct Params {
     int k_stages;        // stages of one matrix row
     int kblocks;         // K / 64
     int split;           // slices of K
-    int nb;              // accumulator columns for T tokens
-    int stages;          // ring depth
-    uint32_t stage_bytes, sfb_bytes;
-    uint32_t tmem_cols, sf_col0, sf_slot;
+    uint32_t ring_bytes; // shared memory of the ring
+    uint32_t tmem_cols;
 };
+
+// Ring and TMEM layout for a block's tokens. A stage holds codes | their
+// scales | B rows | B scales; TMEM the accumulator, then a slot of scale
+// columns per stage.
+struct Geometry {
+    int nb;      // accumulator columns
+    int stages;  // ring depth
+    uint32_t stage_bytes, sfb_bytes;
+    uint32_t sf_col0, sf_slot;
+};
+
+__host__ __device__ __forceinline__ Geometry geometry(int ntok, uint32_t ring_bytes, uint32_t tmem_cols) {
+    Geometry g;
+    g.nb = (kPlanes * ntok + 7) & ~7;
+    const bool wide = g.nb > 128;  // a second 128 rows of B scales
+    g.sfb_bytes = wide ? 4096 : 2048;
+    g.stage_bytes = kWBytes + kSfaBytes + (uint32_t)g.nb * 128 + g.sfb_bytes;
+    g.sf_col0 = ((uint32_t)g.nb + 15) & ~15u;
+    g.sf_slot = wide ? 48 : 32;
+    const uint32_t fit = ring_bytes / g.stage_bytes, slots = (tmem_cols - g.sf_col0) / g.sf_slot;
+    g.stages = (int)(fit < slots ? fit : slots);
+    if (g.stages > kMaxStages) g.stages = kMaxStages;
+    return g;
+}
 
 struct Control {
     uint64_t full[kMaxStages];
@@ -263,8 +288,6 @@ __device__ __forceinline__ void convert_zero(int t, uint8_t* b_rows, uint8_t* sf
     }
 }
 
-__device__ __forceinline__ uint32_t pad8(uint32_t n) { return (n + 7) & ~7u; }
-
 template <bool IMAGE>
 constexpr int kThreads = IMAGE ? 64 + 128 : 64 + 32 * kConvWarps;
 
@@ -273,7 +296,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     stream_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1, const Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    Control& sm = *reinterpret_cast<Control*>(ring + (size_t)p.stages * p.stage_bytes);
+    Control& sm = *reinterpret_cast<Control*>(ring + p.ring_bytes);
     const uint32_t warp = warp_id_uniform();
     const uint32_t lane = lane_id();
     const int rank = (int)cluster_ctarank();
@@ -281,7 +304,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     const int cid = (int)blockIdx.x / csize;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.stages; ++i) {
+        for (int i = 0; i < kMaxStages; ++i) {
             mbar_init(&sm.full[i], IMAGE ? 1 : 1 + kConvWarps);
             mbar_init(&sm.empty[i], 1);
         }
@@ -306,27 +329,25 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     pdl_launch_dependents();
 
     // This block's rows, tokens and stages.
+    constexpr bool kPerExpert = M == Mode::GateUp || M == Mode::DownPart;
     int tile = cid, slice = rank, expert = 0, ntok = p.T, total = p.k_stages;
     bool second = false;  // GateUp: the `up` half of the cluster
-    if constexpr (M == Mode::GateUp) {
+    if constexpr (kPerExpert) {
         const int a = cid / p.tiles;
         tile = cid % p.tiles;
-        second = rank >= p.split;
+        second = M == Mode::GateUp && rank >= p.split;
         slice = second ? rank - p.split : rank;
-        if (a < p.route->n_active) {
-            expert = p.route->active[a];
-            ntok = p.route->count[a];
-            if (threadIdx.x < (unsigned)ntok) sm.slot[threadIdx.x] = p.route->list[a][threadIdx.x];
-        } else {
-            ntok = 0;
-            total = 0;
-        }
+        const int head = p.route->head[a];
+        if (threadIdx.x < kMaxTokens) sm.slot[threadIdx.x] = p.route->list[a][threadIdx.x];
+        expert = head & 0xFFFF;
+        ntok = head >> 16;
+        if (ntok == 0) total = 0;
     } else if constexpr (M == Mode::Down) {
         total = p.route->n_active * p.k_stages;
     }
     const int first = (int)((long long)total * slice / p.split);
     const int nst = (int)((long long)total * (slice + 1) / p.split) - first;
-    const uint32_t nb = M == Mode::GateUp ? pad8((uint32_t)(kPlanes * ntok)) : (uint32_t)p.nb;
+    const Geometry g = geometry(ntok, p.ring_bytes, p.tmem_cols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -340,15 +361,15 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             bool ok = true;
             const CUtensorMap* tm = second ? &tm1 : &tm0;
             const size_t sf_matrix = (size_t)p.tiles * (size_t)p.kblocks * 512;
-            const uint32_t image_bytes = IMAGE ? (uint32_t)p.nb * 128 + p.sfb_bytes : 0u;
+            const uint32_t image_bytes = IMAGE ? (uint32_t)g.nb * 128 + g.sfb_bytes : 0u;
             auto load_weights = [&](int i) {
                 int kb = first + i;
                 if constexpr (M == Mode::Down) {
-                    expert = p.route->active[kb / p.k_stages];
+                    expert = p.route->head[kb / p.k_stages] & 0xFFFF;
                     kb %= p.k_stages;
                 }
                 const uint32_t sf_bytes = 512u * (uint32_t)min(4, p.kblocks - 4 * kb);
-                uint8_t* st = ring + (size_t)stage * p.stage_bytes;
+                uint8_t* st = ring + (size_t)stage * g.stage_bytes;
                 const uint8_t* sf = (second ? p.sf1 : p.sf0) + (size_t)expert * sf_matrix +
                                     ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
                 mbar_arrive_expect_tx(&sm.full[stage], kWBytes + sf_bytes + image_bytes);
@@ -358,11 +379,11 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
             };
             auto load_image = [&](int i) {
-                bulk_load(ring + (size_t)stage * p.stage_bytes + kWBytes + kSfaBytes,
+                bulk_load(ring + (size_t)stage * g.stage_bytes + kWBytes + kSfaBytes,
                           p.image + (size_t)(first + i) * image_bytes, image_bytes, &sm.full[stage]);
             };
             auto advance = [&]() {
-                if (++stage == p.stages) {
+                if (++stage == g.stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
@@ -371,7 +392,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             // the conversion.
             int head = 0;
             if constexpr (IMAGE) {
-                head = min(nst, p.stages);
+                head = min(nst, g.stages);
                 for (int i = 0; i < head; ++i, ++stage) load_weights(i);
                 stage = 0;
                 pdl_wait();
@@ -392,7 +413,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             if (!ok || *(volatile int*)&sm.abort) {
                 // Drain: every issued copy must land before the block exits.
                 int dummy = 0;
-                for (int s2 = 0; s2 < p.stages; ++s2)
+                for (int s2 = 0; s2 < g.stages; ++s2)
                     if (issued_mask & (1u << s2))
                         mbar_wait(&sm.full[s2], (issued_parity >> s2) & 1u, &dummy, 0x0602, 100000000ull);
             }
@@ -403,8 +424,8 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         // The whole warp runs the loop, so addresses and descriptors stay in
         // uniform registers, and one elected lane issues.
         if (nst > 0) {
-            const uint32_t idesc = idesc_nvf4(kTileRows, (int)nb);
-            const uint32_t bstep = p.sf_slot > 32 ? 8u : 4u;
+            const uint32_t idesc = idesc_nvf4(kTileRows, g.nb);
+            const uint32_t bstep = g.sf_slot > 32 ? 8u : 4u;
             const uint64_t op_desc = desc_kmajor_sw128(0), sf_desc = smem_desc(0, 0, 128, 0);
             int stage = 0;
             uint32_t phase = 0;
@@ -418,11 +439,11 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 tc_fence_after();
                 const int kb = M == Mode::Down ? (first + i) % p.k_stages : first + i;
                 const int nblk = min(4, p.kblocks - 4 * kb);
-                const uint32_t a_addr = smem_u32(ring) + (uint32_t)stage * p.stage_bytes;
+                const uint32_t a_addr = smem_u32(ring) + (uint32_t)stage * g.stage_bytes;
                 const uint64_t a_desc = op_desc + (a_addr >> 4), b_desc = a_desc + ((kWBytes + kSfaBytes) >> 4);
                 const uint64_t sfa_desc = sf_desc + ((a_addr + kWBytes) >> 4);
-                const uint64_t sfb_desc = sfa_desc + ((kSfaBytes + (uint32_t)p.nb * 128) >> 4);
-                const uint32_t sf_col = tmem + p.sf_col0 + (uint32_t)stage * p.sf_slot;
+                const uint64_t sfb_desc = sfa_desc + ((kSfaBytes + (uint32_t)g.nb * 128) >> 4);
+                const uint32_t sf_col = tmem + g.sf_col0 + (uint32_t)stage * g.sf_slot;
                 // A: K-block j at sf_col + 4 j. B: K-block j, 128-row half h at
                 // sf_col + 16 + 8 j + 4 h (two halves), or sf_col + 16 + 4 j.
                 auto scales = [&](int j) {
@@ -447,7 +468,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     tc_commit(&sm.empty[stage]);
                 }
                 __syncwarp();
-                if (++stage == p.stages) {
+                if (++stage == g.stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
@@ -479,6 +500,8 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 kb %= p.k_stages;
             } else if constexpr (M == Mode::GateUp) {
                 row = sm.slot[t] / p.top;
+            } else if constexpr (M == Mode::DownPart) {
+                row = sm.slot[t];
             }
             const int k = kb * kStageK + (int)lane * 8;
             r[0] = r[1] = make_uint4(0, 0, 0, 0);
@@ -500,7 +523,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         };
         const Unit first_unit = {ntok > 0 ? w / ntok : 0, ntok > 0 ? w % ntok : 0};
         const int units = nst * ntok;
-        auto b_rows_of = [&](int st) { return ring + (size_t)st * p.stage_bytes + kWBytes + kSfaBytes; };
+        auto b_rows_of = [&](int st) { return ring + (size_t)st * g.stage_bytes + kWBytes + kSfaBytes; };
         auto in_k = [&](int i) {
             const int kb = M == Mode::Down ? (first + i) % p.k_stages : first + i;
             return kb * kStageK + (int)lane * 8 < p.K;
@@ -517,7 +540,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         bool done = false;
         if constexpr (M == Mode::Gemv) {
             constexpr int kHeld = 4;
-            if (nst <= p.stages && units <= kHeld * kConvWarps) {
+            if (nst <= g.stages && units <= kHeld * kConvWarps) {
                 uint4 r[kHeld][2];
                 Unit u = first_unit;
 #pragma unroll
@@ -535,7 +558,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     float v[8];
                     widen<XT>(r[c], v);
                     uint8_t* b_rows = b_rows_of(u.i);
-                    convert(v, anchor_of(sm.amax[u.t]), u.t, in_k(u.i), b_rows, b_rows + (size_t)p.nb * 128, lane);
+                    convert(v, anchor_of(sm.amax[u.t]), u.t, in_k(u.i), b_rows, b_rows + (size_t)g.nb * 128, lane);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -547,7 +570,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         if (!done) {
             if (p.amax) {
                 if (w == 0 && (int)lane < ntok)
-                    sm.amax[lane] = p.amax[M == Mode::GateUp ? sm.slot[lane] / p.top : (int)lane];
+                    sm.amax[lane] = p.amax[kPerExpert ? sm.slot[lane] / p.top : (int)lane];
             } else {
                 Unit u = first_unit;
                 for (int u0 = w; u0 < units; u0 += 4 * kConvWarps) {
@@ -581,7 +604,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 if (!mbar_wait(&sm.empty[stage], phase ^ 1u, &sm.abort, 0x0621)) break;
                 __syncwarp();
                 uint8_t* b_rows = b_rows_of(stage);
-                uint8_t* sfb = b_rows + (size_t)p.nb * 128;
+                uint8_t* sfb = b_rows + (size_t)g.nb * 128;
                 const bool inside = in_k(i);
                 while (cur.i == i) {
                     const int t = cur.t;
@@ -606,7 +629,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.full[stage]);
-                if (++stage == p.stages) {
+                if (++stage == g.stages) {
                     stage = 0;
                     phase ^= 1u;
                 }
@@ -660,29 +683,50 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     // ---------------------------------------------------------------- slices
     // The cluster's blocks share the rows out; slices add in rank order.
     {
-        const int rows = kTileRows / csize;
+        const int rows = kTileRows / csize;  // 16 to 128
         const uint32_t base = smem_u32(ring);
-        for (int i = (int)threadIdx.x; i < ntok * rows; i += kThreads<IMAGE>) {
+        if constexpr (M == Mode::GateUp) {
+            // sm.amax now gathers h's largest magnitudes.
+            __syncthreads();
+            if (threadIdx.x < kMaxTokens) sm.amax[threadIdx.x] = 0;
+            __syncthreads();
+        }
+        for (int i0 = (int)(warp * 32); i0 < ntok * rows; i0 += kThreads<IMAGE>) {
+            const int i = i0 + (int)lane;
             const int t = i / rows, r = rank * rows + i % rows;
             const int n = tile * kTileRows + r;
-            if (n >= p.N) continue;
-            const uint32_t off = base + (uint32_t)(t * kTileRows + r) * 4u;
-            float s = 0.0f;
-            for (int c = 0; c < p.split; ++c) s += ld_cluster_f32(mapa_shared(off, (uint32_t)c));
-            if constexpr (M == Mode::Gemv) {
-                if (p.R) s += static_cast<float>(static_cast<const YT*>(p.R)[(size_t)t * p.ldr + n]);
-                static_cast<YT*>(p.Y)[(size_t)t * p.ldy + n] = from_f32<YT>(s);
-            } else if constexpr (M == Mode::GateUp) {
-                float u = 0.0f;
-                for (int c = 0; c < p.split; ++c) u += ld_cluster_f32(mapa_shared(off, (uint32_t)(p.split + c)));
-                const int slot = sm.slot[t];
-                const float c = p.weights[slot] * __ldg(p.alpha2 + expert);
-                const float h = s / (1.0f + expf(-s)) * u * c;
-                static_cast<float*>(p.Y)[(size_t)slot * p.ldy + n] = h;
-                atomicMax(&p.amax_out[slot / p.top], __float_as_uint(h) & 0x7FFFFFFFu);
-            } else {
-                static_cast<YT*>(p.Y)[(size_t)t * p.ldy + n] = from_f32<YT>(s);
+            const bool valid = i < ntok * rows && n < p.N;
+            float s = 0.0f, u = 0.0f;
+            if (valid) {
+                const uint32_t off = base + (uint32_t)(t * kTileRows + r) * 4u;
+                for (int c = 0; c < p.split; ++c) s += ld_cluster_f32(mapa_shared(off, (uint32_t)c));
+                if constexpr (M == Mode::GateUp)
+                    for (int c = 0; c < p.split; ++c) u += ld_cluster_f32(mapa_shared(off, (uint32_t)(p.split + c)));
             }
+            if constexpr (M == Mode::GateUp) {
+                uint32_t m = 0;
+                if (valid) {
+                    const int slot = sm.slot[t];
+                    const float h = s / (1.0f + expf(-s)) * u * (p.weights[slot] * __ldg(p.alpha2 + expert));
+                    static_cast<float*>(p.Y)[(size_t)slot * p.ldy + n] = h;
+                    m = __float_as_uint(h) & 0x7FFFFFFFu;
+                }
+                // 16 neighbouring lanes have one token.
+#pragma unroll
+                for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                if ((lane & 15) == 0 && m) atomicMax(&sm.amax[t], m);
+            } else if (valid) {
+                if constexpr (M == Mode::Gemv)
+                    if (p.R) s += static_cast<float>(static_cast<const YT*>(p.R)[(size_t)t * p.ldr + n]);
+                const size_t row = M == Mode::DownPart ? sm.slot[t] : t;
+                static_cast<YT*>(p.Y)[row * p.ldy + n] = from_f32<YT>(s);
+            }
+        }
+        if constexpr (M == Mode::GateUp) {
+            __syncthreads();
+            // Maxima: the order of the atomics does not matter.
+            if ((int)threadIdx.x < ntok && sm.amax[threadIdx.x])
+                atomicMax(&p.amax_out[sm.slot[threadIdx.x] / p.top], sm.amax[threadIdx.x]);
         }
     }
     __syncwarp();
@@ -765,30 +809,24 @@ __global__ void __launch_bounds__(kImageThreads)
 
 static inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
-// Accumulator columns, ring depth and TMEM for T tokens. Up to 25 tokens (128
-// columns) two blocks share an SM, each with half of its shared memory and
-// 256 TMEM columns; above, the second 128 rows of B scales and the larger
-// stages leave room for one.
+// Shared memory and TMEM of a block. Two blocks share an SM, each with half of
+// its shared memory and 256 TMEM columns, unless one token count asks for more
+// than 128 accumulator columns in every block.
 struct Shape {
     int per_sm;
     size_t smem;
 };
 
-static Shape set_shape(Params& p) {
-    p.nb = (kPlanes * p.T + 7) & ~7;
-    const bool wide = p.nb > 128;
-    p.sfb_bytes = wide ? 4096 : 2048;
-    p.stage_bytes = kWBytes + (uint32_t)p.nb * 128 + kSfaBytes + p.sfb_bytes;
+static Shape set_shape(Params& p, bool wide) {
     const size_t overhead = 1024 + ((sizeof(Control) + 127) & ~(size_t)127);
     // 228 KiB per SM, 1 KiB of it reserved per block.
     const size_t room = (wide ? 227 * 1024 : (228 * 1024 - 2 * 1024) / 2) - overhead;
-    p.stages = (int)(room / p.stage_bytes);
-    if (p.stages > kMaxStages) p.stages = kMaxStages;
-    p.sf_col0 = ((uint32_t)p.nb + 15) & ~15u;
-    p.sf_slot = wide ? 48 : 32;
+    p.ring_bytes = (uint32_t)(room & ~(size_t)1023);
     p.tmem_cols = wide ? 512 : 256;
-    return {wide ? 1 : 2, (size_t)p.stages * p.stage_bytes + overhead};
+    return {wide ? 1 : 2, p.ring_bytes + overhead};
 }
+
+static bool is_wide(int T) { return kPlanes * T > 128; }
 
 // Slices of K: the split whose waves of blocks, each as long as its stages and
 // about two more for its start and end, take the fewest stage times. `units`
@@ -849,16 +887,17 @@ static bool use_image(int T, int K) { return (long long)T * K > 32768; }
 
 // Workspace of the converted activations: the stages' images, then the
 // tokens' largest magnitudes.
-static size_t image_bytes(const Params& p) { return (size_t)p.k_stages * ((size_t)p.nb * 128 + p.sfb_bytes); }
+static size_t image_bytes(int k_stages, const Geometry& g) { return (size_t)k_stages * ((size_t)g.nb * 128 + g.sfb_bytes); }
 
 template <typename XT>
 static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* workspace, cudaStream_t stream) {
     if (!workspace) return launch_stream<Mode::Gemv, XT, XT>(tm, tm, p, s.smem, p.tiles, stream);
     uint8_t* image = static_cast<uint8_t*>(workspace);
-    uint32_t* amax = reinterpret_cast<uint32_t*>(image + image_bytes(p));
+    const Geometry g = geometry(p.T, p.ring_bytes, p.tmem_cols);
+    uint32_t* amax = reinterpret_cast<uint32_t*>(image + image_bytes(p.k_stages, g));
     const int st = launch_status(launch_pdl(image_kernel<XT>, dim3((unsigned)p.T), dim3(kImageThreads), 0, stream,
-                                            static_cast<const XT*>(p.X), image, amax, p.K, p.ldx, p.x_vec, p.nb,
-                                            p.sfb_bytes));
+                                            static_cast<const XT*>(p.X), image, amax, p.K, p.ldx, p.x_vec, g.nb,
+                                            g.sfb_bytes));
     if (st != GPLK_STATUS_OK) return st;
     p.image = image;
     p.amax = amax;
@@ -871,12 +910,7 @@ static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* w
 extern "C" size_t gplk_gemv_nvfp4_workspace_bytes(int T, int N, int K) {
     using namespace gplk::fewtok;
     if (T <= 0 || T > kMaxTokens || N <= 0 || K <= 0 || K % 64 != 0 || !use_image(T, K)) return 0;
-    Params p;
-    memset(&p, 0, sizeof(p));
-    p.T = T;
-    p.k_stages = (K + kStageK - 1) / kStageK;
-    set_shape(p);
-    return image_bytes(p) + sizeof(uint32_t) * kMaxTokens;
+    return image_bytes((K + kStageK - 1) / kStageK, geometry(T, 0, 512)) + sizeof(uint32_t) * kMaxTokens;
 }
 
 extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* SF, void* Y, const void* R, int T,
@@ -913,7 +947,7 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     p.tiles = (N + kTileRows - 1) / kTileRows;
     p.k_stages = (K + kStageK - 1) / kStageK;
     p.kblocks = K / 64;
-    const Shape s = set_shape(p);
+    const Shape s = set_shape(p, is_wide(T));
     if (s.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
     p.split = choose_split(p.tiles, p.k_stages, 8, s.per_sm * d.sm_count);
     CUtensorMap tm;

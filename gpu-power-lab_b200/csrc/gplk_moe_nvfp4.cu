@@ -25,12 +25,16 @@ namespace moe {
 
 using namespace fewtok;
 
+// Whether the experts' down products go to sums of their own, per (token, rank)
+// slot, that a last kernel adds.
+static bool use_parts(int T) { return T > 8; }
+
 // Workspace: every part starts on a 256-byte boundary.
 struct Layout {
-    size_t route, amax, logits, ids, weights, h, total;
+    size_t route, amax, logits, ids, weights, h, part, total;
 };
 
-static Layout layout(int T, int E, int top, int F) {
+static Layout layout(int T, int E, int top, int D, int F) {
     auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
     Layout l;
     l.route = 0;
@@ -39,7 +43,8 @@ static Layout layout(int T, int E, int top, int F) {
     l.ids = l.logits + up((size_t)T * E * 4);
     l.weights = l.ids + up((size_t)T * top * 4);
     l.h = l.weights + up((size_t)T * top * 4);
-    l.total = l.h + up((size_t)T * top * F * 4);
+    l.part = l.h + up((size_t)T * top * F * 4);
+    l.total = l.part + (use_parts(T) ? up((size_t)T * top * D * 4) : 0);
     return l;
 }
 
@@ -123,9 +128,20 @@ __global__ void __launch_bounds__(kRouterThreads) router_kernel(const RouteParam
                                                          (part[2][threadIdx.x] + part[3][threadIdx.x]);
 }
 
+// Order-preserving integer of a float, NaN below every number.
+__device__ __forceinline__ uint32_t sort_key(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return isnan(v) ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return k == 0 ? __uint_as_float(0x7FC00000u) : __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
 // Softmax and top-k of one token per warp, then the routing tables. A lane
-// holds the logits of experts lane, lane + 32, ...; each rank takes the largest
-// left, the lowest index among equals. A NaN counts below every number.
+// holds the logits of experts lane, lane + 32, ... (PER of them); each rank
+// takes the largest left, the lowest index among equals. A NaN counts below
+// every number.
+template <int PER>
 __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParams p) {
     const int warp = (int)warp_id_uniform();
     const int lane = (int)lane_id();
@@ -139,52 +155,42 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
     pdl_launch_dependents();
     if (warp < p.T) {
         const float* l = p.logits + (size_t)warp * p.E;
-        float v[kPer];
-        float best = -INFINITY;
+        float v[PER];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const int e = lane + 32 * i;
-            v[i] = e < p.E ? l[e] : -INFINITY;
-            best = fmaxf(best, v[i]);
+        for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < p.E ? l[lane + 32 * i] : -INFINITY;
+        uint32_t key[PER];
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            key[i] = lane + 32 * i < p.E ? sort_key(v[i]) : 0u;
+            most = max(most, key[i]);
         }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+        const float best = key_value(__reduce_max_sync(0xffffffffu, most));
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += lane + 32 * i < p.E ? expf(v[i] - best) : 0.0f;
+        for (int i = 0; i < PER; ++i) sum += lane + 32 * i < p.E ? expf(v[i] - best) : 0.0f;
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         uint32_t taken = 0;
         float chosen = 0.0f, top_sum = 0.0f;
         int chosen_id = 0;
         for (int j = 0; j < p.top; ++j) {
-            float bv = 0.0f;
-            int be = INT_MAX;  // INT_MAX: none yet
+            uint32_t k = 0;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int e = lane + 32 * i;
-                if (e >= p.E || (taken >> i & 1)) continue;
-                const float a = isnan(v[i]) ? -INFINITY : v[i];
-                if (be == INT_MAX || a > bv) {
-                    bv = a;
-                    be = e;
-                }
-            }
+            for (int i = 0; i < PER; ++i)
+                if (!(taken >> i & 1)) k = max(k, key[i]);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, k);
+            uint32_t e = 0xFFFFFFFFu;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-                const int oe = __shfl_xor_sync(0xffffffffu, be, o);
-                if (oe != INT_MAX && (be == INT_MAX || ov > bv || (ov == bv && oe < be))) {
-                    bv = ov;
-                    be = oe;
-                }
-            }
-            if ((be & 31) == lane) taken |= 1u << (be >> 5);
-            const float pr = expf(l[be] - best) / sum;
+            for (int i = PER - 1; i >= 0; --i)
+                if (!(taken >> i & 1) && key[i] == m && lane + 32 * i < p.E) e = (uint32_t)(lane + 32 * i);
+            e = __reduce_min_sync(0xffffffffu, e);  // top <= E: one is left
+            if ((int)(e & 31) == lane) taken |= 1u << (e >> 5);
+            const float pr = expf(key_value(m) - best) / sum;
             top_sum += pr;
             if (lane == j) {
                 chosen = pr;
-                chosen_id = be;
+                chosen_id = (int)e;
             }
         }
         if (lane < p.top) {
@@ -203,14 +209,14 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const uint32_t m = chosen_mask[i];
-            if (i < e >> 5) before += __popc(m);
+            if (i < (e >> 5)) before += __popc(m);
             n_active += __popc(m);
         }
         if (e < p.E && (chosen_mask[e >> 5] >> (e & 31) & 1)) {
             const int a = before + __popc(chosen_mask[e >> 5] & ((1u << (e & 31)) - 1));
             active[a] = e;
-            p.route->active[a] = e;
         }
+        if (e < kMaxExperts && e >= n_active) p.route->head[e] = 0;
         if (e == 0) p.route->n_active = n_active;
     }
     __syncthreads();
@@ -222,13 +228,35 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
         const uint32_t m = __ballot_sync(0xffffffffu, slot >= 0);
         if (slot >= 0) p.route->list[a][__popc(m & ((1u << lane) - 1))] = (int16_t)slot;
         p.route->slot[a][lane] = (int16_t)slot;
-        if (lane == 0) p.route->count[a] = __popc(m);
+        if (lane == 0) p.route->head[a] = active[a] | __popc(m) << 16;
     }
+}
+
+// y[t] = the sum of a token's slots, in the order of their ranks.
+template <typename XT>
+__global__ void __launch_bounds__(256) combine_kernel(const float* part, XT* y, int top, int D, int ldy) {
+    const int t = blockIdx.y, n = ((int)blockIdx.x * 256 + (int)threadIdx.x) * 4;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (n >= D) return;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j = 0; j < top; ++j) {
+        const float4 v = *reinterpret_cast<const float4*>(part + ((size_t)t * top + j) * D + n);
+        s.x += v.x;
+        s.y += v.y;
+        s.z += v.z;
+        s.w += v.w;
+    }
+    XT* row = y + (size_t)t * ldy + n;
+    row[0] = from_f32<XT>(s.x);
+    row[1] = from_f32<XT>(s.y);
+    row[2] = from_f32<XT>(s.z);
+    row[3] = from_f32<XT>(s.w);
 }
 
 template <typename XT>
 static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t stream) {
-    const Layout l = layout(c.T, c.E, c.top, c.F);
+    const Layout l = layout(c.T, c.E, c.top, c.D, c.F);
     uint8_t* ws = static_cast<uint8_t*>(c.workspace);
     RouteParams r;
     r.x = c.x;
@@ -254,6 +282,8 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     double active = c.E * (1.0 - miss);
     if (active < 1.0) active = 1.0;
 
+    const bool parts = use_parts(c.T);
+
     Params g;
     memset(&g, 0, sizeof(g));
     g.X = c.x;
@@ -277,24 +307,25 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     g.tiles = (c.F + kTileRows - 1) / kTileRows;
     g.k_stages = (c.D + kStageK - 1) / kStageK;
     g.kblocks = c.D / 64;
-    const Shape gs = set_shape(g);
+    const Shape gs = set_shape(g, false);  // sized by each expert's own tokens
     Params o = g;
     o.X = g.Y;
     o.amax = g.amax_out;
     o.sf0 = c.sf_down;
-    o.Y = c.y;
+    o.Y = parts ? static_cast<void*>(ws + l.part) : c.y;
     o.N = c.D;
     o.K = c.F;
     o.ldx = c.F;
-    o.ldy = c.ldy;
+    o.ldy = parts ? c.D : c.ldy;
     o.x_vec = 1;
     o.tiles = (c.D + kTileRows - 1) / kTileRows;
     o.k_stages = (c.F + kStageK - 1) / kStageK;
     o.kblocks = c.F / 64;
-    const Shape os = set_shape(o);
+    const Shape os = set_shape(o, !parts && is_wide(c.T));
     if (gs.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
     g.split = choose_split(2.0 * g.tiles * active, g.k_stages, 4, gs.per_sm * d.sm_count);
-    o.split = choose_split(o.tiles, o.k_stages * active, 8, os.per_sm * d.sm_count);
+    o.split = parts ? choose_split(o.tiles * active, o.k_stages, 8, os.per_sm * d.sm_count)
+                    : choose_split(o.tiles, o.k_stages * active, 8, os.per_sm * d.sm_count);
 
     CUtensorMap tg, tu, td;
     int st = encode_weights(&tg, c.gate, (uint64_t)c.E * c.F, c.D);
@@ -307,11 +338,16 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     };
     st = c.T == 1 ? router(router_kernel<XT, 1>, 1) : c.T <= 4 ? router(router_kernel<XT, 4>, 4) : router(router_kernel<XT, 8>, 8);
     if (st == GPLK_STATUS_OK)
-        st = launch_status(launch_pdl(route_kernel, dim3(1), dim3(32 * kMaxTokens), 0, stream, r));
+        st = launch_status(launch_pdl(c.E <= 128 ? route_kernel<4> : route_kernel<kMaxExperts / 32>, dim3(1),
+                                      dim3(32 * kMaxTokens), 0, stream, r));
     if (st == GPLK_STATUS_OK)
         st = launch_stream<Mode::GateUp, XT, float>(tg, tu, g, gs.smem, max_active * g.tiles, stream);
-    if (st == GPLK_STATUS_OK) st = launch_stream<Mode::Down, float, XT>(td, td, o, os.smem, o.tiles, stream);
-    return st;
+    if (st != GPLK_STATUS_OK) return st;
+    if (!parts) return launch_stream<Mode::Down, float, XT>(td, td, o, os.smem, o.tiles, stream);
+    st = launch_stream<Mode::DownPart, float, float>(td, td, o, os.smem, max_active * o.tiles, stream);
+    if (st != GPLK_STATUS_OK) return st;
+    return launch_status(launch_pdl(combine_kernel<XT>, dim3((c.D + 1023) / 1024, c.T), dim3(256), 0, stream,
+                                    static_cast<const float*>(o.Y), static_cast<XT*>(c.y), c.top, c.D, c.ldy));
 }
 
 }  // namespace moe
@@ -322,7 +358,7 @@ extern "C" size_t gplk_moe_nvfp4_workspace_bytes(int T, int E, int top, int D, i
     if (T <= 0 || E <= 0 || top <= 0 || D <= 0 || F <= 0 || T > fewtok::kMaxTokens || E > fewtok::kMaxExperts ||
         top > fewtok::kMaxTop || top > E)
         return 0;
-    return moe::layout(T, E, top, F).total;
+    return moe::layout(T, E, top, D, F).total;
 }
 
 extern "C" int gplk_moe_nvfp4(const gplk_moe_cfg* cfg, cudaStream_t stream) {
@@ -348,7 +384,7 @@ extern "C" int gplk_moe_nvfp4(const gplk_moe_cfg* cfg, cudaStream_t stream) {
                           (const void*)c.ids, (const void*)c.weights})
         if (!aligned(q, 4)) return GPLK_STATUS_BAD_ARG;
     if (!aligned(c.x, 2) || !aligned(c.y, 2) || !aligned(c.router, 2)) return GPLK_STATUS_BAD_ARG;
-    if (c.workspace_bytes < moe::layout(c.T, c.E, c.top, c.F).total) return GPLK_STATUS_BAD_ARG;
+    if (c.workspace_bytes < moe::layout(c.T, c.E, c.top, c.D, c.F).total) return GPLK_STATUS_BAD_ARG;
     DeviceInfo d;
     const int st = require_sm100(&d);
     if (st != GPLK_STATUS_OK) return st;
