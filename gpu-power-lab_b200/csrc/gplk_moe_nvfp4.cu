@@ -9,7 +9,7 @@
 //   router    logits, a block per expert and 8 tokens, FP32 sums
 //   route     one block: softmax, top-k, and the lists the products follow
 //             (which experts, whose tokens)
-//   gate/up   stream_kernel (gplk_gemv_nvfp4.cu), a cluster per 128 features of
+//   gate/up   stream_kernel (gplk_nvfp4_stream.cu), a cluster per 128 features of
 //             a chosen expert: half of its blocks multiply gate rows, half up
 //             rows, over slices of D, by the expert's own tokens; the join
 //             writes p_j ad_e silu(g) u, FP32, per (token, rank) slot
@@ -28,6 +28,9 @@ using namespace fewtok;
 // Whether the experts' down products go to sums of their own, per (token, rank)
 // slot, that a last kernel adds.
 static bool use_parts(int T) { return T > 8; }
+
+// Whether a block of the per-slot down products takes two tiles.
+static bool use_down_pairs(int T) { return T > 0; }
 
 // Workspace: every part starts on a 256-byte boundary.
 struct Layout {
@@ -149,6 +152,7 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
     __shared__ int ids[kMaxTokens * kMaxTop];
     __shared__ uint32_t chosen_mask[kPer];
     __shared__ int active[kMaxExperts];
+    __shared__ int chunks[kMaxExperts];
     if (threadIdx.x < kPer) chosen_mask[threadIdx.x] = 0;
     __syncthreads();
     pdl_wait();
@@ -202,9 +206,9 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
         }
     }
     __syncthreads();
-    int n_active = 0;
+    // The chosen experts in ascending order, and how many tokens each has.
+    int n_active = 0, before = 0;
     {
-        int before = 0;
         const int e = (int)threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -212,23 +216,44 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
             if (i < (e >> 5)) before += __popc(m);
             n_active += __popc(m);
         }
-        if (e < p.E && (chosen_mask[e >> 5] >> (e & 31) & 1)) {
-            const int a = before + __popc(chosen_mask[e >> 5] & ((1u << (e & 31)) - 1));
-            active[a] = e;
-        }
-        if (e < kMaxExperts && e >= n_active) p.route->head[e] = 0;
-        if (e == 0) p.route->n_active = n_active;
+        if (e < p.E && (chosen_mask[e >> 5] >> (e & 31) & 1))
+            active[before + __popc(chosen_mask[e >> 5] & ((1u << (e & 31)) - 1))] = e;
     }
     __syncthreads();
-    for (int a = warp; a < n_active; a += kMaxTokens) {
+    auto slot_of = [&](int e) {  // this lane's token's slot with expert e
         int slot = -1;
         if (lane < p.T)
             for (int j = 0; j < p.top; ++j)
-                if (ids[lane * p.top + j] == active[a]) slot = lane * p.top + j;
+                if (ids[lane * p.top + j] == e) slot = lane * p.top + j;
+        return slot;
+    };
+    for (int a = warp; a < n_active; a += kMaxTokens) {
+        const uint32_t m = __ballot_sync(0xffffffffu, slot_of(active[a]) >= 0);
+        if (lane == 0) chunks[a] = (__popc(m) + kMaxEntryTokens - 1) / kMaxEntryTokens;
+    }
+    __syncthreads();
+    for (int a = warp; a < n_active; a += kMaxTokens) {
+        // Entries of the experts before this one.
+        int base = 0;
+        for (int b = lane; b < a; b += 32) base += chunks[b];
+        base = __reduce_add_sync(0xffffffffu, base);
+        const int slot = slot_of(active[a]);
         const uint32_t m = __ballot_sync(0xffffffffu, slot >= 0);
-        if (slot >= 0) p.route->list[a][__popc(m & ((1u << lane) - 1))] = (int16_t)slot;
-        p.route->slot[a][lane] = (int16_t)slot;
-        if (lane == 0) p.route->head[a] = active[a] | __popc(m) << 16;
+        const int n = __popc(m), place = __popc(m & ((1u << lane) - 1));
+        for (int c = 0; c < chunks[a]; ++c) {
+            const int in_chunk = place - c * kMaxEntryTokens;
+            const bool mine = slot >= 0 && in_chunk >= 0 && in_chunk < kMaxEntryTokens;
+            if (mine) p.route->list[base + c][in_chunk] = (int16_t)slot;
+            p.route->slot[base + c][lane] = (int16_t)(mine ? slot : -1);
+            if (lane == 0) p.route->head[base + c] = active[a] | min(kMaxEntryTokens, n - c * kMaxEntryTokens) << 16;
+        }
+    }
+    if (warp == 0) {
+        int entries = 0;
+        for (int b = lane; b < n_active; b += 32) entries += chunks[b];
+        entries = __reduce_add_sync(0xffffffffu, entries);
+        for (int b = entries + lane; b < kMaxExperts; b += 32) p.route->head[b] = 0;
+        if (lane == 0) p.route->n_entries = entries;
     }
 }
 
@@ -275,7 +300,9 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     r.renormalise = c.renormalise;
 
     const int slots = c.T * c.top;
-    const int max_active = slots < c.E ? slots : c.E;
+    // Every entry has a token, and all but one of an expert's kMaxEntryTokens.
+    const int most = c.E + slots / kMaxEntryTokens;
+    const int max_entries = slots < most ? slots : most;
     // Chosen experts to expect of T independent choices, for the splits.
     double miss = 1.0;
     for (int t = 0; t < c.T; ++t) miss *= 1.0 - (double)c.top / c.E;
@@ -307,7 +334,9 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     g.tiles = (c.F + kTileRows - 1) / kTileRows;
     g.k_stages = (c.D + kStageK - 1) / kStageK;
     g.kblocks = c.D / 64;
-    const Shape gs = set_shape(g, false);  // sized by each expert's own tokens
+    g.halves = 2;
+    const int entry_tokens = c.T < kMaxEntryTokens ? c.T : kMaxEntryTokens;
+    const Shape gs = set_shape(g, entry_tokens, true);
     Params o = g;
     o.X = g.Y;
     o.amax = g.amax_out;
@@ -321,11 +350,13 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     o.tiles = (c.D + kTileRows - 1) / kTileRows;
     o.k_stages = (c.F + kStageK - 1) / kStageK;
     o.kblocks = c.F / 64;
-    const Shape os = set_shape(o, !parts && is_wide(c.T));
+    o.halves = parts && use_down_pairs(c.T) ? 2 : 1;
+    const int groups = (o.tiles + o.halves - 1) / o.halves;
+    const Shape os = set_shape(o, parts ? entry_tokens : c.T, parts);
     if (gs.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
-    g.split = choose_split(2.0 * g.tiles * active, g.k_stages, 4, gs.per_sm * d.sm_count);
-    o.split = parts ? choose_split(o.tiles * active, o.k_stages, 8, os.per_sm * d.sm_count)
-                    : choose_split(o.tiles, o.k_stages * active, 8, os.per_sm * d.sm_count);
+    g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, 8, gs.per_sm * d.sm_count);
+    o.split_log2 = parts ? choose_split_log2(groups * active, o.halves * o.k_stages, 8, os.per_sm * d.sm_count)
+                    : choose_split_log2(groups, o.halves * o.k_stages * active, 8, os.per_sm * d.sm_count);
 
     CUtensorMap tg, tu, td;
     int st = encode_weights(&tg, c.gate, (uint64_t)c.E * c.F, c.D);
@@ -341,10 +372,10 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
         st = launch_status(launch_pdl(c.E <= 128 ? route_kernel<4> : route_kernel<kMaxExperts / 32>, dim3(1),
                                       dim3(32 * kMaxTokens), 0, stream, r));
     if (st == GPLK_STATUS_OK)
-        st = launch_stream<Mode::GateUp, XT, float>(tg, tu, g, gs.smem, max_active * g.tiles, stream);
+        st = launch_stream<Mode::GateUp, XT, float>(tg, tu, g, gs.smem, max_entries * g.tiles, stream);
     if (st != GPLK_STATUS_OK) return st;
-    if (!parts) return launch_stream<Mode::Down, float, XT>(td, td, o, os.smem, o.tiles, stream);
-    st = launch_stream<Mode::DownPart, float, float>(td, td, o, os.smem, max_active * o.tiles, stream);
+    if (!parts) return launch_stream<Mode::Down, float, XT>(td, td, o, os.smem, groups, stream);
+    st = launch_stream<Mode::DownPart, float, float>(td, td, o, os.smem, max_entries * groups, stream);
     if (st != GPLK_STATUS_OK) return st;
     return launch_status(launch_pdl(combine_kernel<XT>, dim3((c.D + 1023) / 1024, c.T), dim3(256), 0, stream,
                                     static_cast<const float*>(o.Y), static_cast<XT*>(c.y), c.top, c.D, c.ldy));

@@ -1,0 +1,931 @@
+// gplk_nvfp4_stream.cu - the main loop of the products of a few tokens with NVFP4
+// weights (gplk_gemv_nvfp4.cu, gplk_moe_nvfp4.cu):
+//   y[t][n] = sum_k x[t][k] * sf[n][k / 16] * w[n][k]
+// E2M1 weights and UE4M3 scales in the layout gplk_gemm_nvfp4_tn reads, 16-bit
+// or FP32 activations, FP32 sums.
+//
+// What bounds it: every weight is read once for 2 T operations, so HBM. A
+// B200 reads 46 weights per SM and clock; decoding them on the CUDA cores
+// takes about that many issue slots (one warp per row with FP32 FMAs measured
+// 0.56 TB/s at one token, 16384 x 8192). So the weights are not decoded at all:
+// they go from HBM through TMA to the block-scaled tensor-core MMA
+// (kind::mxf4nvf4), codes and scales as they lie, and the activations are
+// brought to its operand format instead, exactly enough to count as 16-bit:
+//
+//   Within a 16-group of a token, 2^b the power of two at or below its largest
+//   magnitude, x is rounded to a multiple of 2^b / 8192 and written in
+//   balanced base-8 digits  x = 2^b * sum_p d_p / 2 * 8^-p,  p = 0..4,
+//   d_0 in -4..4, the others in -4..3. Every d / 2 is an E2M1 value, so digit p
+//   of all of k is one E2M1 row ("plane") of the MMA's B operand, and 2^b,
+//   relative to the token's largest magnitude 2^A, is the group's UE4M3 scale.
+//   Five planes keep 15 bits: an activation is off by at most 2^-14 of its
+//   group's largest magnitude (2^-28 of the token's, in groups 2^14 below
+//   it), where BF16 itself is off by 2^-9 of each value. The accumulator
+//   column of each (token, plane) is exact products in FP32 sums; the epilogue
+//   adds 8^-p times the planes' columns.
+//
+// So T tokens are an MMA of N = 5 T columns (padded to 8), at most 160 of the
+// 256 an instruction takes.
+//
+// Layout of the work. A block owns 128 weight rows (the MMA's M), or two such
+// tiles that share the activations' rows (gate and up of an expert, or
+// neighbours), and a slice of K; blocks of a cluster share the rows, split K,
+// and add their partial sums in rank order through distributed shared memory,
+// so the bits do not depend on timing. Two blocks share an SM where TMEM allows:
+// one's start and end hide behind the other's stream.
+//   warp 0      TMA producer: 128 rows x 128 bytes of codes and up to 2 KiB of
+//               scales (256 elements of K) per slot of the weights' ring
+//   warp 1      owns TMEM, copies the scales there and issues one MMA per 64
+//               elements of K and tile
+//   warps 2..9  convert the same 256 elements of every token into a slot of
+//               the activations' ring (a warp per token and slot); warps 2..5
+//               then read the accumulators, and all warps add the slices.
+//               In an Image kernel there are warps 2..5 only, and one thread
+//               of them fetches slots that another kernel converted.
+// The MMA warp runs its loop converged and elects the issuing lane: with
+// addresses and descriptors in uniform registers, 65536 x 8192 at one token
+// takes 51 us; issued from a lane of a diverged warp 76 us.
+// Every mbarrier wait is bounded, as everywhere in this library.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+#include <cstring>
+#include <type_traits>
+
+#include "gplk_ptx.cuh"
+
+namespace gplk {
+namespace fewtok {
+
+constexpr int kMaxTokens = 32;
+constexpr int kMaxExperts = 512;
+constexpr int kMaxTop = 16;
+constexpr int kMaxEntryTokens = 12;             // tokens of one expert that a block takes
+constexpr int kPlanes = 5;
+constexpr int kConvWarps = 8;
+constexpr int kTileRows = 128;
+constexpr int kStageK = 256;                    // elements of K per slot
+constexpr uint32_t kWBytes = kTileRows * 128;   // codes of a weights' slot
+constexpr uint32_t kSfaBytes = 4 * 512;         // its scales
+constexpr uint32_t kWSlot = kWBytes + kSfaBytes;
+constexpr int kMaxSlots = 8;
+constexpr uint32_t kDigitBias = 4u * (1u + 8u + 64u + 512u + 4096u);
+
+// Gemv: all tokens against one matrix. GateUp: tokens of a chosen expert against
+// its gate and up matrices. Down: all tokens against every chosen expert's down
+// matrix, accumulated over the experts. DownPart: tokens of a chosen expert
+// against its down matrix.
+enum class Mode { Gemv, GateUp, Down, DownPart };
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+    return static_cast<T>(v);
+}
+
+// ---------------------------------------------------------------- routing tables (MoE)
+// Written by the route kernel into the layer's workspace. An entry is a chosen
+// expert with up to kMaxEntryTokens of its tokens; experts ascend.
+struct Route {
+    int n_entries;
+    int head[kMaxExperts];                      // expert | tokens << 16; 0 behind the last entry
+    int16_t list[kMaxExperts][16];              // the tokens' slots (token * top + rank), ascending
+    int16_t slot[kMaxExperts][kMaxTokens];      // slot of token t in entry a, or -1
+};
+
+// Rings and TMEM of a block. Shared memory: the weights' slots (codes, scales),
+// then the activations' (B rows, B scales). TMEM: an accumulator per tile, the
+// weights' scale columns per slot, the activations'. Worked out by the host: a
+// division takes the device as long as a stage's MMA.
+struct Geometry {
+    int nb;              // accumulator columns, 5 per token padded to 8
+    int w_slots, b_slots;
+    uint32_t sfb_step;   // bytes from one 64-element block of B scales to the next
+    uint32_t image;      // bytes of B rows and scales
+    uint32_t b_slot;     // the same, padded to 1 KiB
+    uint32_t acc_cols;   // from one accumulator to the next
+    uint32_t sfb_cols;   // TMEM columns of a slot's B scales
+};
+
+// A slot of activations has no barriers of its own: it is filled before, and
+// freed with, the weights' slot that follows it. Tile j of the stream (h of stage
+// i: j = i * halves + h) takes weights' slot j % w, so whoever has seen that
+// slot free knows that tiles up to j - w are done; with b slots such that stage
+// i - b is among those, the activations' slot is free too: b = w for single
+// tiles, b = w / 2 + 1 for pairs.
+static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tmem_cols) {
+    Geometry g;
+    g.nb = (kPlanes * ntok + 7) & ~7;
+    const bool wide = g.nb > 128;  // a second 128 rows of B scales
+    // A scale copy reads 512 bytes, 16 per row; with up to 32 rows the blocks
+    // lie as close as their rows, and a copy's rest is never used.
+    g.sfb_step = g.nb <= 32 ? 16u * (uint32_t)g.nb : 512u;
+    g.image = (uint32_t)g.nb * 128 + (wide ? 4096u : 3 * g.sfb_step + 512);
+    g.b_slot = (g.image + 1023) & ~1023u;
+    g.acc_cols = ((uint32_t)g.nb + 15) & ~15u;
+    g.sfb_cols = wide ? 32 : 16;
+    for (g.w_slots = kMaxSlots; g.w_slots > 1; --g.w_slots) {
+        g.b_slots = halves == 1 ? g.w_slots : g.w_slots / 2 + 1;
+        if ((uint32_t)g.w_slots * kWSlot + (uint32_t)g.b_slots * g.b_slot <= ring_bytes &&
+            (uint32_t)halves * g.acc_cols + (uint32_t)g.w_slots * 16 + (uint32_t)g.b_slots * g.sfb_cols <= tmem_cols)
+            break;
+    }
+    return g;
+}
+
+struct Params {
+    const void* X;       // activations (Gemv, GateUp: 16-bit rows; Down*: FP32 h rows by slot)
+    const uint8_t* sf0;  // scales: W, gate or down
+    const uint8_t* sf1;  // GateUp: up
+    const float* alpha0; // Gemv: one; GateUp: gate's, per expert
+    const float* alpha1; // GateUp: up's
+    const float* alpha2; // GateUp: down's, folded into h
+    void* Y;             // Gemv, Down: T rows; GateUp, DownPart: FP32 rows by slot
+    const void* R;
+    const Route* route;
+    const float* weights;  // MoE: per slot
+    const uint8_t* image;  // Image kernels: the converted activations, by stage
+    const uint32_t* amax;  // bits of each token's largest magnitude, or NULL: this kernel finds its slice's
+    uint32_t* amax_out;    // GateUp: h's, by token
+    int T, N, K, ldx, ldy, ldr;
+    int x_vec;           // rows of X are 16-byte aligned
+    int top;
+    uint32_t inverse[kMaxTokens + 1];  // 2^16 / n + 1
+    int tiles;           // 128-row tiles of one matrix
+    int halves;          // tiles a block takes: 1 or 2 (GateUp: 2, gate's and up's)
+    int k_stages;        // stages of one matrix row
+    int kblocks;         // K / 64
+    int split_log2;      // slices of K, the cluster's size
+    uint32_t ring_bytes; // shared memory of the two rings
+    uint32_t tmem_cols;
+    Geometry geo[kMaxEntryTokens];  // per-expert modes: by tokens - 1; else the first, for T tokens
+};
+
+struct Control {
+    uint64_t full[kMaxSlots];   // by weights' slot
+    uint64_t empty[kMaxSlots];
+    uint64_t acc_full;
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort;
+    uint32_t amax[kMaxTokens];  // bits of the largest magnitude in this block's slice
+    int16_t slot[kMaxTokens];   // per-expert modes: slots of the block's tokens
+    uint8_t dirty[kMaxSlots][kMaxTokens];  // Down: the slot holds digits of that token
+};
+
+// A ring position.
+struct Cursor {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void advance(int slots) {
+        if (++slot == slots) {
+            slot = 0;
+            phase ^= 1u;
+        }
+    }
+};
+
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+// True in one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e != 0;
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// Eight consecutive activations of one lane.
+template <typename XT>
+__device__ __forceinline__ void load_raw(const XT* x, bool vec, uint4 (&r)[2]) {
+    if constexpr (sizeof(XT) == 4) {
+        r[0] = *reinterpret_cast<const uint4*>(x);
+        r[1] = *reinterpret_cast<const uint4*>(x + 4);
+    } else if (vec) {
+        r[0] = *reinterpret_cast<const uint4*>(x);
+    } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+        uint32_t v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+        r[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+template <typename XT>
+__device__ __forceinline__ void widen(const uint4 (&r)[2], float (&v)[8]) {
+    const uint32_t w[4] = {r[0].x, r[0].y, r[0].z, r[0].w};
+    if constexpr (sizeof(XT) == 4) {
+        const uint32_t w1[4] = {r[1].x, r[1].y, r[1].z, r[1].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __uint_as_float(w[i]);
+            v[4 + i] = __uint_as_float(w1[i]);
+        }
+    } else if constexpr (std::is_same<XT, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
+            v[2 * i] = __low2float(h);
+            v[2 * i + 1] = __high2float(h);
+        }
+    }
+}
+
+// Bits of the largest magnitude. Integer order is magnitude order, with
+// infinity and then NaN above every finite number.
+__device__ __forceinline__ uint32_t max_bits(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
+}
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// Exponent A of a token's largest magnitude. Below 2^-100 the anchor stays
+// there: what is then lost is below 2^-127, FP32's own subnormal range.
+__device__ __forceinline__ int anchor_of(uint32_t amax_bits) { return max((int)(amax_bits >> 23) - 127, -100); }
+
+// Eight nibbles of biased digits (0..7 for -4..3; 8 for the top digit's 4) to
+// E2M1 codes of d / 2: magnitude |d| in the low three bits, sign above.
+template <bool TOP>
+__device__ __forceinline__ uint32_t digit_codes(uint32_t w) {
+    uint32_t m = ~(w >> 2);  // 1 in the nibbles of negative digits
+    if constexpr (TOP) m &= ~(w >> 3);
+    m &= 0x11111111u;
+    uint32_t c = ((w ^ (m * 3u)) & 0x33333333u) + m * 9u;  // negative: 8 | (3 - w) + 1
+    if constexpr (TOP) c |= (w >> 1) & 0x44444444u;
+    return c;
+}
+
+// Byte of row r's scale for a lane's 16-group: one block per 64 elements, with
+// 16 bytes per row of 32 and 4 per further 32 rows, as the scale copy reads it.
+__device__ __forceinline__ uint32_t sfb_offset(uint32_t r, uint32_t lane, uint32_t step) {
+    return (r >> 7) * 2048 + (lane >> 3) * step + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((lane >> 1) & 3);
+}
+
+// One token's 256 elements of a stage, eight per lane: planes 5 t .. 5 t + 4
+// of the stage's B rows (128-byte swizzled, K-major) and the 16 groups'
+// scales. `on` is false for lanes beyond K, whose blocks no MMA reads.
+__device__ __forceinline__ void convert(const float (&v)[8], int anchor, int t, bool on, uint8_t* b_rows,
+                                        uint8_t* sfb, uint32_t sfb_step, uint32_t lane) {
+    uint32_t m = max_bits(v);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));  // the other half of the 16-group
+    const int b = max((int)(m >> 23) - 127, anchor - 14);
+    const float scale = __uint_as_float((uint32_t)(13 - b + 127) << 23);
+    // x * scale is at most 2^14 in magnitude; adding 1.5 * 2^23 rounds it to an
+    // integer, and the bias makes every digit non-negative.
+    constexpr float kMagic = 12582912.0f + (float)kDigitBias;
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__fmaf_rn(v[i], scale, kMagic));
+    uint32_t q[4];  // elements i and i + 4: nibbles i and i + 4 of a word are 16 bits apart
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = __byte_perm(u[i], u[i + 4], 0x5410);
+    if (!on) return;
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+        const int sh = 3 * (kPlanes - 1 - p);
+        const uint32_t mask = p == 0 ? 0x000F000Fu : 0x00070007u;
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= ((q[i] >> sh) & mask) << (4 * i);
+        w = p == 0 ? digit_codes<true>(w) : digit_codes<false>(w);
+        const uint32_t r = (uint32_t)(kPlanes * t + p);
+        *reinterpret_cast<uint32_t*>(b_rows + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
+                                     (lane & 3) * 4) = w;
+        if ((lane & 1) == (uint32_t)(p & 1))
+            sfb[sfb_offset(r, lane, sfb_step)] = (uint8_t)((b - anchor + 15) << 3);
+    }
+}
+
+// A token without a part in the stage's expert: zero digits, scale 1.
+__device__ __forceinline__ void convert_zero(int t, uint8_t* b_rows, uint8_t* sfb, uint32_t sfb_step,
+                                             uint32_t lane) {
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+        const uint32_t r = (uint32_t)(kPlanes * t + p);
+        *reinterpret_cast<uint32_t*>(b_rows + (r >> 3) * 1024 + (r & 7) * 128 + lane * 4) = 0u;
+        if ((lane & 1) == (uint32_t)(p & 1))
+            sfb[sfb_offset(r, lane, sfb_step)] = 0x38;
+    }
+}
+
+template <bool IMAGE>
+constexpr int kThreads = IMAGE ? 64 + 128 : 64 + 32 * kConvWarps;
+
+template <Mode M, typename XT, typename YT, bool IMAGE>
+__global__ void __launch_bounds__(kThreads<IMAGE>, 2)
+    stream_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1, const __grid_constant__ Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    Control& sm = *reinterpret_cast<Control*>(ring + p.ring_bytes);
+    const uint32_t warp = warp_id_uniform();
+    const uint32_t lane = lane_id();
+    const int slice = (int)cluster_ctarank();
+    const int split = 1 << p.split_log2;
+    const int cid = (int)(blockIdx.x >> p.split_log2);
+    constexpr bool kPerExpert = M == Mode::GateUp || M == Mode::DownPart;
+
+    // Barriers and TMEM. A slot is full when the copies have landed and the
+    // warps with tokens in the stage have converted them.
+    auto set_up = [&](int ntok) {
+        if (threadIdx.x < kMaxSlots) {
+            const int i = (int)threadIdx.x;
+            mbar_init(&sm.full[i], IMAGE ? 1u : 1u + (uint32_t)min(ntok, kConvWarps));
+            mbar_init(&sm.empty[i], 1);
+            if (i == 0) {
+                mbar_init(&sm.acc_full, 1);
+                mbar_init(&sm.drain, 1);
+                sm.abort = 0;
+            }
+            fence_barrier_init();
+        }
+        if (threadIdx.x < kMaxTokens) sm.amax[threadIdx.x] = 0;
+        if (warp == 1) {
+            tmem_alloc(&sm.tmem_base, p.tmem_cols);
+            tmem_relinquish();
+        }
+    };
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tm0);
+        if (M == Mode::GateUp) tma_prefetch_desc(&tm1);
+    }
+    if constexpr (!kPerExpert) set_up(p.T);
+    // What is above may overlap the previous kernel's tail. The conversion
+    // kernel that an Image kernel follows let it start only once every kernel
+    // before the two had completed, so weights may be read at once; what that
+    // kernel wrote is read behind a pdl_wait() of its own. Elsewhere nothing
+    // below touches global memory before the previous kernel has completed.
+    if constexpr (!IMAGE) pdl_wait();
+    pdl_launch_dependents();
+
+    // This block's rows, tokens and stages.
+    int group = cid, expert = 0, ntok = p.T, total = p.k_stages;
+    if constexpr (kPerExpert) {
+        const int groups = M == Mode::GateUp ? p.tiles : (p.tiles + p.halves - 1) / p.halves;
+        const int a = cid / groups;
+        group = cid % groups;
+        const int head = p.route->head[a];
+        if (threadIdx.x < kMaxEntryTokens) sm.slot[threadIdx.x] = p.route->list[a][threadIdx.x];
+        expert = head & 0xFFFF;
+        ntok = head >> 16;
+        if (ntok == 0) return;  // behind the last entry; the whole cluster leaves
+        set_up(ntok);
+    } else if constexpr (M == Mode::Down) {
+        total = p.route->n_entries * p.k_stages;
+    }
+    const int first = (total * slice) >> p.split_log2;
+    const int nst = ((total * (slice + 1)) >> p.split_log2) - first;
+    // Tiles: GateUp the same rows of gate and up, else up to `halves` neighbours.
+    const int tile0 = M == Mode::GateUp ? group : group * p.halves;
+    const int nw = M == Mode::GateUp ? 2 : min(p.halves, p.tiles - tile0);
+    Geometry g = p.geo[kPerExpert ? ntok - 1 : 0];
+    uint8_t* const b_ring = ring + (size_t)g.w_slots * kWSlot;
+    // The last tile of an odd number runs alone in rings made for pairs: as
+    // many slots of weights as of activations.
+    if (M != Mode::GateUp && nw < p.halves) g.w_slots = min(g.w_slots, g.b_slots);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ copies
+        if (lane == 0) {
+            Cursor c, b;
+            int issued = 0;
+            bool ok = true;
+            const size_t sf_matrix = (size_t)p.tiles * (size_t)p.kblocks * 512;
+            int entry = 0, kb = first;
+            if constexpr (M == Mode::Down) {
+                entry = first / p.k_stages;
+                kb = first % p.k_stages;
+                if (nst > 0) expert = p.route->head[entry] & 0xFFFF;
+            }
+            // An Image kernel fills the ring with weights before it waits for
+            // the conversion; tile j's activations follow it when j is `late`.
+            int late = IMAGE ? min(nst * nw, g.w_slots) : 0;
+            auto load_image = [&](int i, uint64_t* bar) {
+                bulk_load(b_ring + (size_t)b.slot * g.b_slot, p.image + (size_t)(first + i) * g.image, g.image, bar);
+                b.advance(g.b_slots);
+            };
+            auto load_late = [&]() {
+                pdl_wait();
+                for (int j = 0; j < late; j += nw) load_image(nw == 2 ? j >> 1 : j, &sm.full[j]);
+                late = 0;
+            };
+            for (int i = 0; i < nst && ok; ++i) {
+                const uint32_t sf_bytes = 512u * (uint32_t)min(4, p.kblocks - 4 * kb);
+                for (int h = 0; h < nw; ++h) {
+                    if (!mbar_wait(&sm.empty[c.slot], c.phase ^ 1u, &sm.abort, 0x0601)) {
+                        ok = false;
+                        break;
+                    }
+                    const bool up = M == Mode::GateUp && h == 1;
+                    const int tile = M == Mode::GateUp ? tile0 : tile0 + h;
+                    uint8_t* st = ring + (size_t)c.slot * kWSlot;
+                    const uint8_t* sf = (up ? p.sf1 : p.sf0) + (size_t)expert * sf_matrix +
+                                        ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
+                    uint64_t* full = &sm.full[c.slot];
+                    mbar_arrive_expect_tx(full, kWBytes + sf_bytes + (IMAGE && h == 0 ? g.image : 0u));
+                    tma_load_2d(st, up ? &tm1 : &tm0, full, kb * 128, expert * p.N + tile * kTileRows);
+                    bulk_load(st + kWBytes, sf, sf_bytes, full);
+                    ++issued;
+                    if constexpr (IMAGE) {
+                        if (issued < late) {
+                            // more weights first
+                        } else if (late) {
+                            load_late();
+                        } else if (h == 0) {
+                            load_image(i, full);
+                        }
+                    }
+                    c.advance(g.w_slots);
+                }
+                ++kb;
+                if constexpr (M == Mode::Down) {
+                    if (kb == p.k_stages) {
+                        kb = 0;
+                        ++entry;
+                        if (i + 1 < nst) expert = p.route->head[entry] & 0xFFFF;
+                    }
+                }
+            }
+            if (late) load_late();
+            if (!ok || *(volatile int*)&sm.abort) {
+                // Drain: every issued copy must land before the block exits.
+                int dummy = 0;
+                for (int j = max(0, issued - g.w_slots); j < issued; ++j)
+                    mbar_wait(&sm.full[j % g.w_slots], (uint32_t)(j / g.w_slots) & 1u, &dummy, 0x0602, 100000000ull);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        // The whole warp runs the loop, so addresses and descriptors stay in
+        // uniform registers, and one elected lane issues.
+        if (nst > 0) {
+            const uint32_t idesc = idesc_nvf4(kTileRows, g.nb);
+            const uint64_t op_desc = desc_kmajor_sw128(0), sf_desc = smem_desc(0, 0, 128, 0);
+            const uint32_t sfa_col0 = tmem + (M == Mode::GateUp ? 2u : (uint32_t)p.halves) * g.acc_cols;
+            const uint32_t sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
+            const bool two = g.sfb_cols == 32;  // two 128-row halves of B scales
+            Cursor w, b;
+            bool ok = true;
+            int kb = M == Mode::Down ? first % p.k_stages : first;
+            for (int i = 0; i < nst && ok; ++i) {
+                const int nblk = min(4, p.kblocks - 4 * kb);
+                const uint32_t b_addr = smem_u32(b_ring) + (uint32_t)b.slot * g.b_slot;
+                const uint64_t b_desc = op_desc + (b_addr >> 4);
+                const uint64_t sfb_desc = sf_desc + ((b_addr + (uint32_t)g.nb * 128) >> 4);
+                const uint32_t sfb_col = sfb_col0 + (uint32_t)b.slot * g.sfb_cols;
+                const uint32_t sfb_step = g.sfb_step >> 4, sfb_next = two ? 8u : 4u;
+                for (int h = 0; h < nw; ++h) {
+                    ok = mbar_wait(&sm.full[w.slot], w.phase, &sm.abort, 0x0611);
+                    if (!ok) break;
+                    __syncwarp();
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(ring) + (uint32_t)w.slot * kWSlot;
+                    const uint64_t a_desc = op_desc + (a_addr >> 4);
+                    const uint64_t sfa_desc = sf_desc + ((a_addr + kWBytes) >> 4);
+                    const uint32_t sfa_col = sfa_col0 + (uint32_t)w.slot * 16;
+                    const uint32_t acc = tmem + (uint32_t)h * g.acc_cols;
+                    // A: K-block j at sfa_col + 4 j. B: K-block j at sfb_col + 4 j, or,
+                    // with two row halves, half q at sfb_col + 8 j + 4 q.
+                    auto scales_a = [&](int j) { tmem_cp_32x128b_warpx4(sfa_col + 4 * j, sfa_desc + 32 * j); };
+                    auto scales_b = [&](int j) {
+                        tmem_cp_32x128b_warpx4(sfb_col + sfb_next * j, sfb_desc + sfb_step * j);
+                        if (two) tmem_cp_32x128b_warpx4(sfb_col + 4 + 8 * j, sfb_desc + 128 + 32 * j);
+                    };
+                    auto product = [&](int j) {
+                        mma_nvf4(acc, a_desc + 2 * j, b_desc + 2 * j, idesc, sfa_col + 4 * j, sfb_col + sfb_next * j,
+                                 (i | j) != 0);
+                    };
+                    if (elect_one()) {
+                        if (nblk == 4) {
+                            if (h == 0) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) scales_b(j);
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) scales_a(j);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) product(j);
+                        } else {
+                            for (int j = 0; j < nblk; ++j) {
+                                if (h == 0) scales_b(j);
+                                scales_a(j);
+                            }
+                            for (int j = 0; j < nblk; ++j) product(j);
+                        }
+                        tc_commit(&sm.empty[w.slot]);
+                    }
+                    __syncwarp();
+                    w.advance(g.w_slots);
+                }
+                b.advance(g.b_slots);
+                if (++kb == p.k_stages && M == Mode::Down) kb = 0;
+            }
+            if (elect_one()) {
+                tc_commit(&sm.acc_full);
+                // Every MMA issued completes before TMEM is freed.
+                tc_commit(&sm.drain);
+            }
+            __syncwarp();
+            int dummy = 0;
+            mbar_wait(&sm.drain, 0, &dummy, 0x0613, 100000000ull);
+        }
+        __syncwarp();
+    } else {
+        const int w = (int)warp - 2;
+        if constexpr (IMAGE) {
+            pdl_wait();
+            if (w == 0) sm.amax[lane] = (int)lane < p.T ? p.amax[lane] : 0u;
+            named_sync(1, 128);
+        } else {
+        // ------------------------------------------------------------ activations
+        // Unit u = i * tokens + t, token t in stage i, is warp u % 8's. A lane
+        // holds eight elements of it; false: the token has none in the stage.
+        struct Unit {
+            int i, t;
+            int entry, kb;  // of the stage; Down only
+        };
+        auto load = [&](const Unit& n, uint4 (&r)[2]) -> bool {
+            const int kb = M == Mode::Down ? n.kb : first + n.i, t = n.t;
+            int row = t;
+            if constexpr (M == Mode::Down) {
+                row = p.route->slot[n.entry][t];
+            } else if constexpr (M == Mode::GateUp) {
+                row = sm.slot[t] / p.top;
+            } else if constexpr (M == Mode::DownPart) {
+                row = sm.slot[t];
+            }
+            const int k = kb * kStageK + (int)lane * 8;
+            r[0] = r[1] = make_uint4(0, 0, 0, 0);
+            if (row < 0) return false;
+            if (k < p.K) load_raw(static_cast<const XT*>(p.X) + (size_t)row * p.ldx + k, p.x_vec != 0, r);
+            return true;
+        };
+        // x / ntok for x <= 8, exactly.
+        const uint32_t inverse = p.inverse[ntok];
+        const int step_i = (int)(kConvWarps * inverse >> 16), step_t = kConvWarps - step_i * ntok;
+        auto next_unit = [&](Unit& u) {
+            const int was = u.i;
+            u.i += step_i;
+            u.t += step_t;
+            if (u.t >= ntok) {
+                u.t -= ntok;
+                ++u.i;
+            }
+            if constexpr (M == Mode::Down) {
+                u.kb += u.i - was;
+                while (u.kb >= p.k_stages) {
+                    u.kb -= p.k_stages;
+                    ++u.entry;
+                }
+            }
+        };
+        Unit first_unit;
+        first_unit.i = (int)((uint32_t)w * inverse >> 16);
+        first_unit.t = w - first_unit.i * ntok;
+        first_unit.entry = M == Mode::Down ? (first + first_unit.i) / p.k_stages : 0;
+        first_unit.kb = M == Mode::Down ? (first + first_unit.i) % p.k_stages : 0;
+        const int units = nst * ntok;
+        auto in_k = [&](const Unit& u) {
+            return (M == Mode::Down ? u.kb : first + u.i) * kStageK + (int)lane * 8 < p.K;
+        };
+        auto keep_max = [&](const uint4 (&r)[2], int t, bool valid) {
+            float v[8];
+            widen<XT>(r, v);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, max_bits(v));
+            if (lane == 0 && valid) atomicMax(&sm.amax[t], m);
+        };
+        // A slice of at most four units per warp that the ring holds whole
+        // stays in registers between the search for the largest magnitude
+        // and the conversion.
+        bool done = false;
+        if constexpr (M == Mode::Gemv) {
+            constexpr int kHeld = 4;
+            if (nst * nw <= g.w_slots && units <= kHeld * kConvWarps) {
+                uint4 r[kHeld][2];
+                Unit u = first_unit;
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c, next_unit(u))
+                    if (u.i < nst) load(u, r[c]);
+                u = first_unit;
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c, next_unit(u))
+                    if (u.i < nst) keep_max(r[c], u.t, true);
+                named_sync(1, 32 * kConvWarps);
+                u = first_unit;
+#pragma unroll
+                for (int c = 0; c < kHeld; ++c, next_unit(u)) {
+                    if (u.i >= nst) continue;
+                    float v[8];
+                    widen<XT>(r[c], v);
+                    uint8_t* b_rows = b_ring + (size_t)u.i * g.b_slot;
+                    convert(v, anchor_of(sm.amax[u.t]), u.t, in_k(u), b_rows, b_rows + (size_t)g.nb * 128, g.sfb_step,
+                            lane);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                // One arrival for each stage in which the warp had a token.
+                if (lane == 0)
+                    for (int i = 0; i < nst; ++i)
+                        if (((w - i * ntok) & (kConvWarps - 1)) < ntok)
+                            for (int h = 0; h < nw; ++h) mbar_arrive(&sm.full[i * nw + h]);
+                done = true;
+            }
+        }
+        if (!done) {
+            if (p.amax) {
+                if (w == 0 && (int)lane < ntok)
+                    sm.amax[lane] = p.amax[kPerExpert ? sm.slot[lane] / p.top : (int)lane];
+            } else {
+                Unit u = first_unit;
+                for (int u0 = w; u0 < units; u0 += 4 * kConvWarps) {
+                    uint4 r[4][2];
+                    int t[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c, next_unit(u)) {
+                        t[c] = u.t;
+                        r[c][0] = r[c][1] = make_uint4(0, 0, 0, 0);
+                        if (u.i < nst) load(u, r[c]);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) keep_max(r[c], t[c], u0 + c * kConvWarps < units);
+                }
+            }
+            if constexpr (M == Mode::Down) {
+                for (int i = w * 32 + (int)lane; i < kMaxSlots * kMaxTokens; i += 32 * kConvWarps)
+                    (&sm.dirty[0][0])[i] = 1;
+            }
+            named_sync(1, 32 * kConvWarps);
+            // Two units' elements are on their way while one is converted.
+            Unit cur = first_unit, ahead = first_unit;
+            uint4 r0[2], r1[2];
+            bool on0 = false, on1 = false;
+            if (ahead.i < nst) on0 = load(ahead, r0);
+            next_unit(ahead);
+            if (ahead.i < nst) on1 = load(ahead, r1);
+            Cursor c, b;
+            for (int i = 0; i < nst; ++i) {
+                // Every warp waits for every slot, whether or not it has a token
+                // in it: a barrier's parity tells one phase from the next only.
+                const int slot0 = c.slot;
+                bool ok = mbar_wait(&sm.empty[c.slot], c.phase ^ 1u, &sm.abort, 0x0621);
+                c.advance(g.w_slots);
+                const int slot1 = c.slot;
+                if (nw == 2) {
+                    ok = ok && mbar_wait(&sm.empty[c.slot], c.phase ^ 1u, &sm.abort, 0x0622);
+                    c.advance(g.w_slots);
+                }
+                if (!ok) break;
+                __syncwarp();
+                if (cur.i == i) {
+                    uint8_t* b_rows = b_ring + (size_t)b.slot * g.b_slot;
+                    uint8_t* sfb = b_rows + (size_t)g.nb * 128;
+                    const bool inside = in_k(cur);
+                    do {
+                        const int t = cur.t;
+                        float v[8];
+                        widen<XT>(r0, v);
+                        const bool on = on0;
+                        r0[0] = r1[0];
+                        r0[1] = r1[1];
+                        on0 = on1;
+                        next_unit(cur);
+                        next_unit(ahead);
+                        if (ahead.i < nst) on1 = load(ahead, r1);
+                        if (M != Mode::Down || on) {
+                            convert(v, anchor_of(sm.amax[t]), t, inside, b_rows, sfb, g.sfb_step, lane);
+                            if (M == Mode::Down && lane == 0) sm.dirty[b.slot][t] = 1;
+                        } else if (sm.dirty[b.slot][t]) {
+                            convert_zero(t, b_rows, sfb, g.sfb_step, lane);
+                            __syncwarp();
+                            if (lane == 0) sm.dirty[b.slot][t] = 0;
+                        }
+                    } while (cur.i == i);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&sm.full[slot0]);
+                        if (nw == 2) mbar_arrive(&sm.full[slot1]);
+                    }
+                }
+                b.advance(g.b_slots);
+            }
+        }
+        }
+        __syncwarp();
+        // ------------------------------------------------------------ partial sums
+        // Warps 2..5: a thread reads its row's columns, adds the planes and
+        // leaves the slice's sums in shared memory (over the rings, whose last
+        // use the accumulator barrier has seen complete).
+        if (w < 4) {
+            float* part = reinterpret_cast<float*>(ring);
+            const uint32_t quarter = warp & 3u;
+            const int row = (int)(quarter * 32 + lane);
+            if (nst > 0) {
+                mbar_wait(&sm.acc_full, 0, &sm.abort, 0x0631);
+                __syncwarp();
+                tc_fence_after();
+            }
+            for (int h = 0; h < nw; ++h, part += ntok * kTileRows) {
+                const float alpha = M == Mode::Gemv ? __ldg(p.alpha0)
+                                    : M == Mode::GateUp ? __ldg((h ? p.alpha1 : p.alpha0) + expert)
+                                                        : 1.0f;
+                const uint32_t acc = tmem + ((quarter * 32u) << 16) + (uint32_t)h * g.acc_cols;
+                for (int t0 = 0; t0 < ntok; t0 += 8) {
+                    if (nst == 0) {
+                        for (int t = t0; t < min(t0 + 8, ntok); ++t) part[t * kTileRows + row] = 0.0f;
+                        continue;
+                    }
+                    uint32_t c[5][8];
+#pragma unroll
+                    for (int i = 0; i < 5; ++i) tmem_ld_32x32b_x8(acc + (uint32_t)(kPlanes * t0 + 8 * i), c[i]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (t0 + i >= ntok) continue;
+                        auto col = [&](int n) { return __uint_as_float(c[n >> 3][n & 7]); };
+                        float s = col(5 * i + 4);
+#pragma unroll
+                        for (int q = 3; q >= 0; --q) s = __fmaf_rn(s, 0.125f, col(5 * i + q));
+                        const uint32_t mb = sm.amax[t0 + i];
+                        s = s * alpha * __uint_as_float((uint32_t)(anchor_of(mb) - 8 + 127) << 23);
+                        if (mb >= kInfBits) s = __uint_as_float(0x7FC00000u);
+                        part[(t0 + i) * kTileRows + row] = s;
+                    }
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncwarp();
+    cluster_sync();
+
+    // ---------------------------------------------------------------- slices
+    // The cluster's blocks share the rows out; slices add in rank order.
+    {
+        const int rows_log2 = 7 - p.split_log2, rows = 1 << rows_log2;  // 16 to 128
+        const uint32_t base = smem_u32(ring);
+        const int sums = ntok * rows;          // of one tile
+        if constexpr (M == Mode::GateUp) {
+            // sm.amax now gathers h's largest magnitudes.
+            __syncthreads();
+            if (threadIdx.x < kMaxTokens) sm.amax[threadIdx.x] = 0;
+            __syncthreads();
+        }
+        for (int i0 = (int)(warp * 32); i0 < (M == Mode::GateUp ? sums : nw * sums); i0 += kThreads<IMAGE>) {
+            const int i = i0 + (int)lane;
+            const int h = i >= sums ? 1 : 0, j = i - h * sums;
+            const int t = j >> rows_log2, r = slice * rows + (j & (rows - 1));
+            const int n = (tile0 + (M == Mode::GateUp ? 0 : h)) * kTileRows + r;
+            const bool valid = i < (M == Mode::GateUp ? sums : nw * sums) && n < p.N;
+            float s = 0.0f, u = 0.0f;
+            if (valid) {
+                const uint32_t off = base + (uint32_t)((h * ntok + t) * kTileRows + r) * 4u;
+                for (int c = 0; c < split; ++c) s += ld_cluster_f32(mapa_shared(off, (uint32_t)c));
+                if constexpr (M == Mode::GateUp)
+                    for (int c = 0; c < split; ++c)
+                        u += ld_cluster_f32(mapa_shared(off + (uint32_t)(ntok * kTileRows) * 4u, (uint32_t)c));
+            }
+            if constexpr (M == Mode::GateUp) {
+                uint32_t m = 0;
+                if (valid) {
+                    const int slot = sm.slot[t];
+                    const float hv = s / (1.0f + expf(-s)) * u * (p.weights[slot] * __ldg(p.alpha2 + expert));
+                    static_cast<float*>(p.Y)[(size_t)slot * p.ldy + n] = hv;
+                    m = __float_as_uint(hv) & 0x7FFFFFFFu;
+                }
+                // 16 neighbouring lanes have one token.
+#pragma unroll
+                for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                if ((lane & 15) == 0 && m) atomicMax(&sm.amax[t], m);
+            } else if (valid) {
+                if constexpr (M == Mode::Gemv)
+                    if (p.R) s += static_cast<float>(static_cast<const YT*>(p.R)[(size_t)t * p.ldr + n]);
+                const size_t row = M == Mode::DownPart ? sm.slot[t] : t;
+                static_cast<YT*>(p.Y)[row * p.ldy + n] = from_f32<YT>(s);
+            }
+        }
+        if constexpr (M == Mode::GateUp) {
+            __syncthreads();
+            // Maxima: the order of the atomics does not matter.
+            if ((int)threadIdx.x < ntok && sm.amax[threadIdx.x])
+                atomicMax(&p.amax_out[sm.slot[threadIdx.x] / p.top], sm.amax[threadIdx.x]);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // no block leaves while another may read its sums
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, p.tmem_cols);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+static inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// Shared memory and TMEM of a block: half an SM's, or all of it where the
+// accumulators of `tokens` tokens leave no room in half of TMEM.
+struct Shape {
+    int per_sm;
+    size_t smem;
+};
+
+// For up to `tokens` tokens in a block: exactly that many, or 1 to `tokens` with
+// a geometry for each.
+static Shape set_shape(Params& p, int tokens, bool each) {
+    const bool all = p.halves * ((kPlanes * tokens + 15) & ~15) > 128;
+    const size_t overhead = 1024 + ((sizeof(Control) + 127) & ~(size_t)127);
+    // 228 KiB per SM, 1 KiB of it reserved per block.
+    const size_t room = (all ? 227 * 1024 : (228 * 1024 - 2 * 1024) / 2) - overhead;
+    p.ring_bytes = (uint32_t)(room & ~(size_t)1023);
+    p.tmem_cols = all ? 512 : 256;
+    for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
+    if (!each) p.geo[0] = geometry(tokens, p.halves, p.ring_bytes, p.tmem_cols);
+    for (int t = 1; each && t <= tokens; ++t) p.geo[t - 1] = geometry(t, p.halves, p.ring_bytes, p.tmem_cols);
+    return {all ? 1 : 2, p.ring_bytes + overhead};
+}
+
+// Slices of K: the split whose waves of blocks, each as long as its stages and
+// about two more for its start and end, take the fewest stage times. `units`
+// blocks would run without a split, each of `stages` stages.
+static int choose_split_log2(double units, double stages, int max_split, int slots) {
+    int best = 0;
+    double best_cost = 0;
+    for (int l = 0, s = 1; s <= max_split; ++l, s *= 2) {
+        if (s > 1 && stages < s) break;
+        const double waves = (double)(long long)((units * s + slots - 1) / slots);
+        const double cost = waves * ((stages + s - 1) / s + 2.0);
+        if (s == 1 || cost < best_cost) {
+            best = l;
+            best_cost = cost;
+        }
+    }
+    return best;
+}
+
+template <Mode M, typename XT, typename YT, bool IMAGE = false>
+static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const Params& p, size_t smem, int clusters,
+                         cudaStream_t stream) {
+    auto kernel = stream_kernel<M, XT, YT, IMAGE>;
+    static thread_local uint64_t configured = 0;  // bit per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GPLK_STATUS_CUDA_ERROR;
+    if (!(configured & (1ull << dev))) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
+            return GPLK_STATUS_LAUNCH_FAIL;
+        configured |= 1ull << dev;
+    }
+        cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters << p.split_log2));
+    cfg.blockDim = dim3(kThreads<IMAGE>);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1u << p.split_log2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return launch_status(cudaLaunchKernelEx(&cfg, kernel, tm0, tm1, p));
+}
+
+// Tensor map of `rows` weight rows of K / 2 bytes, boxes of 128 rows x 128 bytes.
+static int encode_weights(CUtensorMap* map, const uint8_t* W, uint64_t rows, int K) {
+    return encode_tmap_2d_u8(map, W, (uint64_t)K / 2, rows, (uint64_t)K / 2, 128, kTileRows);
+}
+
+
+}  // namespace fewtok
+}  // namespace gplk

@@ -5,6 +5,7 @@
 #include "gplk_sgemm.cu"
 #include "gplk_gemm_pair.cu"
 #include "gplk_gemm_tc.cu"
+#include "gplk_nvfp4_stream.cu"
 #include "gplk_gemv_nvfp4.cu"
 #include "gplk_moe_nvfp4.cu"
 #include "gplk_powervirus.cu"
