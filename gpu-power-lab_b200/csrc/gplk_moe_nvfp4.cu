@@ -25,13 +25,6 @@ namespace moe {
 
 using namespace fewtok;
 
-// Whether the experts' down products go to sums of their own, per (token, rank)
-// slot, that a last kernel adds.
-static bool use_parts(int T) { return T > 8; }
-
-// Whether a block of the per-slot down products takes two tiles.
-static bool use_down_pairs(int T) { return T > 0; }
-
 // Workspace: every part starts on a 256-byte boundary.
 struct Layout {
     size_t route, amax, logits, ids, weights, h, part, total;
@@ -47,7 +40,7 @@ static Layout layout(int T, int E, int top, int D, int F) {
     l.weights = l.ids + up((size_t)T * top * 4);
     l.h = l.weights + up((size_t)T * top * 4);
     l.part = l.h + up((size_t)T * top * F * 4);
-    l.total = l.part + (use_parts(T) ? up((size_t)T * top * D * 4) : 0);
+    l.total = l.part + up((size_t)T * top * D * 4);
     return l;
 }
 
@@ -257,6 +250,365 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
     }
 }
 
+// ---------------------------------------------------------------- resident experts' products
+// With enough work for every SM, one block per SM walks over the items (an
+// entry's two tiles: gate and up of 128 features, or 256 rows of down), and its
+// roles run ahead of one another from item to item: the copies and the
+// conversion fill the rings with the next item's stages while the accumulators
+// (two sets) drain. stream_kernel starts a block per item instead, which costs
+// about 4 us of an SM's stream each; there K is split over a cluster, which is
+// what few items need.
+//   warp 0 copies, warp 1 MMAs, warps 2..9 convert, warps 10..13 epilogue
+constexpr int kItemThreads = 32 * 14;
+
+struct ItemControl {
+    uint64_t full[kMaxSlots];
+    uint64_t empty[kMaxSlots];
+    uint64_t acc_full[2];
+    uint64_t acc_empty[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort;
+};
+
+template <bool GATE_UP, typename XT>
+__global__ void __launch_bounds__(kItemThreads, 1)
+    item_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1,
+                const __grid_constant__ Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    ItemControl& sm = *reinterpret_cast<ItemControl*>(ring + p.ring_bytes);
+    const uint32_t warp = warp_id_uniform();
+    const uint32_t lane = lane_id();
+    const Geometry g = p.geo[0];  // for the most tokens an entry can have
+    uint8_t* const b_ring = ring + (size_t)g.w_slots * kWSlot;
+
+    if (threadIdx.x < kMaxSlots) {
+        mbar_init(&sm.full[threadIdx.x], 1 + kConvWarps);
+        mbar_init(&sm.empty[threadIdx.x], 1);
+        if (threadIdx.x < 2) {
+            mbar_init(&sm.acc_full[threadIdx.x], 1);
+            mbar_init(&sm.acc_empty[threadIdx.x], 4);
+        }
+        if (threadIdx.x == 0) {
+            mbar_init(&sm.drain, 1);
+            sm.abort = 0;
+            tma_prefetch_desc(&tm0);
+            if (GATE_UP) tma_prefetch_desc(&tm1);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&sm.tmem_base, p.tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+    // The down products follow a gate / up kernel that itself waited for the
+    // routing tables: those and weights may be read at once, h behind a
+    // pdl_wait() of the warps that read it.
+    if constexpr (GATE_UP) pdl_wait();
+    pdl_launch_dependents();
+    const int groups = GATE_UP ? p.tiles : (p.tiles + 1) / 2;
+    const int items = p.route->n_entries * groups;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ copies
+        if (lane == 0) {
+            Cursor c;
+            long issued = 0;
+            bool ok = true;
+            const size_t sf_matrix = (size_t)p.tiles * (size_t)p.kblocks * 512;
+            for (int it = (int)blockIdx.x; it < items && ok; it += (int)gridDim.x) {
+                const int group = it % groups, expert = p.route->head[it / groups] & 0xFFFF;
+                const int tile0 = GATE_UP ? group : 2 * group;
+                const int nw = GATE_UP || tile0 + 1 < p.tiles ? 2 : 1;
+                for (int kb = 0; kb < p.k_stages && ok; ++kb) {
+                    const uint32_t sf_bytes = 512u * (uint32_t)min(4, p.kblocks - 4 * kb);
+                    for (int h = 0; h < 2; ++h) {
+                        if (!mbar_wait(&sm.empty[c.slot], c.phase ^ 1u, &sm.abort, 0x0701)) {
+                            ok = false;
+                            break;
+                        }
+                        uint64_t* full = &sm.full[c.slot];
+                        if (h < nw) {
+                            const bool up = GATE_UP && h == 1;
+                            const int tile = GATE_UP ? tile0 : tile0 + h;
+                            uint8_t* st = ring + (size_t)c.slot * kWSlot;
+                            const uint8_t* sf = (up ? p.sf1 : p.sf0) + (size_t)expert * sf_matrix +
+                                                ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
+                            mbar_arrive_expect_tx(full, kWBytes + sf_bytes);
+                            tma_load_2d(st, up ? &tm1 : &tm0, full, kb * 128, expert * p.N + tile * kTileRows);
+                            bulk_load(st + kWBytes, sf, sf_bytes, full);
+                        } else {
+                            mbar_arrive(full);  // an odd last tile: its neighbour's slot stays as it is
+                        }
+                        ++issued;
+                        c.advance(g.w_slots);
+                    }
+                }
+            }
+            if (!ok || *(volatile int*)&sm.abort) {
+                int dummy = 0;
+                for (long j = issued > g.w_slots ? issued - g.w_slots : 0; j < issued; ++j)
+                    mbar_wait(&sm.full[j % g.w_slots], (uint32_t)(j / g.w_slots) & 1u, &dummy, 0x0702, 100000000ull);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        const uint64_t op_desc = desc_kmajor_sw128(0), sf_desc = smem_desc(0, 0, 128, 0);
+        const uint32_t sfa_col0 = tmem + 4u * g.acc_cols, sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
+        const uint32_t sfb_step = g.sfb_step >> 4;
+        Cursor w, b, acc;
+        bool ok = true;
+        for (int it = (int)blockIdx.x; it < items && ok; it += (int)gridDim.x) {
+            const int ntok = p.route->head[it / groups] >> 16;
+            const int tile0 = GATE_UP ? 0 : 2 * (it % groups);
+            const int nw = GATE_UP || tile0 + 1 < p.tiles ? 2 : 1;
+            const uint32_t idesc = idesc_nvf4(kTileRows, (kPlanes * ntok + 7) & ~7);
+            if (!mbar_wait(&sm.acc_empty[acc.slot], acc.phase ^ 1u, &sm.abort, 0x0711)) break;
+            __syncwarp();
+            tc_fence_after();
+            for (int kb = 0; kb < p.k_stages && ok; ++kb) {
+                const int nblk = min(4, p.kblocks - 4 * kb);
+                const uint32_t b_addr = smem_u32(b_ring) + (uint32_t)b.slot * g.b_slot;
+                const uint64_t b_desc = op_desc + (b_addr >> 4);
+                const uint64_t sfb_desc = sf_desc + ((b_addr + (uint32_t)g.nb * 128) >> 4);
+                const uint32_t sfb_col = sfb_col0 + (uint32_t)b.slot * 16;
+                for (int h = 0; h < 2; ++h) {
+                    ok = mbar_wait(&sm.full[w.slot], w.phase, &sm.abort, 0x0712);
+                    if (!ok) break;
+                    __syncwarp();
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(ring) + (uint32_t)w.slot * kWSlot;
+                    const uint64_t a_desc = op_desc + (a_addr >> 4);
+                    const uint64_t sfa_desc = sf_desc + ((a_addr + kWBytes) >> 4);
+                    const uint32_t sfa_col = sfa_col0 + (uint32_t)w.slot * 16;
+                    const uint32_t d = tmem + (uint32_t)(2 * acc.slot + h) * g.acc_cols;
+                    auto scales = [&](int j) {
+                        if (h == 0) tmem_cp_32x128b_warpx4(sfb_col + 4 * j, sfb_desc + sfb_step * j);
+                        tmem_cp_32x128b_warpx4(sfa_col + 4 * j, sfa_desc + 32 * j);
+                    };
+                    auto product = [&](int j) {
+                        mma_nvf4(d, a_desc + 2 * j, b_desc + 2 * j, idesc, sfa_col + 4 * j, sfb_col + 4 * j, (kb | j) != 0);
+                    };
+                    if (elect_one()) {
+                        if (h < nw) {
+                            if (nblk == 4) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) scales(j);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) product(j);
+                            } else {
+                                for (int j = 0; j < nblk; ++j) scales(j);
+                                for (int j = 0; j < nblk; ++j) product(j);
+                            }
+                        }
+                        tc_commit(&sm.empty[w.slot]);
+                    }
+                    __syncwarp();
+                    w.advance(g.w_slots);
+                }
+                b.advance(g.b_slots);
+            }
+            if (ok && elect_one()) tc_commit(&sm.acc_full[acc.slot]);
+            __syncwarp();
+            acc.advance(2);
+        }
+        // Every MMA issued completes before TMEM is freed.
+        if (elect_one()) tc_commit(&sm.drain);
+        __syncwarp();
+        int dummy = 0;
+        mbar_wait(&sm.drain, 0, &dummy, 0x0713, 100000000ull);
+        __syncwarp();
+    } else if (warp < 2 + kConvWarps) {
+        // ------------------------------------------------------------ activations
+        // Unit u = kb * tokens + t of an item is warp u % 8's.
+        const int w = (int)warp - 2;
+        if constexpr (!GATE_UP) pdl_wait();
+        struct Unit {
+            int it, kb, t, ntok, step_kb, step_t, entry;
+        };
+        auto enter = [&](Unit& u) {  // the unit is the first of the item, if any is left
+            while (u.it < items) {
+                u.entry = u.it / groups;
+                u.ntok = p.route->head[u.entry] >> 16;
+                const uint32_t inverse = p.inverse[u.ntok];
+                u.step_kb = (int)(kConvWarps * inverse >> 16);
+                u.step_t = kConvWarps - u.step_kb * u.ntok;
+                u.kb = (int)((uint32_t)w * inverse >> 16);
+                u.t = w - u.kb * u.ntok;
+                if (u.kb < p.k_stages) return;
+                u.it += (int)gridDim.x;
+            }
+        };
+        auto next_unit = [&](Unit& u) {
+            u.kb += u.step_kb;
+            u.t += u.step_t;
+            if (u.t >= u.ntok) {
+                u.t -= u.ntok;
+                ++u.kb;
+            }
+            if (u.kb >= p.k_stages) {
+                u.it += (int)gridDim.x;
+                enter(u);
+            }
+        };
+        // The lane's eight elements and the token's anchor.
+        auto load = [&](const Unit& u, uint4 (&r)[2], int& anchor) {
+            r[0] = r[1] = make_uint4(0, 0, 0, 0);
+            if (u.it >= items) return;
+            const int slot = p.route->list[u.entry][u.t];
+            const int row = GATE_UP ? slot / p.top : slot;
+            const int k = u.kb * kStageK + (int)lane * 8;
+            if (k < p.K) load_raw(static_cast<const XT*>(p.X) + (size_t)row * p.ldx + k, p.x_vec != 0, r);
+            anchor = anchor_of(p.amax[slot / p.top]);
+        };
+        Unit cur;
+        cur.it = (int)blockIdx.x;
+        enter(cur);
+        Unit ahead = cur;
+        uint4 r0[2], r1[2];
+        int a0 = 0, a1 = 0;
+        load(ahead, r0, a0);
+        if (ahead.it < items) next_unit(ahead);
+        load(ahead, r1, a1);
+        Cursor c, b;
+        bool ok = true;
+        for (int it = (int)blockIdx.x; it < items && ok; it += (int)gridDim.x) {
+            for (int kb = 0; kb < p.k_stages; ++kb) {
+                const int slot0 = c.slot;
+                ok = mbar_wait(&sm.empty[c.slot], c.phase ^ 1u, &sm.abort, 0x0721);
+                c.advance(g.w_slots);
+                const int slot1 = c.slot;
+                ok = ok && mbar_wait(&sm.empty[c.slot], c.phase ^ 1u, &sm.abort, 0x0722);
+                c.advance(g.w_slots);
+                if (!ok) break;
+                __syncwarp();
+                if (cur.it == it && cur.kb == kb) {
+                    uint8_t* b_rows = b_ring + (size_t)b.slot * g.b_slot;
+                    uint8_t* sfb = b_rows + (size_t)g.nb * 128;
+                    const bool inside = kb * kStageK + (int)lane * 8 < p.K;
+                    do {
+                        float v[8];
+                        widen<XT>(r0, v);
+                        const int t = cur.t, anchor = a0;
+                        r0[0] = r1[0];
+                        r0[1] = r1[1];
+                        a0 = a1;
+                        next_unit(cur);
+                        if (ahead.it < items) next_unit(ahead);
+                        load(ahead, r1, a1);
+                        convert(v, anchor, t, inside, b_rows, sfb, g.sfb_step, lane);
+                    } while (cur.it == it && cur.kb == kb);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    mbar_arrive(&sm.full[slot0]);
+                    mbar_arrive(&sm.full[slot1]);
+                }
+                b.advance(g.b_slots);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------ epilogue
+        // A thread has one row of both tiles.
+        if constexpr (!GATE_UP) pdl_wait();
+        const uint32_t quarter = warp & 3u;
+        const int row = (int)(quarter * 32 + lane);
+        Cursor acc;
+        for (int it = (int)blockIdx.x; it < items; it += (int)gridDim.x) {
+            const int entry = it / groups, group = it % groups, head = p.route->head[entry];
+            const int ntok = head >> 16, expert = head & 0xFFFF;
+            // Lane t: token t's slot, magnitude and, for gate / up, what h is scaled by.
+            const int my_slot = (int)lane < ntok ? p.route->list[entry][lane] : 0;
+            const uint32_t my_max = (int)lane < ntok ? p.amax[my_slot / p.top] : 0u;
+            float ag = 1.0f, au = 1.0f, my_scale = 1.0f;
+            if constexpr (GATE_UP) {
+                ag = p.alpha0[expert];
+                au = p.alpha1[expert];
+                my_scale = (int)lane < ntok ? p.weights[my_slot] * p.alpha2[expert] : 0.0f;
+            }
+            if (!mbar_wait_sleepy(&sm.acc_full[acc.slot], acc.phase, &sm.abort, 0x0731, false)) break;
+            __syncwarp();
+            tc_fence_after();
+            const uint32_t acc0 = tmem + ((quarter * 32u) << 16) + (uint32_t)(2 * acc.slot) * g.acc_cols;
+            for (int t0 = 0; t0 < ntok; t0 += 4) {  // 20 columns of each tile
+                uint32_t c0[3][8], c1[3][8];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    tmem_ld_32x32b_x8(acc0 + (uint32_t)(kPlanes * t0 + 8 * i), c0[i]);
+                    tmem_ld_32x32b_x8(acc0 + g.acc_cols + (uint32_t)(kPlanes * t0 + 8 * i), c1[i]);
+                }
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (t0 + i >= ntok) continue;
+                    float s = __uint_as_float(c0[(5 * i + 4) >> 3][(5 * i + 4) & 7]);
+                    float u = __uint_as_float(c1[(5 * i + 4) >> 3][(5 * i + 4) & 7]);
+#pragma unroll
+                    for (int q = 3; q >= 0; --q) {
+                        s = __fmaf_rn(s, 0.125f, __uint_as_float(c0[(5 * i + q) >> 3][(5 * i + q) & 7]));
+                        u = __fmaf_rn(u, 0.125f, __uint_as_float(c1[(5 * i + q) >> 3][(5 * i + q) & 7]));
+                    }
+                    const uint32_t mb = __shfl_sync(0xffffffffu, my_max, t0 + i);
+                    const int slot = __shfl_sync(0xffffffffu, my_slot, t0 + i);
+                    const float unit = __uint_as_float((uint32_t)(anchor_of(mb) - 8 + 127) << 23);
+                    s = s * ag * unit;
+                    u = u * au * unit;
+                    if (mb >= kInfBits) s = u = __uint_as_float(0x7FC00000u);
+                    float* y = static_cast<float*>(p.Y) + (size_t)slot * p.ldy;
+                    if constexpr (GATE_UP) {
+                        const int n = group * kTileRows + row;
+                        const float h = s / (1.0f + expf(-s)) * u * __shfl_sync(0xffffffffu, my_scale, t0 + i);
+                        if (n < p.N) y[n] = h;
+                        const uint32_t m = __reduce_max_sync(0xffffffffu, n < p.N ? __float_as_uint(h) & 0x7FFFFFFFu : 0u);
+                        if (lane == 0 && m) atomicMax(&p.amax_out[slot / p.top], m);
+                    } else {
+                        const int n = 2 * group * kTileRows + row;
+                        if (n < p.N) y[n] = s;
+                        if (n + kTileRows < p.N) y[n + kTileRows] = u;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.acc_empty[acc.slot]);
+            acc.advance(2);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, p.tmem_cols);
+    }
+}
+
+// Shared memory and TMEM of such a block: all of an SM's.
+static size_t set_item_shape(Params& p, int entry_tokens) {
+    const size_t overhead = 1024 + ((sizeof(ItemControl) + 127) & ~(size_t)127);
+    p.halves = 2;
+    p.ring_bytes = (uint32_t)((227 * 1024 - overhead) & ~(size_t)1023);
+    p.tmem_cols = 512;
+    for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
+    p.geo[0] = geometry(entry_tokens, 2, p.ring_bytes, p.tmem_cols, 2);
+    return p.ring_bytes + overhead;
+}
+
+template <bool GATE_UP, typename XT>
+static int launch_items(const CUtensorMap& tm0, const CUtensorMap& tm1, const Params& p, size_t smem, int blocks,
+                        cudaStream_t stream) {
+    static thread_local uint64_t configured = 0;  // bit per device
+    return launch_clusters(item_kernel<GATE_UP, XT>, &configured, blocks, kItemThreads, 1, smem, stream, tm0, tm1, p);
+}
+
 // y[t] = the sum of a token's slots, in the order of their ranks.
 template <typename XT>
 __global__ void __launch_bounds__(256) combine_kernel(const float* part, XT* y, int top, int D, int ldy) {
@@ -278,6 +630,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* part, XT* y, 
     row[2] = from_f32<XT>(s.z);
     row[3] = from_f32<XT>(s.w);
 }
+
+// Whether the experts' products run as resident blocks over `items`.
+static bool use_items(double items, int sm_count) { return items >= sm_count; }
 
 template <typename XT>
 static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t stream) {
@@ -309,7 +664,7 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     double active = c.E * (1.0 - miss);
     if (active < 1.0) active = 1.0;
 
-    const bool parts = use_parts(c.T);
+    const int entry_tokens = c.T < kMaxEntryTokens ? c.T : kMaxEntryTokens;
 
     Params g;
     memset(&g, 0, sizeof(g));
@@ -334,29 +689,39 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     g.tiles = (c.F + kTileRows - 1) / kTileRows;
     g.k_stages = (c.D + kStageK - 1) / kStageK;
     g.kblocks = c.D / 64;
-    g.halves = 2;
-    const int entry_tokens = c.T < kMaxEntryTokens ? c.T : kMaxEntryTokens;
-    const Shape gs = set_shape(g, entry_tokens, true);
     Params o = g;
     o.X = g.Y;
     o.amax = g.amax_out;
     o.sf0 = c.sf_down;
-    o.Y = parts ? static_cast<void*>(ws + l.part) : c.y;
     o.N = c.D;
     o.K = c.F;
     o.ldx = c.F;
-    o.ldy = parts ? c.D : c.ldy;
     o.x_vec = 1;
     o.tiles = (c.D + kTileRows - 1) / kTileRows;
     o.k_stages = (c.F + kStageK - 1) / kStageK;
     o.kblocks = c.F / 64;
-    o.halves = parts && use_down_pairs(c.T) ? 2 : 1;
-    const int groups = (o.tiles + o.halves - 1) / o.halves;
-    const Shape os = set_shape(o, parts ? entry_tokens : c.T, parts);
-    if (gs.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
-    g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, 8, gs.per_sm * d.sm_count);
-    o.split_log2 = parts ? choose_split_log2(groups * active, o.halves * o.k_stages, 8, os.per_sm * d.sm_count)
-                    : choose_split_log2(groups, o.halves * o.k_stages * active, 8, os.per_sm * d.sm_count);
+    const int pairs = (o.tiles + 1) / 2;
+    const bool g_items = use_items(active * g.tiles, d.sm_count), o_items = use_items(active * pairs, d.sm_count);
+    o.Y = o_items ? static_cast<void*>(ws + l.part) : c.y;
+    o.ldy = o_items ? c.D : c.ldy;
+    size_t g_smem, o_smem;
+    if (g_items) {
+        g_smem = set_item_shape(g, entry_tokens);
+    } else {
+        g.halves = 2;
+        const Shape s = set_shape(g, entry_tokens, true);
+        g_smem = s.smem;
+        g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, 8, s.per_sm * d.sm_count);
+    }
+    if (o_items) {
+        o_smem = set_item_shape(o, entry_tokens);
+    } else {
+        o.halves = 1;
+        const Shape s = set_shape(o, c.T, false);
+        o_smem = s.smem;
+        o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, 8, s.per_sm * d.sm_count);
+    }
+    if (g_smem > (size_t)d.max_smem_optin || o_smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
 
     CUtensorMap tg, tu, td;
     int st = encode_weights(&tg, c.gate, (uint64_t)c.E * c.F, c.D);
@@ -372,10 +737,11 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
         st = launch_status(launch_pdl(c.E <= 128 ? route_kernel<4> : route_kernel<kMaxExperts / 32>, dim3(1),
                                       dim3(32 * kMaxTokens), 0, stream, r));
     if (st == GPLK_STATUS_OK)
-        st = launch_stream<Mode::GateUp, XT, float>(tg, tu, g, gs.smem, max_entries * g.tiles, stream);
+        st = g_items ? launch_items<true, XT>(tg, tu, g, g_smem, d.sm_count, stream)
+                     : launch_stream<Mode::GateUp, XT, float>(tg, tu, g, g_smem, max_entries * g.tiles, stream);
     if (st != GPLK_STATUS_OK) return st;
-    if (!parts) return launch_stream<Mode::Down, float, XT>(td, td, o, os.smem, groups, stream);
-    st = launch_stream<Mode::DownPart, float, float>(td, td, o, os.smem, max_entries * groups, stream);
+    if (!o_items) return launch_stream<Mode::Down, float, XT>(td, td, o, o_smem, o.tiles, stream);
+    st = launch_items<false, float>(td, td, o, o_smem, d.sm_count, stream);
     if (st != GPLK_STATUS_OK) return st;
     return launch_status(launch_pdl(combine_kernel<XT>, dim3((c.D + 1023) / 1024, c.T), dim3(256), 0, stream,
                                     static_cast<const float*>(o.Y), static_cast<XT*>(c.y), c.top, c.D, c.ldy));

@@ -69,14 +69,13 @@ constexpr int kStageK = 256;                    // elements of K per slot
 constexpr uint32_t kWBytes = kTileRows * 128;   // codes of a weights' slot
 constexpr uint32_t kSfaBytes = 4 * 512;         // its scales
 constexpr uint32_t kWSlot = kWBytes + kSfaBytes;
-constexpr int kMaxSlots = 8;
+constexpr int kMaxSlots = 10;
 constexpr uint32_t kDigitBias = 4u * (1u + 8u + 64u + 512u + 4096u);
 
 // Gemv: all tokens against one matrix. GateUp: tokens of a chosen expert against
 // its gate and up matrices. Down: all tokens against every chosen expert's down
-// matrix, accumulated over the experts. DownPart: tokens of a chosen expert
-// against its down matrix.
-enum class Mode { Gemv, GateUp, Down, DownPart };
+// matrix, accumulated over the experts.
+enum class Mode { Gemv, GateUp, Down };
 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
@@ -113,7 +112,7 @@ struct Geometry {
 // slot free knows that tiles up to j - w are done; with b slots such that stage
 // i - b is among those, the activations' slot is free too: b = w for single
 // tiles, b = w / 2 + 1 for pairs.
-static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tmem_cols) {
+static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tmem_cols, int accs = 1) {
     Geometry g;
     g.nb = (kPlanes * ntok + 7) & ~7;
     const bool wide = g.nb > 128;  // a second 128 rows of B scales
@@ -127,7 +126,7 @@ static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tme
     for (g.w_slots = kMaxSlots; g.w_slots > 1; --g.w_slots) {
         g.b_slots = halves == 1 ? g.w_slots : g.w_slots / 2 + 1;
         if ((uint32_t)g.w_slots * kWSlot + (uint32_t)g.b_slots * g.b_slot <= ring_bytes &&
-            (uint32_t)halves * g.acc_cols + (uint32_t)g.w_slots * 16 + (uint32_t)g.b_slots * g.sfb_cols <= tmem_cols)
+            (uint32_t)(accs * halves) * g.acc_cols + (uint32_t)g.w_slots * 16 + (uint32_t)g.b_slots * g.sfb_cols <= tmem_cols)
             break;
     }
     return g;
@@ -346,7 +345,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     const int slice = (int)cluster_ctarank();
     const int split = 1 << p.split_log2;
     const int cid = (int)(blockIdx.x >> p.split_log2);
-    constexpr bool kPerExpert = M == Mode::GateUp || M == Mode::DownPart;
+    constexpr bool kPerExpert = M == Mode::GateUp;
 
     // Barriers and TMEM. A slot is full when the copies have landed and the
     // warps with tokens in the stage have converted them.
@@ -375,18 +374,20 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     if constexpr (!kPerExpert) set_up(p.T);
     // What is above may overlap the previous kernel's tail. The conversion
     // kernel that an Image kernel follows let it start only once every kernel
-    // before the two had completed, so weights may be read at once; what that
-    // kernel wrote is read behind a pdl_wait() of its own. Elsewhere nothing
-    // below touches global memory before the previous kernel has completed.
-    if constexpr (!IMAGE) pdl_wait();
+    // before the two had completed, so weights may be read at once, and what that
+    // kernel wrote is read behind a pdl_wait() of its own. A Down kernel follows
+    // a gate / up kernel that itself waited for the routing tables, so it may
+    // read those and weights at once. Elsewhere nothing below touches global
+    // memory before the previous kernel has completed.
+    constexpr bool kEarly = IMAGE || M == Mode::Down;
+    if constexpr (!kEarly) pdl_wait();
     pdl_launch_dependents();
 
     // This block's rows, tokens and stages.
     int group = cid, expert = 0, ntok = p.T, total = p.k_stages;
     if constexpr (kPerExpert) {
-        const int groups = M == Mode::GateUp ? p.tiles : (p.tiles + p.halves - 1) / p.halves;
-        const int a = cid / groups;
-        group = cid % groups;
+        const int a = cid / p.tiles;
+        group = cid % p.tiles;
         const int head = p.route->head[a];
         if (threadIdx.x < kMaxEntryTokens) sm.slot[threadIdx.x] = p.route->list[a][threadIdx.x];
         expert = head & 0xFFFF;
@@ -566,6 +567,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             named_sync(1, 128);
         } else {
         // ------------------------------------------------------------ activations
+        if constexpr (kEarly) pdl_wait();
         // Unit u = i * tokens + t, token t in stage i, is warp u % 8's. A lane
         // holds eight elements of it; false: the token has none in the stage.
         struct Unit {
@@ -579,8 +581,6 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 row = p.route->slot[n.entry][t];
             } else if constexpr (M == Mode::GateUp) {
                 row = sm.slot[t] / p.top;
-            } else if constexpr (M == Mode::DownPart) {
-                row = sm.slot[t];
             }
             const int k = kb * kStageK + (int)lane * 8;
             r[0] = r[1] = make_uint4(0, 0, 0, 0);
@@ -828,8 +828,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             } else if (valid) {
                 if constexpr (M == Mode::Gemv)
                     if (p.R) s += static_cast<float>(static_cast<const YT*>(p.R)[(size_t)t * p.ldr + n]);
-                const size_t row = M == Mode::DownPart ? sm.slot[t] : t;
-                static_cast<YT*>(p.Y)[row * p.ldy + n] = from_f32<YT>(s);
+                static_cast<YT*>(p.Y)[(size_t)t * p.ldy + n] = from_f32<YT>(s);
             }
         }
         if constexpr (M == Mode::GateUp) {
@@ -892,33 +891,40 @@ static int choose_split_log2(double units, double stages, int max_split, int slo
     return best;
 }
 
-template <Mode M, typename XT, typename YT, bool IMAGE = false>
-static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const Params& p, size_t smem, int clusters,
-                         cudaStream_t stream) {
-    auto kernel = stream_kernel<M, XT, YT, IMAGE>;
-    static thread_local uint64_t configured = 0;  // bit per device
+// Launches a kernel of this family in clusters of `csize` blocks.
+static int launch_clusters(void (*kernel)(CUtensorMap, CUtensorMap, Params), uint64_t* configured, int blocks,
+                           int threads, int csize, size_t smem, cudaStream_t stream, const CUtensorMap& tm0,
+                           const CUtensorMap& tm1, const Params& p) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GPLK_STATUS_CUDA_ERROR;
-    if (!(configured & (1ull << dev))) {
+    if (!(*configured & (1ull << dev))) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess)
             return GPLK_STATUS_LAUNCH_FAIL;
-        configured |= 1ull << dev;
+        *configured |= 1ull << dev;
     }
-        cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(clusters << p.split_log2));
-    cfg.blockDim = dim3(kThreads<IMAGE>);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 1u << p.split_log2;
+    attr[1].val.clusterDim.x = (unsigned)csize;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     return launch_status(cudaLaunchKernelEx(&cfg, kernel, tm0, tm1, p));
+}
+
+template <Mode M, typename XT, typename YT, bool IMAGE = false>
+static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const Params& p, size_t smem, int clusters,
+                         cudaStream_t stream) {
+    static thread_local uint64_t configured = 0;  // bit per device
+    return launch_clusters(stream_kernel<M, XT, YT, IMAGE>, &configured, clusters << p.split_log2, kThreads<IMAGE>,
+                           1 << p.split_log2, smem, stream, tm0, tm1, p);
 }
 
 // Tensor map of `rows` weight rows of K / 2 bytes, boxes of 128 rows x 128 bytes.
