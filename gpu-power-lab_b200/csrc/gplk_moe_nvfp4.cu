@@ -258,11 +258,13 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
 // (two sets) drain. stream_kernel starts a block per item instead, which costs
 // about 4 us of an SM's stream each; there K is split over a cluster, which is
 // what few items need.
-//   warp 0 copies, warp 1 MMAs, warps 2..9 convert, warps 10..13 epilogue
-constexpr int kItemThreads = 32 * 14;
+//   warp 0 copies, warp 1 MMAs, warps 2..9 convert, warps 10..13 epilogue,
+//   warps 14..17 scales to TMEM
+constexpr int kItemThreads = 32 * 18;
 
 struct ItemControl {
     uint64_t full[kMaxSlots];
+    uint64_t scaled[kMaxSlots];
     uint64_t empty[kMaxSlots];
     uint64_t acc_full[2];
     uint64_t acc_empty[2];
@@ -285,6 +287,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
 
     if (threadIdx.x < kMaxSlots) {
         mbar_init(&sm.full[threadIdx.x], 1 + kConvWarps);
+        mbar_init(&sm.scaled[threadIdx.x], 4);
         mbar_init(&sm.empty[threadIdx.x], 1);
         if (threadIdx.x < 2) {
             mbar_init(&sm.acc_full[threadIdx.x], 1);
@@ -311,6 +314,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     // pdl_wait() of the warps that read it.
     if constexpr (GATE_UP) pdl_wait();
     pdl_launch_dependents();
+    const uint32_t sfa_col0 = tmem + 4u * g.acc_cols, sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
     const int groups = GATE_UP ? p.tiles : (p.tiles + 1) / 2;
     const int items = p.route->n_entries * groups;
 
@@ -359,9 +363,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        const uint64_t op_desc = desc_kmajor_sw128(0), sf_desc = smem_desc(0, 0, 128, 0);
-        const uint32_t sfa_col0 = tmem + 4u * g.acc_cols, sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
-        const uint32_t sfb_step = g.sfb_step >> 4;
+        const uint64_t op_desc = desc_kmajor_sw128(0);
         Cursor w, b, acc;
         bool ok = true;
         for (int it = (int)blockIdx.x; it < items && ok; it += (int)gridDim.x) {
@@ -376,34 +378,26 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                 const int nblk = min(4, p.kblocks - 4 * kb);
                 const uint32_t b_addr = smem_u32(b_ring) + (uint32_t)b.slot * g.b_slot;
                 const uint64_t b_desc = op_desc + (b_addr >> 4);
-                const uint64_t sfb_desc = sf_desc + ((b_addr + (uint32_t)g.nb * 128) >> 4);
-                const uint32_t sfb_col = sfb_col0 + (uint32_t)b.slot * 16;
+                const uint32_t sfb_col = sfb_col0 + (uint32_t)b.slot * g.sfb_cols;
                 for (int h = 0; h < 2; ++h) {
-                    ok = mbar_wait(&sm.full[w.slot], w.phase, &sm.abort, 0x0712);
+                    ok = mbar_wait(&sm.scaled[w.slot], w.phase, &sm.abort, 0x0712);
                     if (!ok) break;
                     __syncwarp();
                     tc_fence_after();
                     const uint32_t a_addr = smem_u32(ring) + (uint32_t)w.slot * kWSlot;
                     const uint64_t a_desc = op_desc + (a_addr >> 4);
-                    const uint64_t sfa_desc = sf_desc + ((a_addr + kWBytes) >> 4);
                     const uint32_t sfa_col = sfa_col0 + (uint32_t)w.slot * 16;
                     const uint32_t d = tmem + (uint32_t)(2 * acc.slot + h) * g.acc_cols;
-                    auto scales = [&](int j) {
-                        if (h == 0) tmem_cp_32x128b_warpx4(sfb_col + 4 * j, sfb_desc + sfb_step * j);
-                        tmem_cp_32x128b_warpx4(sfa_col + 4 * j, sfa_desc + 32 * j);
-                    };
                     auto product = [&](int j) {
-                        mma_nvf4(d, a_desc + 2 * j, b_desc + 2 * j, idesc, sfa_col + 4 * j, sfb_col + 4 * j, (kb | j) != 0);
+                        mma_nvf4(d, a_desc + 2 * j, b_desc + 2 * j, idesc, sfa_col + 4 * j, sfb_col + 4 * j,
+                                 (kb | j) != 0);
                     };
                     if (elect_one()) {
                         if (h < nw) {
                             if (nblk == 4) {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) scales(j);
-#pragma unroll
                                 for (int j = 0; j < 4; ++j) product(j);
                             } else {
-                                for (int j = 0; j < nblk; ++j) scales(j);
                                 for (int j = 0; j < nblk; ++j) product(j);
                             }
                         }
@@ -510,6 +504,28 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                 if (lane == 0) {
                     mbar_arrive(&sm.full[slot0]);
                     mbar_arrive(&sm.full[slot1]);
+                }
+                b.advance(g.b_slots);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 6 + kConvWarps) {
+        // ------------------------------------------------------------ scales
+        Cursor c, b;
+        bool ok = true;
+        const uint32_t quarter = (warp & 3u) << 21;
+        for (int it = (int)blockIdx.x; it < items && ok; it += (int)gridDim.x) {
+            for (int kb = 0; kb < p.k_stages && ok; ++kb) {
+                for (int h = 0; h < 2; ++h) {
+                    ok = mbar_wait(&sm.full[c.slot], c.phase, &sm.abort, 0x0741);
+                    if (!ok) break;
+                    __syncwarp();
+                    scales_to_tmem(ring + (size_t)c.slot * kWSlot + kWBytes, sfa_col0 + (uint32_t)c.slot * 16 + quarter,
+                                   b_ring + (size_t)b.slot * g.b_slot + (size_t)g.nb * 128,
+                                   sfb_col0 + (uint32_t)b.slot * g.sfb_cols + quarter, g.sfb_step,
+                                   h == 0 ? g.sfb_cols : 0u, lane);
+                    if (lane == 0) mbar_arrive(&sm.scaled[c.slot]);
+                    c.advance(g.w_slots);
                 }
                 b.advance(g.b_slots);
             }

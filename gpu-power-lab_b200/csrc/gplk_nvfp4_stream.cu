@@ -40,8 +40,8 @@
 //   warps 2..9  convert the same 256 elements of every token into a slot of
 //               the activations' ring (a warp per token and slot); warps 2..5
 //               then read the accumulators, and all warps add the slices.
-//               In an Image kernel there are warps 2..5 only, and one thread
-//               of them fetches slots that another kernel converted.
+//               An Image kernel copies what another kernel converted; it has
+//               warps 2..5 only, and they bring the scales to TMEM.
 // The MMA warp runs its loop converged and elects the issuing lane: with
 // addresses and descriptors in uniform registers, 65536 x 8192 at one token
 // takes 51 us; issued from a lane of a diverged warp 76 us.
@@ -116,8 +116,10 @@ static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tme
     Geometry g;
     g.nb = (kPlanes * ntok + 7) & ~7;
     const bool wide = g.nb > 128;  // a second 128 rows of B scales
-    // A scale copy reads 512 bytes, 16 per row; with up to 32 rows the blocks
-    // lie as close as their rows, and a copy's rest is never used.
+    // Four blocks of B scales, one per 64 elements of K: 32 lanes of 16 bytes, the
+    // scales of rows r, r + 32, r + 64 and r + 96 (and four more for a second 128
+    // rows). With up to 32 rows the blocks lie as close as their rows; what a copy
+    // of 512 bytes then takes from the next block is never used.
     g.sfb_step = g.nb <= 32 ? 16u * (uint32_t)g.nb : 512u;
     g.image = (uint32_t)g.nb * 128 + (wide ? 4096u : 3 * g.sfb_step + 512);
     g.b_slot = (g.image + 1023) & ~1023u;
@@ -162,6 +164,7 @@ struct Params {
 
 struct Control {
     uint64_t full[kMaxSlots];   // by weights' slot
+    uint64_t scaled[kMaxSlots]; // Image kernels: full, and its scales are in TMEM
     uint64_t empty[kMaxSlots];
     uint64_t acc_full;
     uint64_t drain;
@@ -202,10 +205,36 @@ __device__ __forceinline__ bool elect_one() {
     return e != 0;
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
     return v;
+}
+
+// Sum of the four floats at the same place of the cluster's n blocks (1, 2, 4 or
+// 8), added in rank order, four loads on their way at a time.
+__device__ __forceinline__ float4 sum_cluster(uint32_t addr, int n) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int c0 = 0; c0 < 8; c0 += 4) {
+        if (c0 >= n) break;
+        float4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (c < n) v[c] = ld_cluster_f32x4(mapa_shared(addr, (uint32_t)(c0 + c)));
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (c < n) {
+                s.x += v[c].x;
+                s.y += v[c].y;
+                s.z += v[c].z;
+                s.w += v[c].w;
+            }
+    }
+    return s;
 }
 
 // Eight consecutive activations of one lane.
@@ -279,7 +308,7 @@ __device__ __forceinline__ uint32_t digit_codes(uint32_t w) {
 }
 
 // Byte of row r's scale for a lane's 16-group: one block per 64 elements, with
-// 16 bytes per row of 32 and 4 per further 32 rows, as the scale copy reads it.
+// 16 bytes per row of 32 and 4 per further 32 rows, as the MMA wants them in TMEM.
 __device__ __forceinline__ uint32_t sfb_offset(uint32_t r, uint32_t lane, uint32_t step) {
     return (r >> 7) * 2048 + (lane >> 3) * step + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((lane >> 1) & 3);
 }
@@ -331,6 +360,36 @@ __device__ __forceinline__ void convert_zero(int t, uint8_t* b_rows, uint8_t* sf
     }
 }
 
+// A stage's scales from shared memory to one warp's 32 TMEM lanes, which the four
+// warps of a group do with the same data, as the MMA wants it. (tcgen05.cp does
+// all four at once, but in the MMAs' own queue, where each copy takes about as
+// long as an MMA of 8 columns: at 25 tokens, 16384 x 8192 out of L2, XXX.)
+__device__ __forceinline__ void scales_to_tmem(const uint8_t* sfa, uint32_t sfa_col, const uint8_t* sfb,
+                                               uint32_t sfb_col, uint32_t sfb_step, uint32_t sfb_cols,
+                                               uint32_t lane) {
+    auto put = [&](uint32_t col, const uint8_t* block) {
+        const uint4 v = *reinterpret_cast<const uint4*>(block + lane * 16);
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(col), "r"(v.x), "r"(v.y),
+                     "r"(v.z), "r"(v.w)
+                     : "memory");
+    };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put(sfa_col + 4 * j, sfa + 512 * j);
+    if (sfb_cols == 16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put(sfb_col + 4 * j, sfb + sfb_step * j);
+    } else if (sfb_cols == 32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            put(sfb_col + 8 * j, sfb + 512 * j);
+            put(sfb_col + 8 * j + 4, sfb + 2048 + 512 * j);
+        }
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    tc_fence_before();
+    __syncwarp();
+}
+
 template <bool IMAGE>
 constexpr int kThreads = IMAGE ? 64 + 128 : 64 + 32 * kConvWarps;
 
@@ -353,6 +412,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         if (threadIdx.x < kMaxSlots) {
             const int i = (int)threadIdx.x;
             mbar_init(&sm.full[i], IMAGE ? 1u : 1u + (uint32_t)min(ntok, kConvWarps));
+            mbar_init(&sm.scaled[i], 4);
             mbar_init(&sm.empty[i], 1);
             if (i == 0) {
                 mbar_init(&sm.acc_full, 1);
@@ -411,6 +471,8 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
+    const uint32_t sfa_col0 = tmem + (M == Mode::GateUp ? 2u : (uint32_t)p.halves) * g.acc_cols;
+    const uint32_t sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
 
     if (warp == 0) {
         // ------------------------------------------------------------ copies
@@ -490,9 +552,9 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         if (nst > 0) {
             const uint32_t idesc = idesc_nvf4(kTileRows, g.nb);
             const uint64_t op_desc = desc_kmajor_sw128(0), sf_desc = smem_desc(0, 0, 128, 0);
-            const uint32_t sfa_col0 = tmem + (M == Mode::GateUp ? 2u : (uint32_t)p.halves) * g.acc_cols;
-            const uint32_t sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
-            const bool two = g.sfb_cols == 32;  // two 128-row halves of B scales
+            // A: K-block j at sfa_col + 4 j. B: K-block j at sfb_col + 4 j, or, with
+            // two row halves, half q at sfb_col + 8 j + 4 q.
+            const uint32_t sfb_step = g.sfb_step >> 4, sfb_next = g.sfb_cols / 4;
             Cursor w, b;
             bool ok = true;
             int kb = M == Mode::Down ? first % p.k_stages : first;
@@ -502,9 +564,8 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 const uint64_t b_desc = op_desc + (b_addr >> 4);
                 const uint64_t sfb_desc = sf_desc + ((b_addr + (uint32_t)g.nb * 128) >> 4);
                 const uint32_t sfb_col = sfb_col0 + (uint32_t)b.slot * g.sfb_cols;
-                const uint32_t sfb_step = g.sfb_step >> 4, sfb_next = two ? 8u : 4u;
                 for (int h = 0; h < nw; ++h) {
-                    ok = mbar_wait(&sm.full[w.slot], w.phase, &sm.abort, 0x0611);
+                    ok = mbar_wait(IMAGE ? &sm.scaled[w.slot] : &sm.full[w.slot], w.phase, &sm.abort, 0x0611);
                     if (!ok) break;
                     __syncwarp();
                     tc_fence_after();
@@ -513,32 +574,31 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     const uint64_t sfa_desc = sf_desc + ((a_addr + kWBytes) >> 4);
                     const uint32_t sfa_col = sfa_col0 + (uint32_t)w.slot * 16;
                     const uint32_t acc = tmem + (uint32_t)h * g.acc_cols;
-                    // A: K-block j at sfa_col + 4 j. B: K-block j at sfb_col + 4 j, or,
-                    // with two row halves, half q at sfb_col + 8 j + 4 q.
-                    auto scales_a = [&](int j) { tmem_cp_32x128b_warpx4(sfa_col + 4 * j, sfa_desc + 32 * j); };
-                    auto scales_b = [&](int j) {
-                        tmem_cp_32x128b_warpx4(sfb_col + sfb_next * j, sfb_desc + sfb_step * j);
-                        if (two) tmem_cp_32x128b_warpx4(sfb_col + 4 + 8 * j, sfb_desc + 128 + 32 * j);
-                    };
+                    auto scales = [&](int j) { tmem_cp_32x128b_warpx4(sfa_col + 4 * j, sfa_desc + 32 * j); };
                     auto product = [&](int j) {
                         mma_nvf4(acc, a_desc + 2 * j, b_desc + 2 * j, idesc, sfa_col + 4 * j, sfb_col + sfb_next * j,
                                  (i | j) != 0);
                     };
                     if (elect_one()) {
-                        if (nblk == 4) {
+                        if constexpr (!IMAGE) {
                             if (h == 0) {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) scales_b(j);
+                                for (int j = 0; j < 4; ++j) {
+                                    tmem_cp_32x128b_warpx4(sfb_col + sfb_next * j, sfb_desc + sfb_step * j);
+                                    if (sfb_next == 8u) tmem_cp_32x128b_warpx4(sfb_col + 4 + 8 * j, sfb_desc + 128 + 32 * j);
+                                }
                             }
+                        }
+                        if (nblk == 4) {
+                            if constexpr (!IMAGE) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) scales_a(j);
+                                for (int j = 0; j < 4; ++j) scales(j);
+                            }
 #pragma unroll
                             for (int j = 0; j < 4; ++j) product(j);
                         } else {
-                            for (int j = 0; j < nblk; ++j) {
-                                if (h == 0) scales_b(j);
-                                scales_a(j);
-                            }
+                            if constexpr (!IMAGE)
+                                for (int j = 0; j < nblk; ++j) scales(j);
                             for (int j = 0; j < nblk; ++j) product(j);
                         }
                         tc_commit(&sm.empty[w.slot]);
@@ -565,6 +625,25 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             pdl_wait();
             if (w == 0) sm.amax[lane] = (int)lane < p.T ? p.amax[lane] : 0u;
             named_sync(1, 128);
+            Cursor c, b;
+            bool ok = true;
+            for (int i = 0; i < nst && ok; ++i) {
+                for (int h = 0; h < nw; ++h) {
+                    ok = mbar_wait(&sm.full[c.slot], c.phase, &sm.abort, 0x0624);
+                    if (!ok) break;
+                    __syncwarp();
+                    const uint8_t* sfb = b_ring + (size_t)b.slot * g.b_slot + (size_t)g.nb * 128;
+                    scales_to_tmem(ring + (size_t)c.slot * kWSlot + kWBytes,
+                                   sfa_col0 + (uint32_t)c.slot * 16 + ((warp & 3u) << 21), sfb,
+                                   sfb_col0 + (uint32_t)b.slot * g.sfb_cols + ((warp & 3u) << 21),
+                                   g.sfb_step,
+                                   h == 0 ? g.sfb_cols : 0u, lane);
+                    if (lane == 0) mbar_arrive(&sm.scaled[c.slot]);
+                    c.advance(g.w_slots);
+                }
+                b.advance(g.b_slots);
+            }
+            __syncwarp();
         } else {
         // ------------------------------------------------------------ activations
         if constexpr (kEarly) pdl_wait();
@@ -746,6 +825,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         // use the accumulator barrier has seen complete).
         if (w < 4) {
             float* part = reinterpret_cast<float*>(ring);
+            const bool direct = M != Mode::GateUp && split == 1;
             const uint32_t quarter = warp & 3u;
             const int row = (int)(quarter * 32 + lane);
             if (nst > 0) {
@@ -766,6 +846,16 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     uint32_t c[5][8];
 #pragma unroll
                     for (int i = 0; i < 5; ++i) tmem_ld_32x32b_x8(acc + (uint32_t)(kPlanes * t0 + 8 * i), c[i]);
+                    // With one slice the sums are final: no other block has a part.
+                    const int n = (tile0 + h) * kTileRows + row;
+                    float r[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        r[i] = 0.0f;
+                        if constexpr (M == Mode::Gemv)
+                            if (direct && p.R && t0 + i < ntok && n < p.N)
+                                r[i] = static_cast<float>(static_cast<const YT*>(p.R)[(size_t)(t0 + i) * p.ldr + n]);
+                    }
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -777,7 +867,8 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                         const uint32_t mb = sm.amax[t0 + i];
                         s = s * alpha * __uint_as_float((uint32_t)(anchor_of(mb) - 8 + 127) << 23);
                         if (mb >= kInfBits) s = __uint_as_float(0x7FC00000u);
-                        part[(t0 + i) * kTileRows + row] = s;
+                        if (!direct) part[(t0 + i) * kTileRows + row] = s;
+                        else if (n < p.N) static_cast<YT*>(p.Y)[(size_t)(t0 + i) * p.ldy + n] = from_f32<YT>(s + r[i]);
                     }
                 }
             }
@@ -790,45 +881,56 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     // ---------------------------------------------------------------- slices
     // The cluster's blocks share the rows out; slices add in rank order.
     {
-        const int rows_log2 = 7 - p.split_log2, rows = 1 << rows_log2;  // 16 to 128
+        // A thread has four rows of a token at a time.
+        const int rows = kTileRows >> p.split_log2;  // 16 to 128
         const uint32_t base = smem_u32(ring);
-        const int sums = ntok * rows;          // of one tile
+        const int sums = (ntok * rows) >> 2;  // of one tile, in fours
+        const int fours = M == Mode::GateUp ? sums : split == 1 ? 0 : nw * sums;
         if constexpr (M == Mode::GateUp) {
             // sm.amax now gathers h's largest magnitudes.
             __syncthreads();
             if (threadIdx.x < kMaxTokens) sm.amax[threadIdx.x] = 0;
             __syncthreads();
         }
-        for (int i0 = (int)(warp * 32); i0 < (M == Mode::GateUp ? sums : nw * sums); i0 += kThreads<IMAGE>) {
-            const int i = i0 + (int)lane;
-            const int h = i >= sums ? 1 : 0, j = i - h * sums;
-            const int t = j >> rows_log2, r = slice * rows + (j & (rows - 1));
+        for (int i = (int)threadIdx.x; i < fours; i += kThreads<IMAGE>) {
+            const int h = i >= sums ? 1 : 0, j = (i - h * sums) << 2;
+            const int t = j >> (7 - p.split_log2), r = slice * rows + (j & (rows - 1));
             const int n = (tile0 + (M == Mode::GateUp ? 0 : h)) * kTileRows + r;
-            const bool valid = i < (M == Mode::GateUp ? sums : nw * sums) && n < p.N;
-            float s = 0.0f, u = 0.0f;
-            if (valid) {
-                const uint32_t off = base + (uint32_t)((h * ntok + t) * kTileRows + r) * 4u;
-                for (int c = 0; c < split; ++c) s += ld_cluster_f32(mapa_shared(off, (uint32_t)c));
-                if constexpr (M == Mode::GateUp)
-                    for (int c = 0; c < split; ++c)
-                        u += ld_cluster_f32(mapa_shared(off + (uint32_t)(ntok * kTileRows) * 4u, (uint32_t)c));
-            }
+            if (n >= p.N) continue;
+            const uint32_t off = base + (uint32_t)((h * ntok + t) * kTileRows + r) * 4u;
             if constexpr (M == Mode::GateUp) {
+                const float4 s4 = sum_cluster(off, split);
+                const float4 u4 = sum_cluster(off + (uint32_t)(ntok * kTileRows) * 4u, split);
+                const int slot = sm.slot[t];
+                const float c = p.weights[slot] * __ldg(p.alpha2 + expert);
+                const float s[4] = {s4.x, s4.y, s4.z, s4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+                float hv[4];
                 uint32_t m = 0;
-                if (valid) {
-                    const int slot = sm.slot[t];
-                    const float hv = s / (1.0f + expf(-s)) * u * (p.weights[slot] * __ldg(p.alpha2 + expert));
-                    static_cast<float*>(p.Y)[(size_t)slot * p.ldy + n] = hv;
-                    m = __float_as_uint(hv) & 0x7FFFFFFFu;
-                }
-                // 16 neighbouring lanes have one token.
 #pragma unroll
-                for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                if ((lane & 15) == 0 && m) atomicMax(&sm.amax[t], m);
-            } else if (valid) {
-                if constexpr (M == Mode::Gemv)
-                    if (p.R) s += static_cast<float>(static_cast<const YT*>(p.R)[(size_t)t * p.ldr + n]);
-                static_cast<YT*>(p.Y)[(size_t)t * p.ldy + n] = from_f32<YT>(s);
+                for (int q = 0; q < 4; ++q) {
+                    hv[q] = s[q] / (1.0f + expf(-s[q])) * u[q] * c;
+                    m = max(m, __float_as_uint(hv[q]) & 0x7FFFFFFFu);
+                }
+                // F is a multiple of 64, so the four are all inside.
+                *reinterpret_cast<float4*>(static_cast<float*>(p.Y) + (size_t)slot * p.ldy + n) =
+                    make_float4(hv[0], hv[1], hv[2], hv[3]);
+                if (m) atomicMax(&sm.amax[t], m);
+            } else {
+                const float4 s4 = sum_cluster(off, split);
+                const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+                YT* y = static_cast<YT*>(p.Y) + (size_t)t * p.ldy + n;
+                float res[4] = {};
+                if constexpr (M == Mode::Gemv) {
+                    if (p.R) {
+                        const YT* rr = static_cast<const YT*>(p.R) + (size_t)t * p.ldr + n;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (n + q < p.N) res[q] = static_cast<float>(rr[q]);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (n + q < p.N) y[q] = from_f32<YT>(s[q] + res[q]);
             }
         }
         if constexpr (M == Mode::GateUp) {
