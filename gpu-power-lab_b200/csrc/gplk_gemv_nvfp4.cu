@@ -7,6 +7,13 @@
 namespace gplk {
 namespace fewtok {
 
+// Whether a block takes two tiles, which then share the activations' slots.
+static bool use_pairs(int T, int tiles, int stages) {
+    (void)tiles;
+    (void)stages;
+    return false && T;
+}
+
 // ---------------------------------------------------------------- conversion ahead of the products
 // Writes the B rows and scales of every stage as the ring holds them, a block
 // per token, so that the blocks of an Image kernel fetch them with one bulk
@@ -73,12 +80,32 @@ __global__ void __launch_bounds__(kImageThreads)
     }
 }
 
-// Whether the activations are converted once, by a kernel of their own, or by
-// every block for itself.
-static bool use_image(int T, int K) { return (long long)T * K > 32768; }
+constexpr int kSms = 148;
 
-// Whether a block takes two tiles, which then share the activations' slots.
-static bool use_pairs(int T, int tiles) { return false; }
+// Shape of a product of T tokens on a B200. Up to 12 tokens' accumulators of two
+// tiles fit half of TMEM: a block then takes two tiles where that leaves at
+// least a block for every SM.
+static Shape plan(Params& p, int T, int N, int K) {
+    p.T = T;
+    p.N = N;
+    p.K = K;
+    p.tiles = (N + kTileRows - 1) / kTileRows;
+    p.k_stages = (K + kStageK - 1) / kStageK;
+    p.kblocks = K / 64;
+    p.halves = use_pairs(T, p.tiles, p.k_stages) ? 2 : 1;
+    const int groups = (p.tiles + p.halves - 1) / p.halves;
+    const int per_sm = p.halves * ((kPlanes * T + 15) & ~15) > 128 ? 1 : 2;
+    p.split_log2 = choose_split_log2(groups, p.k_stages * p.halves, 8, per_sm * kSms);
+    return set_shape(p, T, false, ((p.k_stages - 1) >> p.split_log2) + 1);
+}
+
+// Whether the activations are converted once, by a kernel of their own, or by
+// every block for itself: that keeps up with the weights up to about four tokens
+// a stage, and a launch costs as much as some 20 units (a token's stage) of it.
+// Measured, fused / image, us: 4x16384x8192 19.1 / 18.8 (64 units in a block),
+// 8x16384x4096 17.1 / 12.2 (64), 8x16384x2048 10.7 / 9.8 (32), 8x8192x2048
+// 7.2 / 7.5 (16), 6x4096x4096 7.4 / 8.0 (12), 2x16384x8192 16.3 / 18.8 (32).
+static bool use_image(const Params& p) { return p.T >= 4 && p.T * (((p.k_stages - 1) >> p.split_log2) + 1) >= 24; }
 
 // Workspace of the converted activations: the stages' images, then the
 // tokens' largest magnitudes.
@@ -104,7 +131,13 @@ static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* w
 
 extern "C" size_t gplk_gemv_nvfp4_workspace_bytes(int T, int N, int K) {
     using namespace gplk::fewtok;
-    if (T <= 0 || T > kMaxTokens || N <= 0 || K <= 0 || K % 64 != 0 || !use_image(T, K)) return 0;
+    if (T <= 0 || T > kMaxTokens || N <= 0 || K <= 0 || K % 64 != 0 || N > INT_MAX / 8 ||
+        K > INT_MAX / 8)
+        return 0;
+    Params p;
+    memset(&p, 0, sizeof(p));
+    plan(p, T, N, K);
+    if (!use_image(p)) return 0;
     return image_bytes(T, (K + kStageK - 1) / kStageK) + sizeof(uint32_t) * kMaxTokens;
 }
 
@@ -117,7 +150,7 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     if (dtype != GPLK_DTYPE_BF16 && dtype != GPLK_DTYPE_F16) return GPLK_STATUS_BAD_ARG;
     if (T == 0 || N == 0) return GPLK_STATUS_OK;
     if (K == 0 || K % 64 != 0 || ldx < K || ldy < N || (R && ldr < N)) return GPLK_STATUS_BAD_ARG;
-    if (N > INT_MAX / 8) return GPLK_STATUS_BAD_ARG;  // N / 128 tiles of 8 slices fit a grid
+    if (N > INT_MAX / 8 || K > INT_MAX / 8) return GPLK_STATUS_BAD_ARG;  // grids, sums of stages
     if (!X || !W || !SF || !Y || !alpha) return GPLK_STATUS_BAD_ARG;
     if (!aligned16(W) || !aligned16(SF) || !aligned(X, 2) || !aligned(Y, 2) || !aligned(R, 2) || !aligned(alpha, 4) ||
         !aligned16(workspace))
@@ -132,22 +165,14 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     p.alpha0 = alpha;
     p.Y = Y;
     p.R = R;
-    p.T = T;
-    p.N = N;
-    p.K = K;
     p.ldx = ldx;
     p.ldy = ldy;
     p.ldr = ldr;
     p.x_vec = aligned16(X) && (T == 1 || ldx % 8 == 0);
-    p.tiles = (N + kTileRows - 1) / kTileRows;
-    p.k_stages = (K + kStageK - 1) / kStageK;
-    p.kblocks = K / 64;
-    const size_t need = gplk_gemv_nvfp4_workspace_bytes(T, N, K);
-    void* ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;
-    p.halves = use_pairs(T, p.tiles) ? 2 : 1;
-    const Shape s = set_shape(p, T, false);
+    const Shape s = plan(p, T, N, K);
     if (s.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
-    p.split_log2 = choose_split_log2((p.tiles + p.halves - 1) / p.halves, p.k_stages * p.halves, 8, s.per_sm * d.sm_count);
+    const size_t need = use_image(p) ? image_bytes(T, p.k_stages) + sizeof(uint32_t) * kMaxTokens : 0;
+    void* ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;
     CUtensorMap tm;
     st = encode_weights(&tm, W, (uint64_t)N, K);
     if (st != GPLK_STATUS_OK) return st;

@@ -56,51 +56,47 @@ struct RouteParams {
     int vec;  // rows of x and of the router are 16-byte aligned
 };
 
-// Router product: a block per expert and up to 8 tokens, whose four warps
-// share out K. One more block per 8 tokens finds the tokens' largest
-// magnitudes, which anchor the conversion of x, and clears those of h.
-constexpr int kRouterThreads = 128;
-
-template <typename XT, int NX>
-__global__ void __launch_bounds__(kRouterThreads) router_kernel(const RouteParams p) {
-    const int e = blockIdx.x, t0 = blockIdx.y * NX;
-    const int nx = min(NX, p.T - t0);
-    const int warp = (int)warp_id_uniform();
+// Largest magnitude of token t, by one warp: it anchors the conversion of x. The
+// magnitude of the token's h starts at zero.
+template <typename XT>
+__device__ __forceinline__ void token_amax(const RouteParams& p, int t) {
     const int lane = (int)lane_id();
-    pdl_wait();
-    pdl_launch_dependents();
-    const XT* x = static_cast<const XT*>(p.x) + (size_t)t0 * p.ldx;
-    const bool vec = p.vec != 0;
-    if (e == p.E) {
-        for (int t = warp; t < nx; t += kRouterThreads / 32) {
-            uint32_t m = 0;
-            for (int k0 = lane * 8; k0 < p.D; k0 += 4 * 256) {
-                uint4 r[4][2];
+    const XT* x = static_cast<const XT*>(p.x) + (size_t)t * p.ldx;
+    uint32_t m = 0;
+    for (int k0 = lane * 8; k0 < p.D; k0 += 4 * 256) {
+        uint4 r[4][2];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    r[c][0] = make_uint4(0, 0, 0, 0);
-                    if (k0 + 256 * c < p.D) load_raw(x + (size_t)t * p.ldx + k0 + 256 * c, vec, r[c]);
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float v[8];
-                    widen<XT>(r[c], v);
-                    m = max(m, max_bits(v));
-                }
-            }
-            m = __reduce_max_sync(0xffffffffu, m);
-            if (lane == 0) p.amax[t0 + t] = m;
-            if (lane == 1) p.amax[kMaxTokens + t0 + t] = 0;
+        for (int c = 0; c < 4; ++c) {
+            r[c][0] = make_uint4(0, 0, 0, 0);
+            if (k0 + 256 * c < p.D) load_raw(x + k0 + 256 * c, p.vec != 0, r[c]);
         }
-        return;
-    }
-    const XT* r = static_cast<const XT*>(p.router) + (size_t)e * p.D;
-    float acc[NX] = {};
-    for (int k = (int)threadIdx.x * 8; k < p.D; k += kRouterThreads * 8) {
-        uint4 wr[2], xr[NX][2];
-        load_raw(r + k, vec, wr);
 #pragma unroll
-        for (int i = 0; i < NX; ++i) load_raw(x + (size_t)min(i, nx - 1) * p.ldx + k, vec, xr[i]);
+        for (int c = 0; c < 4; ++c) {
+            float v[8];
+            widen<XT>(r[c], v);
+            m = max(m, max_bits(v));
+        }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) p.amax[t] = m;
+    if (lane == 1) p.amax[kMaxTokens + t] = 0;
+}
+
+// Sums over this thread's share of K (from k0 in steps of `step`) of the products
+// of a router row with the rows of tokens t0 .. t0 + nx - 1.
+template <typename XT, int NX>
+__device__ __forceinline__ void router_dots(const RouteParams& p, int e, int t0, int nx, int k0, int step,
+                                            float (&acc)[NX]) {
+    const XT* r = static_cast<const XT*>(p.router) + (size_t)e * p.D;
+    const XT* x = static_cast<const XT*>(p.x) + (size_t)t0 * p.ldx;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) acc[i] = 0.0f;
+#pragma unroll(NX == 1 ? 4 : NX <= 4 ? 2 : 1)
+    for (int k = k0; k < p.D; k += step) {
+        uint4 wr[2], xr[NX][2];
+        load_raw(r + k, p.vec != 0, wr);
+#pragma unroll
+        for (int i = 0; i < NX; ++i) load_raw(x + (size_t)min(i, nx - 1) * p.ldx + k, p.vec != 0, xr[i]);
         float w[8];
         widen<XT>(wr, w);
 #pragma unroll
@@ -111,12 +107,33 @@ __global__ void __launch_bounds__(kRouterThreads) router_kernel(const RouteParam
             for (int j = 0; j < 8; ++j) acc[i] = fmaf(w[j], v[j], acc[i]);
         }
     }
-    __shared__ float part[4][NX];
 #pragma unroll
-    for (int i = 0; i < NX; ++i) {
+    for (int i = 0; i < NX; ++i)
 #pragma unroll
         for (int o = 16; o; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-        if (lane == 0) part[warp][i] = acc[i];
+}
+
+// Router product of many experts: a block per expert and up to NX tokens, whose
+// four warps share out K; one more block per NX tokens for their magnitudes.
+constexpr int kRouterThreads = 128;
+
+template <typename XT, int NX>
+__global__ void __launch_bounds__(kRouterThreads) router_kernel(const RouteParams p) {
+    const int e = blockIdx.x, t0 = blockIdx.y * NX;
+    const int nx = min(NX, p.T - t0);
+    const int warp = (int)warp_id_uniform();
+    pdl_wait();
+    pdl_launch_dependents();
+    if (e == p.E) {
+        for (int t = warp; t < nx; t += kRouterThreads / 32) token_amax<XT>(p, t0 + t);
+        return;
+    }
+    float acc[NX];
+    router_dots<XT, NX>(p, e, t0, nx, (int)threadIdx.x * 8, kRouterThreads * 8, acc);
+    __shared__ float part[4][NX];
+    if (lane_id() == 0) {
+#pragma unroll
+        for (int i = 0; i < NX; ++i) part[warp][i] = acc[i];
     }
     __syncthreads();
     if (threadIdx.x < (unsigned)nx)
@@ -133,28 +150,35 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return k == 0 ? __uint_as_float(0x7FC00000u) : __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// Softmax and top-k of one token per warp, then the routing tables. A lane
-// holds the logits of experts lane, lane + 32, ... (PER of them); each rank
-// takes the largest left, the lowest index among equals. A NaN counts below
-// every number.
-template <int PER>
-__global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParams p) {
+// Softmax and top-k of one token per warp, then the routing tables, by one block
+// of WARPS warps (at least T of them, and a thread for every expert). A lane holds
+// the logits of experts lane, lane + 32, ... (PER of them); each rank takes the
+// largest left, the lowest index among equals. A NaN counts below every number.
+constexpr int kPer = kMaxExperts / 32;
+
+struct RouteShared {
+    int ids[kMaxTokens * kMaxTop];
+    uint32_t chosen_mask[kPer];
+    int active[kMaxExperts];
+    int chunks[kMaxExperts];
+};
+
+template <int PER, int WARPS>
+__device__ __forceinline__ void route_body(const RouteParams& p, RouteShared& sh) {
+    static_assert(32 * WARPS >= kMaxExperts, "a thread per expert");
     const int warp = (int)warp_id_uniform();
     const int lane = (int)lane_id();
-    constexpr int kPer = kMaxExperts / 32;
-    __shared__ int ids[kMaxTokens * kMaxTop];
-    __shared__ uint32_t chosen_mask[kPer];
-    __shared__ int active[kMaxExperts];
-    __shared__ int chunks[kMaxExperts];
+    int* const ids = sh.ids;
+    int* const active = sh.active;
+    int* const chunks = sh.chunks;
+    uint32_t* const chosen_mask = sh.chosen_mask;
     if (threadIdx.x < kPer) chosen_mask[threadIdx.x] = 0;
     __syncthreads();
-    pdl_wait();
-    pdl_launch_dependents();
     if (warp < p.T) {
         const float* l = p.logits + (size_t)warp * p.E;
         float v[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < p.E ? l[lane + 32 * i] : -INFINITY;
+        for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < p.E ? __ldcg(l + lane + 32 * i) : -INFINITY;
         uint32_t key[PER];
         uint32_t most = 0;
 #pragma unroll
@@ -220,12 +244,12 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
                 if (ids[lane * p.top + j] == e) slot = lane * p.top + j;
         return slot;
     };
-    for (int a = warp; a < n_active; a += kMaxTokens) {
+    for (int a = warp; a < n_active; a += WARPS) {
         const uint32_t m = __ballot_sync(0xffffffffu, slot_of(active[a]) >= 0);
         if (lane == 0) chunks[a] = (__popc(m) + kMaxEntryTokens - 1) / kMaxEntryTokens;
     }
     __syncthreads();
-    for (int a = warp; a < n_active; a += kMaxTokens) {
+    for (int a = warp; a < n_active; a += WARPS) {
         // Entries of the experts before this one.
         int base = 0;
         for (int b = lane; b < a; b += 32) base += chunks[b];
@@ -250,6 +274,60 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
     }
 }
 
+template <int PER>
+__global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParams p) {
+    __shared__ RouteShared sh;
+    pdl_wait();
+    pdl_launch_dependents();
+    route_body<PER, kMaxTokens>(p, sh);
+}
+
+// Router product and routing of few experts and tokens in one launch: a cluster of
+// eight blocks shares out the experts and the first block routes. On the device
+// it takes as long as two launches do (layer of 8 experts, 1024 x 512: 16.2 us
+// with it, 16.1 with two; of 32, 2048 x 704: 24.1 and 24.4; but of 64, 2048 x
+// 1024: 22.1 and 20.8, so it stops at 65536 weights); the host saves one.
+constexpr int kFewBlocks = 8;
+constexpr int kFewWarps = 16;
+constexpr int kFewPer = 4;  // at most 128 experts
+
+template <typename XT, int NX>
+__global__ void __cluster_dims__(kFewBlocks, 1, 1) __launch_bounds__(32 * (kFewWarps + 1))
+    few_route_kernel(const RouteParams p, int sub_log2) {
+    __shared__ RouteShared sh;
+    __shared__ float part[kFewWarps][NX];
+    const int rank = (int)cluster_ctarank(), warp = (int)warp_id_uniform(), lane = (int)lane_id();
+    pdl_wait();
+    pdl_launch_dependents();
+    // 2^sub_log2 warps share out an expert's K, so that a block's experts take
+    // all of its warps.
+    // The last warp finds the tokens' magnitudes meanwhile.
+    const bool dots = warp < kFewWarps;
+    if (!dots)
+        for (int t = rank; t < p.T; t += kFewBlocks) token_amax<XT>(p, t);
+    const int subs = 1 << sub_log2, mine = warp >> sub_log2, sub = warp & (subs - 1);
+    for (int e0 = rank; e0 < p.E; e0 += kFewBlocks * (kFewWarps >> sub_log2)) {
+        const int e = e0 + kFewBlocks * mine;
+        float acc[NX] = {};
+        if (dots && e < p.E) router_dots<XT, NX>(p, e, 0, p.T, (sub * 32 + lane) * 8, subs * 256, acc);
+#pragma unroll
+        for (int i = 0; i < NX; ++i)
+            if (dots && lane == i) part[warp][i] = acc[i];
+        __syncthreads();
+        if (dots && sub == 0 && e < p.E && lane < p.T) {
+            float v = 0.0f;
+            for (int q = 0; q < subs; ++q) v += part[warp + q][lane];
+            p.logits[(size_t)lane * p.E + e] = v;
+        }
+        __syncthreads();
+    }
+    __syncwarp();
+    cluster_sync();
+    if (rank == 0) route_body<kFewPer, kFewWarps + 1>(p, sh);
+}
+
+static bool few_experts(int T, int E, int D) { return T <= 4 && E <= 32 * kFewPer && (long long)E * D <= 1 << 16; }
+
 // ---------------------------------------------------------------- resident experts' products
 // With enough work for every SM, one block per SM walks over the items (an
 // entry's two tiles: gate and up of 128 features, or 256 rows of down), and its
@@ -258,13 +336,11 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
 // (two sets) drain. stream_kernel starts a block per item instead, which costs
 // about 4 us of an SM's stream each; there K is split over a cluster, which is
 // what few items need.
-//   warp 0 copies, warp 1 MMAs, warps 2..9 convert, warps 10..13 epilogue,
-//   warps 14..17 scales to TMEM
-constexpr int kItemThreads = 32 * 18;
+//   warp 0 copies, warp 1 MMAs, warps 2..9 convert, warps 10..13 epilogue
+constexpr int kItemThreads = 32 * 14;
 
 struct ItemControl {
     uint64_t full[kMaxSlots];
-    uint64_t scaled[kMaxSlots];
     uint64_t empty[kMaxSlots];
     uint64_t acc_full[2];
     uint64_t acc_empty[2];
@@ -287,7 +363,6 @@ __global__ void __launch_bounds__(kItemThreads, 1)
 
     if (threadIdx.x < kMaxSlots) {
         mbar_init(&sm.full[threadIdx.x], 1 + kConvWarps);
-        mbar_init(&sm.scaled[threadIdx.x], 4);
         mbar_init(&sm.empty[threadIdx.x], 1);
         if (threadIdx.x < 2) {
             mbar_init(&sm.acc_full[threadIdx.x], 1);
@@ -363,7 +438,8 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        const uint64_t op_desc = desc_kmajor_sw128(0);
+        const uint64_t op_desc = desc_kmajor_sw128(0), sf_desc = smem_desc(0, 0, 128, 0);
+        const uint32_t sfb_step = g.sfb_step >> 4;
         Cursor w, b, acc;
         bool ok = true;
         for (int it = (int)blockIdx.x; it < items && ok; it += (int)gridDim.x) {
@@ -378,9 +454,10 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                 const int nblk = min(4, p.kblocks - 4 * kb);
                 const uint32_t b_addr = smem_u32(b_ring) + (uint32_t)b.slot * g.b_slot;
                 const uint64_t b_desc = op_desc + (b_addr >> 4);
+                const uint64_t sfb_desc = sf_desc + ((b_addr + (uint32_t)g.nb * 128) >> 4);
                 const uint32_t sfb_col = sfb_col0 + (uint32_t)b.slot * g.sfb_cols;
                 for (int h = 0; h < 2; ++h) {
-                    ok = mbar_wait(&sm.scaled[w.slot], w.phase, &sm.abort, 0x0712);
+                    ok = mbar_wait(&sm.full[w.slot], w.phase, &sm.abort, 0x0712);
                     if (!ok) break;
                     __syncwarp();
                     tc_fence_after();
@@ -388,6 +465,11 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                     const uint64_t a_desc = op_desc + (a_addr >> 4);
                     const uint32_t sfa_col = sfa_col0 + (uint32_t)w.slot * 16;
                     const uint32_t d = tmem + (uint32_t)(2 * acc.slot + h) * g.acc_cols;
+                    const uint64_t sfa_desc = sf_desc + ((a_addr + kWBytes) >> 4);
+                    auto scales = [&](int j) {
+                        if (h == 0) tmem_cp_32x128b_warpx4(sfb_col + 4 * j, sfb_desc + sfb_step * j);
+                        tmem_cp_32x128b_warpx4(sfa_col + 4 * j, sfa_desc + 32 * j);
+                    };
                     auto product = [&](int j) {
                         mma_nvf4(d, a_desc + 2 * j, b_desc + 2 * j, idesc, sfa_col + 4 * j, sfb_col + 4 * j,
                                  (kb | j) != 0);
@@ -396,8 +478,11 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                         if (h < nw) {
                             if (nblk == 4) {
 #pragma unroll
+                                for (int j = 0; j < 4; ++j) scales(j);
+#pragma unroll
                                 for (int j = 0; j < 4; ++j) product(j);
                             } else {
+                                for (int j = 0; j < nblk; ++j) scales(j);
                                 for (int j = 0; j < nblk; ++j) product(j);
                             }
                         }
@@ -504,28 +589,6 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                 if (lane == 0) {
                     mbar_arrive(&sm.full[slot0]);
                     mbar_arrive(&sm.full[slot1]);
-                }
-                b.advance(g.b_slots);
-            }
-        }
-        __syncwarp();
-    } else if (warp >= 6 + kConvWarps) {
-        // ------------------------------------------------------------ scales
-        Cursor c, b;
-        bool ok = true;
-        const uint32_t quarter = (warp & 3u) << 21;
-        for (int it = (int)blockIdx.x; it < items && ok; it += (int)gridDim.x) {
-            for (int kb = 0; kb < p.k_stages && ok; ++kb) {
-                for (int h = 0; h < 2; ++h) {
-                    ok = mbar_wait(&sm.full[c.slot], c.phase, &sm.abort, 0x0741);
-                    if (!ok) break;
-                    __syncwarp();
-                    scales_to_tmem(ring + (size_t)c.slot * kWSlot + kWBytes, sfa_col0 + (uint32_t)c.slot * 16 + quarter,
-                                   b_ring + (size_t)b.slot * g.b_slot + (size_t)g.nb * 128,
-                                   sfb_col0 + (uint32_t)b.slot * g.sfb_cols + quarter, g.sfb_step,
-                                   h == 0 ? g.sfb_cols : 0u, lane);
-                    if (lane == 0) mbar_arrive(&sm.scaled[c.slot]);
-                    c.advance(g.w_slots);
                 }
                 b.advance(g.b_slots);
             }
@@ -725,7 +788,7 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
         g_smem = set_item_shape(g, entry_tokens);
     } else {
         g.halves = 2;
-        const Shape s = set_shape(g, entry_tokens, true);
+        const Shape s = set_shape(g, entry_tokens, true, g.k_stages);
         g_smem = s.smem;
         g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, 8, s.per_sm * d.sm_count);
     }
@@ -733,7 +796,7 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
         o_smem = set_item_shape(o, entry_tokens);
     } else {
         o.halves = 1;
-        const Shape s = set_shape(o, c.T, false);
+        const Shape s = set_shape(o, c.T, false, o.k_stages * max_entries);
         o_smem = s.smem;
         o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, 8, s.per_sm * d.sm_count);
     }
@@ -748,10 +811,19 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     auto router = [&](auto kernel, int nx) {
         return launch_status(launch_pdl(kernel, dim3(c.E + 1, (c.T + nx - 1) / nx), dim3(kRouterThreads), 0, stream, r));
     };
-    st = c.T == 1 ? router(router_kernel<XT, 1>, 1) : c.T <= 4 ? router(router_kernel<XT, 4>, 4) : router(router_kernel<XT, 8>, 8);
-    if (st == GPLK_STATUS_OK)
-        st = launch_status(launch_pdl(c.E <= 128 ? route_kernel<4> : route_kernel<kMaxExperts / 32>, dim3(1),
-                                      dim3(32 * kMaxTokens), 0, stream, r));
+    if (few_experts(c.T, c.E, c.D)) {
+        int sub_log2 = 4;
+        while (sub_log2 > 0 && (c.E + kFewBlocks - 1) / kFewBlocks > kFewWarps >> sub_log2) --sub_log2;
+        st = launch_status(launch_pdl(c.T == 1 ? few_route_kernel<XT, 1> : few_route_kernel<XT, 4>, dim3(kFewBlocks),
+                                      dim3(32 * (kFewWarps + 1)), 0, stream, r, sub_log2));
+    } else {
+        st = c.T == 1   ? router(router_kernel<XT, 1>, 1)
+             : c.T <= 4 ? router(router_kernel<XT, 4>, 4)
+                        : router(router_kernel<XT, 8>, 8);
+        if (st == GPLK_STATUS_OK)
+            st = launch_status(launch_pdl(c.E <= 128 ? route_kernel<4> : route_kernel<kPer>, dim3(1),
+                                          dim3(32 * kMaxTokens), 0, stream, r));
+    }
     if (st == GPLK_STATUS_OK)
         st = g_items ? launch_items<true, XT>(tg, tu, g, g_smem, d.sm_count, stream)
                      : launch_stream<Mode::GateUp, XT, float>(tg, tu, g, g_smem, max_entries * g.tiles, stream);

@@ -40,8 +40,8 @@
 //   warps 2..9  convert the same 256 elements of every token into a slot of
 //               the activations' ring (a warp per token and slot); warps 2..5
 //               then read the accumulators, and all warps add the slices.
-//               An Image kernel copies what another kernel converted; it has
-//               warps 2..5 only, and they bring the scales to TMEM.
+//               An Image kernel copies what another kernel converted, and has
+//               warps 2..5 only.
 // The MMA warp runs its loop converged and elects the issuing lane: with
 // addresses and descriptors in uniform registers, 65536 x 8192 at one token
 // takes 51 us; issued from a lane of a diverged warp 76 us.
@@ -112,7 +112,15 @@ struct Geometry {
 // slot free knows that tiles up to j - w are done; with b slots such that stage
 // i - b is among those, the activations' slot is free too: b = w for single
 // tiles, b = w / 2 + 1 for pairs.
-static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tmem_cols, int accs = 1) {
+static uint32_t ring_of(const Geometry& g) {
+    return (uint32_t)g.w_slots * kWSlot + (uint32_t)g.b_slots * g.b_slot;
+}
+static uint32_t columns_of(const Geometry& g, int accs) {
+    return (uint32_t)accs * g.acc_cols + (uint32_t)g.w_slots * 16 + (uint32_t)g.b_slots * g.sfb_cols;
+}
+
+static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tmem_cols, int accs = 1,
+                         int most_slots = kMaxSlots) {
     Geometry g;
     g.nb = (kPlanes * ntok + 7) & ~7;
     const bool wide = g.nb > 128;  // a second 128 rows of B scales
@@ -125,12 +133,11 @@ static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tme
     g.b_slot = (g.image + 1023) & ~1023u;
     g.acc_cols = ((uint32_t)g.nb + 15) & ~15u;
     g.sfb_cols = wide ? 32 : 16;
-    for (g.w_slots = kMaxSlots; g.w_slots > 1; --g.w_slots) {
+    for (g.w_slots = most_slots; g.w_slots > 1; --g.w_slots) {
         g.b_slots = halves == 1 ? g.w_slots : g.w_slots / 2 + 1;
-        if ((uint32_t)g.w_slots * kWSlot + (uint32_t)g.b_slots * g.b_slot <= ring_bytes &&
-            (uint32_t)(accs * halves) * g.acc_cols + (uint32_t)g.w_slots * 16 + (uint32_t)g.b_slots * g.sfb_cols <= tmem_cols)
-            break;
+        if (ring_of(g) <= ring_bytes && columns_of(g, accs * halves) <= tmem_cols) return g;
     }
+    g.b_slots = 1;
     return g;
 }
 
@@ -164,7 +171,6 @@ struct Params {
 
 struct Control {
     uint64_t full[kMaxSlots];   // by weights' slot
-    uint64_t scaled[kMaxSlots]; // Image kernels: full, and its scales are in TMEM
     uint64_t empty[kMaxSlots];
     uint64_t acc_full;
     uint64_t drain;
@@ -360,36 +366,6 @@ __device__ __forceinline__ void convert_zero(int t, uint8_t* b_rows, uint8_t* sf
     }
 }
 
-// A stage's scales from shared memory to one warp's 32 TMEM lanes, which the four
-// warps of a group do with the same data, as the MMA wants it. (tcgen05.cp does
-// all four at once, but in the MMAs' own queue, where each copy takes about as
-// long as an MMA of 8 columns: at 25 tokens, 16384 x 8192 out of L2, XXX.)
-__device__ __forceinline__ void scales_to_tmem(const uint8_t* sfa, uint32_t sfa_col, const uint8_t* sfb,
-                                               uint32_t sfb_col, uint32_t sfb_step, uint32_t sfb_cols,
-                                               uint32_t lane) {
-    auto put = [&](uint32_t col, const uint8_t* block) {
-        const uint4 v = *reinterpret_cast<const uint4*>(block + lane * 16);
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(col), "r"(v.x), "r"(v.y),
-                     "r"(v.z), "r"(v.w)
-                     : "memory");
-    };
-#pragma unroll
-    for (int j = 0; j < 4; ++j) put(sfa_col + 4 * j, sfa + 512 * j);
-    if (sfb_cols == 16) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) put(sfb_col + 4 * j, sfb + sfb_step * j);
-    } else if (sfb_cols == 32) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            put(sfb_col + 8 * j, sfb + 512 * j);
-            put(sfb_col + 8 * j + 4, sfb + 2048 + 512 * j);
-        }
-    }
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-    tc_fence_before();
-    __syncwarp();
-}
-
 template <bool IMAGE>
 constexpr int kThreads = IMAGE ? 64 + 128 : 64 + 32 * kConvWarps;
 
@@ -406,13 +382,13 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     const int cid = (int)(blockIdx.x >> p.split_log2);
     constexpr bool kPerExpert = M == Mode::GateUp;
 
-    // Barriers and TMEM. A slot is full when the copies have landed and the
-    // warps with tokens in the stage have converted them.
+    // Barriers and TMEM. A slot is full when the copies have landed and the warps
+    // with tokens in the stage have converted them (where the tokens are not
+    // known yet: when every warp has been there).
     auto set_up = [&](int ntok) {
         if (threadIdx.x < kMaxSlots) {
             const int i = (int)threadIdx.x;
-            mbar_init(&sm.full[i], IMAGE ? 1u : 1u + (uint32_t)min(ntok, kConvWarps));
-            mbar_init(&sm.scaled[i], 4);
+            mbar_init(&sm.full[i], IMAGE ? 1u : 1u + (uint32_t)(kPerExpert ? kConvWarps : min(ntok, kConvWarps)));
             mbar_init(&sm.empty[i], 1);
             if (i == 0) {
                 mbar_init(&sm.acc_full, 1);
@@ -431,7 +407,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         tma_prefetch_desc(&tm0);
         if (M == Mode::GateUp) tma_prefetch_desc(&tm1);
     }
-    if constexpr (!kPerExpert) set_up(p.T);
+    set_up(p.T);
     // What is above may overlap the previous kernel's tail. The conversion
     // kernel that an Image kernel follows let it start only once every kernel
     // before the two had completed, so weights may be read at once, and what that
@@ -452,8 +428,11 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         if (threadIdx.x < kMaxEntryTokens) sm.slot[threadIdx.x] = p.route->list[a][threadIdx.x];
         expert = head & 0xFFFF;
         ntok = head >> 16;
-        if (ntok == 0) return;  // behind the last entry; the whole cluster leaves
-        set_up(ntok);
+        if (ntok == 0) {  // behind the last entry: the whole cluster leaves
+            __syncthreads();
+            if (warp == 1) tmem_dealloc(sm.tmem_base, p.tmem_cols);
+            return;
+        }
     } else if constexpr (M == Mode::Down) {
         total = p.route->n_entries * p.k_stages;
     }
@@ -565,7 +544,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 const uint64_t sfb_desc = sf_desc + ((b_addr + (uint32_t)g.nb * 128) >> 4);
                 const uint32_t sfb_col = sfb_col0 + (uint32_t)b.slot * g.sfb_cols;
                 for (int h = 0; h < nw; ++h) {
-                    ok = mbar_wait(IMAGE ? &sm.scaled[w.slot] : &sm.full[w.slot], w.phase, &sm.abort, 0x0611);
+                    ok = mbar_wait(&sm.full[w.slot], w.phase, &sm.abort, 0x0611);
                     if (!ok) break;
                     __syncwarp();
                     tc_fence_after();
@@ -580,25 +559,20 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                                  (i | j) != 0);
                     };
                     if (elect_one()) {
-                        if constexpr (!IMAGE) {
-                            if (h == 0) {
+                        if (h == 0) {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    tmem_cp_32x128b_warpx4(sfb_col + sfb_next * j, sfb_desc + sfb_step * j);
-                                    if (sfb_next == 8u) tmem_cp_32x128b_warpx4(sfb_col + 4 + 8 * j, sfb_desc + 128 + 32 * j);
-                                }
+                            for (int j = 0; j < 4; ++j) {
+                                tmem_cp_32x128b_warpx4(sfb_col + sfb_next * j, sfb_desc + sfb_step * j);
+                                if (sfb_next == 8u) tmem_cp_32x128b_warpx4(sfb_col + 4 + 8 * j, sfb_desc + 128 + 32 * j);
                             }
                         }
                         if (nblk == 4) {
-                            if constexpr (!IMAGE) {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) scales(j);
-                            }
+                            for (int j = 0; j < 4; ++j) scales(j);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) product(j);
                         } else {
-                            if constexpr (!IMAGE)
-                                for (int j = 0; j < nblk; ++j) scales(j);
+                            for (int j = 0; j < nblk; ++j) scales(j);
                             for (int j = 0; j < nblk; ++j) product(j);
                         }
                         tc_commit(&sm.empty[w.slot]);
@@ -625,48 +599,28 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             pdl_wait();
             if (w == 0) sm.amax[lane] = (int)lane < p.T ? p.amax[lane] : 0u;
             named_sync(1, 128);
-            Cursor c, b;
-            bool ok = true;
-            for (int i = 0; i < nst && ok; ++i) {
-                for (int h = 0; h < nw; ++h) {
-                    ok = mbar_wait(&sm.full[c.slot], c.phase, &sm.abort, 0x0624);
-                    if (!ok) break;
-                    __syncwarp();
-                    const uint8_t* sfb = b_ring + (size_t)b.slot * g.b_slot + (size_t)g.nb * 128;
-                    scales_to_tmem(ring + (size_t)c.slot * kWSlot + kWBytes,
-                                   sfa_col0 + (uint32_t)c.slot * 16 + ((warp & 3u) << 21), sfb,
-                                   sfb_col0 + (uint32_t)b.slot * g.sfb_cols + ((warp & 3u) << 21),
-                                   g.sfb_step,
-                                   h == 0 ? g.sfb_cols : 0u, lane);
-                    if (lane == 0) mbar_arrive(&sm.scaled[c.slot]);
-                    c.advance(g.w_slots);
-                }
-                b.advance(g.b_slots);
-            }
-            __syncwarp();
         } else {
         // ------------------------------------------------------------ activations
-        if constexpr (kEarly) pdl_wait();
         // Unit u = i * tokens + t, token t in stage i, is warp u % 8's. A lane
         // holds eight elements of it; false: the token has none in the stage.
         struct Unit {
             int i, t;
             int entry, kb;  // of the stage; Down only
         };
-        auto load = [&](const Unit& n, uint4 (&r)[2]) -> bool {
-            const int kb = M == Mode::Down ? n.kb : first + n.i, t = n.t;
-            int row = t;
-            if constexpr (M == Mode::Down) {
-                row = p.route->slot[n.entry][t];
-            } else if constexpr (M == Mode::GateUp) {
-                row = sm.slot[t] / p.top;
-            }
+        auto row_of = [&](const Unit& n) -> int {
+            if constexpr (M == Mode::Down) return p.route->slot[n.entry][n.t];
+            if constexpr (M == Mode::GateUp) return sm.slot[n.t] / p.top;
+            return n.t;
+        };
+        auto load_row = [&](const Unit& n, int row, uint4 (&r)[2]) -> bool {
+            const int kb = M == Mode::Down ? n.kb : first + n.i;
             const int k = kb * kStageK + (int)lane * 8;
             r[0] = r[1] = make_uint4(0, 0, 0, 0);
             if (row < 0) return false;
             if (k < p.K) load_raw(static_cast<const XT*>(p.X) + (size_t)row * p.ldx + k, p.x_vec != 0, r);
             return true;
         };
+        auto load = [&](const Unit& n, uint4 (&r)[2]) { return load_row(n, row_of(n), r); };
         // x / ntok for x <= 8, exactly.
         const uint32_t inverse = p.inverse[ntok];
         const int step_i = (int)(kConvWarps * inverse >> 16), step_t = kConvWarps - step_i * ntok;
@@ -739,6 +693,17 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             }
         }
         if (!done) {
+            // Two units' elements are on their way while one is converted. A Down
+            // block looks its first rows up before it waits for h.
+            Unit cur = first_unit, ahead = first_unit;
+            uint4 r0[2], r1[2];
+            bool on0 = false, on1 = false;
+            const int row0 = ahead.i < nst ? row_of(ahead) : 0;
+            next_unit(ahead);
+            const int row1 = ahead.i < nst ? row_of(ahead) : 0;
+            if constexpr (kEarly) pdl_wait();
+            if (cur.i < nst) on0 = load_row(cur, row0, r0);
+            if (ahead.i < nst) on1 = load_row(ahead, row1, r1);
             if (p.amax) {
                 if (w == 0 && (int)lane < ntok)
                     sm.amax[lane] = p.amax[kPerExpert ? sm.slot[lane] / p.top : (int)lane];
@@ -762,13 +727,6 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     (&sm.dirty[0][0])[i] = 1;
             }
             named_sync(1, 32 * kConvWarps);
-            // Two units' elements are on their way while one is converted.
-            Unit cur = first_unit, ahead = first_unit;
-            uint4 r0[2], r1[2];
-            bool on0 = false, on1 = false;
-            if (ahead.i < nst) on0 = load(ahead, r0);
-            next_unit(ahead);
-            if (ahead.i < nst) on1 = load(ahead, r1);
             Cursor c, b;
             for (int i = 0; i < nst; ++i) {
                 // Every warp waits for every slot, whether or not it has a token
@@ -809,10 +767,14 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     } while (cur.i == i);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) {
+                    if (!kPerExpert && lane == 0) {
                         mbar_arrive(&sm.full[slot0]);
                         if (nw == 2) mbar_arrive(&sm.full[slot1]);
                     }
+                }
+                if (kPerExpert && lane == 0) {
+                    mbar_arrive(&sm.full[slot0]);
+                    mbar_arrive(&sm.full[slot1]);
                 }
                 b.advance(g.b_slots);
             }
@@ -953,26 +915,48 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
 
 static inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
-// Shared memory and TMEM of a block: half an SM's, or all of it where the
-// accumulators of `tokens` tokens leave no room in half of TMEM.
+// Shared memory and TMEM of a block.
 struct Shape {
     int per_sm;
     size_t smem;
 };
 
-// For up to `tokens` tokens in a block: exactly that many, or 1 to `tokens` with
-// a geometry for each.
-static Shape set_shape(Params& p, int tokens, bool each) {
-    const bool all = p.halves * ((kPlanes * tokens + 15) & ~15) > 128;
+// Blocks of a cluster wait for one another, so none may wait for TMEM that a
+// block of another cluster holds while that cluster waits for this one. Every
+// launch of this family takes at least the share of an SM's shared memory that it
+// takes of its 512 TMEM columns: blocks that fit an SM's shared memory, of
+// whatever launches, then fit its TMEM too.
+static size_t share_of_smem(uint32_t tmem_cols) { return (size_t)228 * 1024 * tmem_cols / 512 - 1024; }
+
+// A block of `tokens` tokens, or of 1 to `tokens` with a geometry for each, and of
+// at most `stages` stages: no more than those want, up to half of an SM, or up to
+// all of it where half holds fewer than three tiles' slots.
+static Shape set_shape(Params& p, int tokens, bool each, int stages) {
     const size_t overhead = 1024 + ((sizeof(Control) + 127) & ~(size_t)127);
-    // 228 KiB per SM, 1 KiB of it reserved per block.
-    const size_t room = (all ? 227 * 1024 : (228 * 1024 - 2 * 1024) / 2) - overhead;
-    p.ring_bytes = (uint32_t)(room & ~(size_t)1023);
-    p.tmem_cols = all ? 512 : 256;
+    const int want = (long long)stages * p.halves < kMaxSlots ? stages * p.halves : kMaxSlots;
     for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
-    if (!each) p.geo[0] = geometry(tokens, p.halves, p.ring_bytes, p.tmem_cols);
-    for (int t = 1; each && t <= tokens; ++t) p.geo[t - 1] = geometry(t, p.halves, p.ring_bytes, p.tmem_cols);
-    return {all ? 1 : 2, p.ring_bytes + overhead};
+    Shape s;
+    uint32_t ring = 0, cols = 0;
+    for (uint32_t most = 256; most <= 512; most *= 2) {
+        ring = cols = 0;
+        bool enough = true;
+        for (int t = each ? 1 : tokens; t <= tokens; ++t) {
+            const Geometry g = geometry(t, p.halves, (uint32_t)(share_of_smem(most) - overhead), most, 1, want);
+            enough = enough && columns_of(g, p.halves) <= most && g.w_slots >= (want < 3 ? want : 3);
+            ring = ring_of(g) > ring ? ring_of(g) : ring;
+            cols = columns_of(g, p.halves) > cols ? columns_of(g, p.halves) : cols;
+            p.geo[each ? t - 1 : 0] = g;
+        }
+        if (enough) break;
+    }
+    for (p.tmem_cols = 32; p.tmem_cols < cols;) p.tmem_cols *= 2;
+    // The slices' sums lie over the rings.
+    const uint32_t sums = (uint32_t)(p.halves * tokens * kTileRows * 4);
+    p.ring_bytes = ((ring > sums ? ring : sums) + 1023) & ~1023u;
+    s.smem = p.ring_bytes + overhead;
+    if (s.smem < share_of_smem(p.tmem_cols)) s.smem = share_of_smem(p.tmem_cols);
+    s.per_sm = (int)(512 / p.tmem_cols < 2 ? 1 : 2);
+    return s;
 }
 
 // Slices of K: the split whose waves of blocks, each as long as its stages and

@@ -148,7 +148,7 @@ size_t gplk_nvfp4_sf_bytes(int rows, int k);
  * ldr >= N in elements. R may be NULL, and may be Y itself (Y is then
  * updated in place); X must not overlap Y. Sums are FP32; each output is
  * rounded once. alpha is a device pointer to the weights' per-tensor scale.
- * Requires K % 64 == 0, N < 2^28 and 16-byte aligned W and SF; X, Y and R may have any
+ * Requires K % 64 == 0, N and K below 2^28 and 16-byte aligned W and SF; X, Y and R may have any
  * alignment and leading dimension (rows of X on 16-byte boundaries load
  * fastest). The result does not depend on other calls or on timing: equal
  * inputs give equal bits. */
