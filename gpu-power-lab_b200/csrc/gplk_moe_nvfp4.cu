@@ -18,6 +18,8 @@
 //             (experts x F) against each token's h (zero where the expert is
 //             not the token's), so the weighted sum over experts happens in
 //             the accumulator and no atomics or second pass join it.
+#include <cmath>
+
 #include "gplk_ptx.cuh"
 
 namespace gplk {
@@ -114,8 +116,9 @@ __device__ __forceinline__ void router_dots(const RouteParams& p, int e, int t0,
 }
 
 // Router product of many experts: a block per expert and up to NX tokens, whose
-// four warps share out K; one more block per NX tokens for their magnitudes.
-constexpr int kRouterThreads = 128;
+// warps share out K (a thread's loads are then one round trip up to K = 4096);
+// one more block per NX tokens for their magnitudes.
+constexpr int kRouterThreads = 512;
 
 template <typename XT, int NX>
 __global__ void __launch_bounds__(kRouterThreads) router_kernel(const RouteParams p) {
@@ -130,15 +133,18 @@ __global__ void __launch_bounds__(kRouterThreads) router_kernel(const RouteParam
     }
     float acc[NX];
     router_dots<XT, NX>(p, e, t0, nx, (int)threadIdx.x * 8, kRouterThreads * 8, acc);
-    __shared__ float part[4][NX];
+    __shared__ float part[kRouterThreads / 32][NX];
     if (lane_id() == 0) {
 #pragma unroll
         for (int i = 0; i < NX; ++i) part[warp][i] = acc[i];
     }
     __syncthreads();
-    if (threadIdx.x < (unsigned)nx)
-        p.logits[(size_t)(t0 + threadIdx.x) * p.E + e] = (part[0][threadIdx.x] + part[1][threadIdx.x]) +
-                                                         (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    if (threadIdx.x < (unsigned)nx) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRouterThreads / 32; ++w) v += part[w][threadIdx.x];
+        p.logits[(size_t)(t0 + threadIdx.x) * p.E + e] = v;
+    }
 }
 
 // Order-preserving integer of a float, NaN below every number.
@@ -710,8 +716,26 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* part, XT* y, 
     row[3] = from_f32<XT>(s.w);
 }
 
-// Whether the experts' products run as resident blocks over `items`.
-static bool use_items(double items, int sm_count) { return items >= sm_count; }
+// Whether gate and up run as resident blocks over `items`: from two for every SM.
+// Measured, us of the layer, a block per item / resident: 310 items (8 tokens,
+// 128/8, 4096x768) 85 / 71, 976 (32, 64/6, 4096x2048) 183 / 174, but 256 (8, 8/2,
+// 4096x4096) 51.6 / 52.1 and (32, 8/2, 4096x4096) 75 / 88, 64 (16, 8/2, 2048x1024)
+// 23.3 / 26.9.
+static bool use_gate_items(double items, int sm_count) { return items >= 2.0 * sm_count; }
+
+// Whether down runs as resident blocks with a sum per slot, or accumulates over the
+// experts, which splits K further but converts and multiplies for every token in
+// every stage: by the tiles an SM streams, the second's weighed by its tokens.
+// Measured, us of the layer, accumulating / resident: 1 token 8/2 4096x14336
+// 47 / 68, 64/8 2048x1024 20.4 / 21.6; 2 tokens 16/4 4096x2048 32.5 / 33.2; 4 tokens
+// 32/4 2048x704 23.2 / 22.6; 8 tokens 8/2 4096x4096 59 / 52; 16 tokens 8/2
+// 2048x1024 27.2 / 23.3; 32 tokens 8/2 4096x4096 132 / 75.
+static bool use_down_items(int T, double active, int tiles, int k_stages, int split, int sm_count) {
+    const int pairs = (tiles + 1) / 2;
+    const double resident = 2.0 * k_stages * ceil(active * pairs / sm_count);
+    const double accumulated = ceil(active * k_stages / split) * ceil((double)tiles * split / sm_count);
+    return resident <= accumulated * (T < 4 ? 0.8 : 1.0 + T / 8.0);
+}
 
 template <typename XT>
 static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t stream) {
@@ -779,11 +803,8 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     o.tiles = (c.D + kTileRows - 1) / kTileRows;
     o.k_stages = (c.F + kStageK - 1) / kStageK;
     o.kblocks = c.F / 64;
-    const int pairs = (o.tiles + 1) / 2;
-    const bool g_items = use_items(active * g.tiles, d.sm_count), o_items = use_items(active * pairs, d.sm_count);
-    o.Y = o_items ? static_cast<void*>(ws + l.part) : c.y;
-    o.ldy = o_items ? c.D : c.ldy;
     size_t g_smem, o_smem;
+    const bool g_items = use_gate_items(active * g.tiles, d.sm_count);
     if (g_items) {
         g_smem = set_item_shape(g, entry_tokens);
     } else {
@@ -792,14 +813,13 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
         g_smem = s.smem;
         g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, 8, s.per_sm * d.sm_count);
     }
-    if (o_items) {
-        o_smem = set_item_shape(o, entry_tokens);
-    } else {
-        o.halves = 1;
-        const Shape s = set_shape(o, c.T, false, o.k_stages * max_entries);
-        o_smem = s.smem;
-        o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, 8, s.per_sm * d.sm_count);
-    }
+    o.halves = 1;
+    const Shape os = set_shape(o, c.T, false, o.k_stages * max_entries);
+    o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, 8, os.per_sm * d.sm_count);
+    const bool o_items = use_down_items(c.T, active, o.tiles, o.k_stages, 1 << o.split_log2, d.sm_count);
+    o_smem = o_items ? set_item_shape(o, entry_tokens) : os.smem;
+    o.Y = o_items ? static_cast<void*>(ws + l.part) : c.y;
+    o.ldy = o_items ? c.D : c.ldy;
     if (g_smem > (size_t)d.max_smem_optin || o_smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
 
     CUtensorMap tg, tu, td;
