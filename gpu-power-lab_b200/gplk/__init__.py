@@ -269,15 +269,16 @@ def _need(fn: str, cond: bool) -> None:
         raise GplkError(fn, 1)
 
 
-def _fresh(nbytes: int, stream, device):
-    """A block of the caching allocator in the stream's own pool: calls that
-    overlap, and captured graphs, never share it."""
+def _fresh(nbytes: int, stream, like):
+    """A block of the caching allocator in the stream's own pool, on the device
+    of `like`, a uint8 tensor: calls that overlap, and captured graphs, never
+    share it."""
+    if stream is None:
+        return like.new_empty(nbytes)
     import torch
 
-    if stream is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return like.new_empty(nbytes)
 
 
 def _launch_on(index: int, stream, call) -> None:
@@ -285,7 +286,7 @@ def _launch_on(index: int, stream, call) -> None:
     take microseconds: torch.cuda.current_stream() alone would take three."""
     import torch
 
-    if torch.cuda.current_device() != index:
+    if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return _launch_on(index, stream, call)
     if stream is None:
@@ -330,7 +331,7 @@ def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None)
         ldx, ldy, ldr = K, N, N
     if isinstance(workspace, str):
         need = gemv_nvfp4_workspace_bytes(T, N, K)
-        workspace = _fresh(need, stream, X.device) if need else None
+        workspace = _fresh(need, stream, W) if need else None
     if workspace is not None:
         _need(fn, workspace.get_device() == dev and workspace.is_contiguous())
         wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
@@ -378,7 +379,7 @@ def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = Tr
     if T < 2:
         ldx = ldy = D
     if isinstance(workspace, str):
-        workspace = _fresh(max(1, moe_nvfp4_workspace_bytes(T, E, top, D, F)), stream, X.device)
+        workspace = _fresh(max(1, moe_nvfp4_workspace_bytes(T, E, top, D, F)), stream, gw)
     _need(fn, workspace.get_device() == dev and workspace.is_contiguous())
     # The bytes of a MoeCfg, packed in a third of the time its constructor takes.
     c = _moe_cfg(X.data_ptr(), router.data_ptr(), gw.data_ptr(), uw.data_ptr(), dw.data_ptr(), gs.data_ptr(),
