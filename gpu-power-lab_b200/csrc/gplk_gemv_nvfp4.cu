@@ -7,13 +7,6 @@
 namespace gplk {
 namespace fewtok {
 
-// Whether a block takes two tiles, which then share the activations' slots.
-static bool use_pairs(int T, int tiles, int stages) {
-    (void)tiles;
-    (void)stages;
-    return false && T;
-}
-
 // ---------------------------------------------------------------- conversion ahead of the products
 // Writes the B rows and scales of every stage as the ring holds them, a block
 // per token, so that the blocks of an Image kernel fetch them with one bulk
@@ -82,22 +75,18 @@ __global__ void __launch_bounds__(kImageThreads)
 
 constexpr int kSms = 148;
 
-// Shape of a product of T tokens on a B200. Up to 12 tokens' accumulators of two
-// tiles fit half of TMEM: a block then takes two tiles where that leaves at
-// least a block for every SM.
-static Shape plan(Params& p, int T, int N, int K) {
+// Sizes and slices of a product of T tokens.
+static void plan(Params& p, int T, int N, int K) {
     p.T = T;
     p.N = N;
     p.K = K;
     p.tiles = (N + kTileRows - 1) / kTileRows;
     p.k_stages = (K + kStageK - 1) / kStageK;
     p.kblocks = K / 64;
-    p.halves = use_pairs(T, p.tiles, p.k_stages) ? 2 : 1;
-    const int groups = (p.tiles + p.halves - 1) / p.halves;
-    const int per_sm = p.halves * ((kPlanes * T + 15) & ~15) > 128 ? 1 : 2;
-    p.split_log2 = choose_split_log2(groups, p.k_stages * p.halves, 8, per_sm * kSms);
-    return set_shape(p, T, false, ((p.k_stages - 1) >> p.split_log2) + 1);
+    const int per_sm = kPlanes * T > 128 ? 1 : 2;
+    p.split_log2 = choose_split_log2(p.tiles, p.k_stages, 8, per_sm * kSms);
 }
+static int block_stages(const Params& p) { return ((p.k_stages - 1) >> p.split_log2) + 1; }
 
 // Whether the activations are converted once, by a kernel of their own, or by
 // every block for itself: that keeps up with the weights up to about four tokens
@@ -105,16 +94,15 @@ static Shape plan(Params& p, int T, int N, int K) {
 // Measured, fused / image, us: 4x16384x8192 19.1 / 18.8 (64 units in a block),
 // 8x16384x4096 17.1 / 12.2 (64), 8x16384x2048 10.7 / 9.8 (32), 8x8192x2048
 // 7.2 / 7.5 (16), 6x4096x4096 7.4 / 8.0 (12), 2x16384x8192 16.3 / 18.8 (32).
-static bool use_image(const Params& p) { return p.T >= 4 && p.T * (((p.k_stages - 1) >> p.split_log2) + 1) >= 24; }
+static bool use_image(const Params& p) { return p.T >= 4 && p.T * block_stages(p) >= 24; }
 
 // Workspace of the converted activations: the stages' images, then the
 // tokens' largest magnitudes.
-static size_t image_bytes(int T, int k_stages) { return (size_t)k_stages * geometry(T, 1, 0, 0).image; }
+static size_t image_bytes(int T, int k_stages) { return (size_t)k_stages * geometry(T, 1, Fill::Image, 0, 0).image; }
 
 template <typename XT>
 static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* workspace, cudaStream_t stream) {
-    const int groups = (p.tiles + p.halves - 1) / p.halves;
-    if (!workspace) return launch_stream<Mode::Gemv, XT, XT>(tm, tm, p, s.smem, groups, stream);
+    if (!workspace) return launch_stream<Mode::Gemv, XT, XT>(tm, tm, p, s.smem, p.tiles, stream);
     uint8_t* image = static_cast<uint8_t*>(workspace);
     uint32_t* amax = reinterpret_cast<uint32_t*>(image + image_bytes(p.T, p.k_stages));
     const int st = launch_status(launch_pdl(image_kernel<XT>, dim3((unsigned)p.T), dim3(kImageThreads), 0, stream,
@@ -123,7 +111,7 @@ static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* w
     if (st != GPLK_STATUS_OK) return st;
     p.image = image;
     p.amax = amax;
-    return launch_stream<Mode::Gemv, XT, XT, true>(tm, tm, p, s.smem, groups, stream);
+    return launch_stream<Mode::Gemv, XT, XT, true>(tm, tm, p, s.smem, p.tiles, stream);
 }
 
 }  // namespace fewtok
@@ -169,10 +157,11 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     p.ldy = ldy;
     p.ldr = ldr;
     p.x_vec = aligned16(X) && (T == 1 || ldx % 8 == 0);
-    const Shape s = plan(p, T, N, K);
-    if (s.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
+    plan(p, T, N, K);
     const size_t need = use_image(p) ? image_bytes(T, p.k_stages) + sizeof(uint32_t) * kMaxTokens : 0;
     void* ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;
+    const Shape s = set_shape(p, T, false, 1, ws ? Fill::Image : Fill::Convert, block_stages(p));
+    if (s.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
     CUtensorMap tm;
     st = encode_weights(&tm, W, (uint64_t)N, K);
     if (st != GPLK_STATUS_OK) return st;

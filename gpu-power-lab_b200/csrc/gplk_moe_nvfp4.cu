@@ -679,11 +679,10 @@ __global__ void __launch_bounds__(kItemThreads, 1)
 // Shared memory and TMEM of such a block: all of an SM's.
 static size_t set_item_shape(Params& p, int entry_tokens) {
     const size_t overhead = 1024 + ((sizeof(ItemControl) + 127) & ~(size_t)127);
-    p.halves = 2;
     p.ring_bytes = (uint32_t)((227 * 1024 - overhead) & ~(size_t)1023);
     p.tmem_cols = 512;
     for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
-    p.geo[0] = geometry(entry_tokens, 2, p.ring_bytes, p.tmem_cols, 2);
+    p.geo[0] = geometry(entry_tokens, 2, Fill::Convert, p.ring_bytes, p.tmem_cols, 2);
     return p.ring_bytes + overhead;
 }
 
@@ -808,13 +807,11 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     if (g_items) {
         g_smem = set_item_shape(g, entry_tokens);
     } else {
-        g.halves = 2;
-        const Shape s = set_shape(g, entry_tokens, true, g.k_stages);
+        const Shape s = set_shape(g, entry_tokens, true, 2, Fill::Convert, g.k_stages);
         g_smem = s.smem;
         g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, 8, s.per_sm * d.sm_count);
     }
-    o.halves = 1;
-    const Shape os = set_shape(o, c.T, false, o.k_stages * max_entries);
+    const Shape os = set_shape(o, c.T, false, 1, Fill::Convert, o.k_stages * max_entries);
     o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, 8, os.per_sm * d.sm_count);
     const bool o_items = use_down_items(c.T, active, o.tiles, o.k_stages, 1 << o.split_log2, d.sm_count);
     o_smem = o_items ? set_item_shape(o, entry_tokens) : os.smem;

@@ -106,12 +106,17 @@ struct Geometry {
     uint32_t sfb_cols;   // TMEM columns of a slot's B scales
 };
 
-// A slot of activations has no barriers of its own: it is filled before, and
-// freed with, the weights' slot that follows it. Tile j of the stream (h of stage
-// i: j = i * halves + h) takes weights' slot j % w, so whoever has seen that
-// slot free knows that tiles up to j - w are done; with b slots such that stage
-// i - b is among those, the activations' slot is free too: b = w for single
-// tiles, b = w / 2 + 1 for pairs.
+// A slot of activations has no barriers of its own. Tile j of the stream (tile h
+// of stage i: j = i * tiles + h) takes weights' slot j % w, so whoever has seen
+// that slot free knows that tiles up to j - w are done. Blocks that convert
+// fill the activations' slot of stage i then, which has to be free too: b = w
+// slots for single tiles, b = w / 2 + 1 for pairs. An Image block copies stage
+// i - w + b's then: its activations come out of L2, sooner than the weights, so
+// that it holds four stages of them and the more of weights. (Weights on their
+// way are what counts: with as many slots of both, 28 x 8192 x 8192 takes 18.6
+// instead of 16.8 us, 8 x 16384 x 8192 18.5 instead of 17.9.)
+constexpr int kImageSlots = 4;
+
 static uint32_t ring_of(const Geometry& g) {
     return (uint32_t)g.w_slots * kWSlot + (uint32_t)g.b_slots * g.b_slot;
 }
@@ -119,7 +124,9 @@ static uint32_t columns_of(const Geometry& g, int accs) {
     return (uint32_t)accs * g.acc_cols + (uint32_t)g.w_slots * 16 + (uint32_t)g.b_slots * g.sfb_cols;
 }
 
-static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tmem_cols, int accs = 1,
+enum class Fill { Convert, Image };
+
+static Geometry geometry(int ntok, int tiles, Fill fill, uint32_t ring_bytes, uint32_t tmem_cols, int accs = 1,
                          int most_slots = kMaxSlots) {
     Geometry g;
     g.nb = (kPlanes * ntok + 7) & ~7;
@@ -134,8 +141,10 @@ static Geometry geometry(int ntok, int halves, uint32_t ring_bytes, uint32_t tme
     g.acc_cols = ((uint32_t)g.nb + 15) & ~15u;
     g.sfb_cols = wide ? 32 : 16;
     for (g.w_slots = most_slots; g.w_slots > 1; --g.w_slots) {
-        g.b_slots = halves == 1 ? g.w_slots : g.w_slots / 2 + 1;
-        if (ring_of(g) <= ring_bytes && columns_of(g, accs * halves) <= tmem_cols) return g;
+        g.b_slots = tiles == 2 ? g.w_slots / 2 + 1
+                    : fill == Fill::Image && g.w_slots > kImageSlots ? kImageSlots
+                                                                     : g.w_slots;
+        if (ring_of(g) <= ring_bytes && columns_of(g, accs * tiles) <= tmem_cols) return g;
     }
     g.b_slots = 1;
     return g;
@@ -160,7 +169,6 @@ struct Params {
     int top;
     uint32_t inverse[kMaxTokens + 1];  // 2^16 / n + 1
     int tiles;           // 128-row tiles of one matrix
-    int halves;          // tiles a block takes: 1 or 2 (GateUp: 2, gate's and up's)
     int k_stages;        // stages of one matrix row
     int kblocks;         // K / 64
     int split_log2;      // slices of K, the cluster's size
@@ -388,7 +396,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     auto set_up = [&](int ntok) {
         if (threadIdx.x < kMaxSlots) {
             const int i = (int)threadIdx.x;
-            mbar_init(&sm.full[i], IMAGE ? 1u : 1u + (uint32_t)(kPerExpert ? kConvWarps : min(ntok, kConvWarps)));
+            mbar_init(&sm.full[i], IMAGE ? 2u : 1u + (uint32_t)(kPerExpert ? kConvWarps : min(ntok, kConvWarps)));
             mbar_init(&sm.empty[i], 1);
             if (i == 0) {
                 mbar_init(&sm.acc_full, 1);
@@ -420,10 +428,10 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     pdl_launch_dependents();
 
     // This block's rows, tokens and stages.
-    int group = cid, expert = 0, ntok = p.T, total = p.k_stages;
+    int tile = cid, expert = 0, ntok = p.T, total = p.k_stages;
     if constexpr (kPerExpert) {
         const int a = cid / p.tiles;
-        group = cid % p.tiles;
+        tile = cid % p.tiles;
         const int head = p.route->head[a];
         if (threadIdx.x < kMaxEntryTokens) sm.slot[threadIdx.x] = p.route->list[a][threadIdx.x];
         expert = head & 0xFFFF;
@@ -438,19 +446,14 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     }
     const int first = (total * slice) >> p.split_log2;
     const int nst = ((total * (slice + 1)) >> p.split_log2) - first;
-    // Tiles: GateUp the same rows of gate and up, else up to `halves` neighbours.
-    const int tile0 = M == Mode::GateUp ? group : group * p.halves;
-    const int nw = M == Mode::GateUp ? 2 : min(p.halves, p.tiles - tile0);
-    Geometry g = p.geo[kPerExpert ? ntok - 1 : 0];
+    constexpr int nw = M == Mode::GateUp ? 2 : 1;  // tiles: GateUp the same rows of gate and of up
+    const Geometry g = p.geo[kPerExpert ? ntok - 1 : 0];
     uint8_t* const b_ring = ring + (size_t)g.w_slots * kWSlot;
-    // The last tile of an odd number runs alone in rings made for pairs: as
-    // many slots of weights as of activations.
-    if (M != Mode::GateUp && nw < p.halves) g.w_slots = min(g.w_slots, g.b_slots);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
-    const uint32_t sfa_col0 = tmem + (M == Mode::GateUp ? 2u : (uint32_t)p.halves) * g.acc_cols;
+    const uint32_t sfa_col0 = tmem + (uint32_t)nw * g.acc_cols;
     const uint32_t sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
 
     if (warp == 0) {
@@ -466,17 +469,22 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 kb = first % p.k_stages;
                 if (nst > 0) expert = p.route->head[entry] & 0xFFFF;
             }
-            // An Image kernel fills the ring with weights before it waits for
-            // the conversion; tile j's activations follow it when j is `late`.
-            int late = IMAGE ? min(nst * nw, g.w_slots) : 0;
-            auto load_image = [&](int i, uint64_t* bar) {
-                bulk_load(b_ring + (size_t)b.slot * g.b_slot, p.image + (size_t)(first + i) * g.image, g.image, bar);
+            // An Image kernel fills the ring with weights before it waits for the
+            // conversion; then stage i - w + b's activations follow tile i's weights.
+            Cursor img;
+            int next_image = 0;
+            auto load_image = [&]() {
+                uint64_t* full = &sm.full[img.slot];
+                mbar_arrive_expect_tx(full, g.image);
+                bulk_load(b_ring + (size_t)b.slot * g.b_slot, p.image + (size_t)(first + next_image) * g.image, g.image,
+                          full);
+                ++next_image;
+                img.advance(g.w_slots);
                 b.advance(g.b_slots);
             };
-            auto load_late = [&]() {
+            auto first_images = [&]() {
                 pdl_wait();
-                for (int j = 0; j < late; j += nw) load_image(nw == 2 ? j >> 1 : j, &sm.full[j]);
-                late = 0;
+                while (next_image < min(nst, g.b_slots)) load_image();
             };
             for (int i = 0; i < nst && ok; ++i) {
                 const uint32_t sf_bytes = 512u * (uint32_t)min(4, p.kblocks - 4 * kb);
@@ -485,24 +493,18 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                         ok = false;
                         break;
                     }
-                    const bool up = M == Mode::GateUp && h == 1;
-                    const int tile = M == Mode::GateUp ? tile0 : tile0 + h;
+                    const bool up = h == 1;
                     uint8_t* st = ring + (size_t)c.slot * kWSlot;
                     const uint8_t* sf = (up ? p.sf1 : p.sf0) + (size_t)expert * sf_matrix +
                                         ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
                     uint64_t* full = &sm.full[c.slot];
-                    mbar_arrive_expect_tx(full, kWBytes + sf_bytes + (IMAGE && h == 0 ? g.image : 0u));
+                    mbar_arrive_expect_tx(full, kWBytes + sf_bytes);
                     tma_load_2d(st, up ? &tm1 : &tm0, full, kb * 128, expert * p.N + tile * kTileRows);
                     bulk_load(st + kWBytes, sf, sf_bytes, full);
                     ++issued;
                     if constexpr (IMAGE) {
-                        if (issued < late) {
-                            // more weights first
-                        } else if (late) {
-                            load_late();
-                        } else if (h == 0) {
-                            load_image(i, full);
-                        }
+                        if (issued == min(nst, g.w_slots)) first_images();
+                        else if (issued > g.w_slots) load_image();
                     }
                     c.advance(g.w_slots);
                 }
@@ -515,7 +517,18 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     }
                 }
             }
-            if (late) load_late();
+            if constexpr (IMAGE) {
+                // The last stages' activations, as their slots come free: stage m's with
+                // stage m - b, which is when tile m - b + w could go on.
+                if (nst < g.w_slots) {
+                    c.slot = 0;
+                    c.phase = 1;
+                }
+                for (; ok && next_image < nst; c.advance(g.w_slots)) {
+                    ok = mbar_wait(&sm.empty[c.slot], c.phase ^ 1u, &sm.abort, 0x0603);
+                    if (ok) load_image();
+                }
+            }
             if (!ok || *(volatile int*)&sm.abort) {
                 // Drain: every issued copy must land before the block exits.
                 int dummy = 0;
@@ -809,7 +822,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
 #pragma unroll
                     for (int i = 0; i < 5; ++i) tmem_ld_32x32b_x8(acc + (uint32_t)(kPlanes * t0 + 8 * i), c[i]);
                     // With one slice the sums are final: no other block has a part.
-                    const int n = (tile0 + h) * kTileRows + row;
+                    const int n = tile * kTileRows + row;
                     float r[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -846,8 +859,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         // A thread has four rows of a token at a time.
         const int rows = kTileRows >> p.split_log2;  // 16 to 128
         const uint32_t base = smem_u32(ring);
-        const int sums = (ntok * rows) >> 2;  // of one tile, in fours
-        const int fours = M == Mode::GateUp ? sums : split == 1 ? 0 : nw * sums;
+        const int fours = M != Mode::GateUp && split == 1 ? 0 : (ntok * rows) >> 2;
         if constexpr (M == Mode::GateUp) {
             // sm.amax now gathers h's largest magnitudes.
             __syncthreads();
@@ -855,11 +867,10 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             __syncthreads();
         }
         for (int i = (int)threadIdx.x; i < fours; i += kThreads<IMAGE>) {
-            const int h = i >= sums ? 1 : 0, j = (i - h * sums) << 2;
-            const int t = j >> (7 - p.split_log2), r = slice * rows + (j & (rows - 1));
-            const int n = (tile0 + (M == Mode::GateUp ? 0 : h)) * kTileRows + r;
+            const int j = i << 2, t = j >> (7 - p.split_log2), r = slice * rows + (j & (rows - 1));
+            const int n = tile * kTileRows + r;
             if (n >= p.N) continue;
-            const uint32_t off = base + (uint32_t)((h * ntok + t) * kTileRows + r) * 4u;
+            const uint32_t off = base + (uint32_t)(t * kTileRows + r) * 4u;
             if constexpr (M == Mode::GateUp) {
                 const float4 s4 = sum_cluster(off, split);
                 const float4 u4 = sum_cluster(off + (uint32_t)(ntok * kTileRows) * 4u, split);
@@ -928,12 +939,12 @@ struct Shape {
 // whatever launches, then fit its TMEM too.
 static size_t share_of_smem(uint32_t tmem_cols) { return (size_t)228 * 1024 * tmem_cols / 512 - 1024; }
 
-// A block of `tokens` tokens, or of 1 to `tokens` with a geometry for each, and of
-// at most `stages` stages: no more than those want, up to half of an SM, or up to
+// A block of `tokens` tokens, or of 1 to `tokens` with a geometry for each, of 1 or
+// 2 tiles and of at most `stages` stages: no more than those want, up to half of an SM, or up to
 // all of it where half holds fewer than three tiles' slots.
-static Shape set_shape(Params& p, int tokens, bool each, int stages) {
+static Shape set_shape(Params& p, int tokens, bool each, int tiles, Fill fill, int stages) {
     const size_t overhead = 1024 + ((sizeof(Control) + 127) & ~(size_t)127);
-    const int want = (long long)stages * p.halves < kMaxSlots ? stages * p.halves : kMaxSlots;
+    const int want = stages < kMaxSlots ? (stages * tiles < kMaxSlots ? stages * tiles : kMaxSlots) : kMaxSlots;
     for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
     Shape s;
     uint32_t ring = 0, cols = 0;
@@ -941,17 +952,17 @@ static Shape set_shape(Params& p, int tokens, bool each, int stages) {
         ring = cols = 0;
         bool enough = true;
         for (int t = each ? 1 : tokens; t <= tokens; ++t) {
-            const Geometry g = geometry(t, p.halves, (uint32_t)(share_of_smem(most) - overhead), most, 1, want);
-            enough = enough && columns_of(g, p.halves) <= most && g.w_slots >= (want < 3 ? want : 3);
+            const Geometry g = geometry(t, tiles, fill, (uint32_t)(share_of_smem(most) - overhead), most, 1, want);
+            enough = enough && columns_of(g, tiles) <= most && g.w_slots >= (want < 3 ? want : 3);
             ring = ring_of(g) > ring ? ring_of(g) : ring;
-            cols = columns_of(g, p.halves) > cols ? columns_of(g, p.halves) : cols;
+            cols = columns_of(g, tiles) > cols ? columns_of(g, tiles) : cols;
             p.geo[each ? t - 1 : 0] = g;
         }
         if (enough) break;
     }
     for (p.tmem_cols = 32; p.tmem_cols < cols;) p.tmem_cols *= 2;
     // The slices' sums lie over the rings.
-    const uint32_t sums = (uint32_t)(p.halves * tokens * kTileRows * 4);
+    const uint32_t sums = (uint32_t)(tiles * tokens * kTileRows * 4);
     p.ring_bytes = ((ring > sums ? ring : sums) + 1023) & ~1023u;
     s.smem = p.ring_bytes + overhead;
     if (s.smem < share_of_smem(p.tmem_cols)) s.smem = share_of_smem(p.tmem_cols);
