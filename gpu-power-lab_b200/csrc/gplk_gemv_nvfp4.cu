@@ -84,7 +84,7 @@ static void plan(Params& p, int T, int N, int K) {
     p.k_stages = (K + kStageK - 1) / kStageK;
     p.kblocks = K / 64;
     const int per_sm = kPlanes * T > 128 ? 1 : 2;
-    p.split_log2 = choose_split_log2(p.tiles, p.k_stages, 8, per_sm * kSms);
+    p.split_log2 = choose_split_log2(p.tiles, p.k_stages, kSms, per_sm);
 }
 static int block_stages(const Params& p) { return ((p.k_stages - 1) >> p.split_log2) + 1; }
 

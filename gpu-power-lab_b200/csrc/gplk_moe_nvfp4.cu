@@ -18,8 +18,6 @@
 //             (experts x F) against each token's h (zero where the expert is
 //             not the token's), so the weighted sum over experts happens in
 //             the accumulator and no atomics or second pass join it.
-#include <cmath>
-
 #include "gplk_ptx.cuh"
 
 namespace gplk {
@@ -809,10 +807,10 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     } else {
         const Shape s = set_shape(g, entry_tokens, true, 2, Fill::Convert, g.k_stages);
         g_smem = s.smem;
-        g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, 8, s.per_sm * d.sm_count);
+        g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, d.sm_count, s.per_sm);
     }
     const Shape os = set_shape(o, c.T, false, 1, Fill::Convert, o.k_stages * max_entries);
-    o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, 8, os.per_sm * d.sm_count);
+    o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, d.sm_count, os.per_sm);
     const bool o_items = use_down_items(c.T, active, o.tiles, o.k_stages, 1 << o.split_log2, d.sm_count);
     o_smem = o_items ? set_item_shape(o, entry_tokens) : os.smem;
     o.Y = o_items ? static_cast<void*>(ws + l.part) : c.y;
