@@ -28,11 +28,11 @@
 // 256 an instruction takes.
 //
 // Layout of the work. A block owns 128 weight rows (the MMA's M), or two such
-// tiles that share the activations' rows (gate and up of an expert, or
-// neighbours), and a slice of K; blocks of a cluster share the rows, split K,
-// and add their partial sums in rank order through distributed shared memory,
-// so the bits do not depend on timing. Two blocks share an SM where TMEM allows:
-// one's start and end hide behind the other's stream.
+// tiles that share the activations' rows (gate and up of an expert), and a slice
+// of K; blocks of a cluster share the rows, split K, and add their partial sums
+// in rank order through distributed shared memory, so the bits do not depend on
+// timing. Two blocks share an SM where TMEM allows: one's start and end hide
+// behind the other's stream.
 //   warp 0      TMA producer: 128 rows x 128 bytes of codes and up to 2 KiB of
 //               scales (256 elements of K) per slot of the weights' ring
 //   warp 1      owns TMEM, copies the scales there and issues one MMA per 64
@@ -44,7 +44,10 @@
 //               warps 2..5 only.
 // The MMA warp runs its loop converged and elects the issuing lane: with
 // addresses and descriptors in uniform registers, 65536 x 8192 at one token
-// takes 51 us; issued from a lane of a diverged warp 76 us.
+// takes 51 us; issued from a lane of a diverged warp 76 us. At one token that is
+// 5.9 TB/s, with 4.5 us of start and end in smaller calls; at 32 tokens what counts
+// is the weights on their way (16384 x 16384: 42 us; 37 without any MMA, scale
+// copy or activation), since activations take half of the shared memory.
 // Every mbarrier wait is bounded, as everywhere in this library.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -152,13 +155,13 @@ static Geometry geometry(int ntok, int tiles, Fill fill, uint32_t ring_bytes, ui
 }
 
 struct Params {
-    const void* X;       // activations (Gemv, GateUp: 16-bit rows; Down*: FP32 h rows by slot)
+    const void* X;       // activations (16-bit rows; for down: FP32 h rows by slot)
     const uint8_t* sf0;  // scales: W, gate or down
     const uint8_t* sf1;  // GateUp: up
     const float* alpha0; // Gemv: one; GateUp: gate's, per expert
     const float* alpha1; // GateUp: up's
     const float* alpha2; // GateUp: down's, folded into h
-    void* Y;             // Gemv, Down: T rows; GateUp, DownPart: FP32 rows by slot
+    void* Y;             // T rows; from gate and up, and from resident down blocks: FP32 rows by slot
     const void* R;
     const Route* route;
     const float* weights;  // MoE: per slot
@@ -380,7 +383,8 @@ constexpr int kThreads = IMAGE ? 64 + 128 : 64 + 32 * kConvWarps;
 
 template <Mode M, typename XT, typename YT, bool IMAGE>
 __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
-    stream_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1, const __grid_constant__ Params p) {
+    stream_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1,
+                  const __grid_constant__ Params p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     Control& sm = *reinterpret_cast<Control*>(ring + p.ring_bytes);
@@ -438,7 +442,9 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         expert = head & 0xFFFF;
         ntok = head >> 16;
         if (ntok == 0) {  // behind the last entry: the whole cluster leaves
+            tc_fence_before();
             __syncthreads();
+            tc_fence_after();
             if (warp == 1) tmem_dealloc(sm.tmem_base, p.tmem_cols);
             return;
         }
@@ -810,8 +816,8 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 tc_fence_after();
             }
             for (int h = 0; h < nw; ++h, part += ntok * kTileRows) {
-                const float alpha = M == Mode::Gemv ? __ldg(p.alpha0)
-                                    : M == Mode::GateUp ? __ldg((h ? p.alpha1 : p.alpha0) + expert)
+                const float alpha = M == Mode::Gemv ? p.alpha0[0]
+                                    : M == Mode::GateUp ? (h ? p.alpha1 : p.alpha0)[expert]
                                                         : 1.0f;
                 const uint32_t acc = tmem + ((quarter * 32u) << 16) + (uint32_t)h * g.acc_cols;
                 for (int t0 = 0; t0 < ntok; t0 += 8) {
@@ -876,7 +882,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 const float4 s4 = sum_cluster(off, split);
                 const float4 u4 = sum_cluster(off + (uint32_t)(ntok * kTileRows) * 4u, split);
                 const int slot = sm.slot[t];
-                const float c = p.weights[slot] * __ldg(p.alpha2 + expert);
+                const float c = p.weights[slot] * p.alpha2[expert];
                 const float s[4] = {s4.x, s4.y, s4.z, s4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
                 float hv[4];
                 uint32_t m = 0;
@@ -941,8 +947,8 @@ struct Shape {
 static size_t share_of_smem(uint32_t tmem_cols) { return (size_t)228 * 1024 * tmem_cols / 512 - 1024; }
 
 // A block of `tokens` tokens, or of 1 to `tokens` with a geometry for each, of 1 or
-// 2 tiles and of at most `stages` stages: no more than those want, up to half of an SM, or up to
-// all of it where half holds fewer than three tiles' slots.
+// 2 tiles and of at most `stages` stages: no more than those want, up to half of an
+// SM, or up to all of it where half holds fewer than three tiles' slots.
 static Shape set_shape(Params& p, int tokens, bool each, int tiles, Fill fill, int stages) {
     const size_t overhead = 1024 + ((sizeof(Control) + 127) & ~(size_t)127);
     const int want = stages < kMaxSlots ? (stages * tiles < kMaxSlots ? stages * tiles : kMaxSlots) : kMaxSlots;
@@ -1042,7 +1048,6 @@ static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const P
 static int encode_weights(CUtensorMap* map, const uint8_t* W, uint64_t rows, int K) {
     return encode_tmap_2d_u8(map, W, (uint64_t)K / 2, rows, (uint64_t)K / 2, 128, kTileRows);
 }
-
 
 }  // namespace fewtok
 }  // namespace gplk

@@ -18,7 +18,8 @@ def _gen(cuda, seed):
     return g
 
 
-def _check(gplk, cuda, t, n, k, dtype="bf16", residual=None, pad=0, seed=0, x=None, alpha=0.0123, pad_byte=0x7F):
+def _check(gplk, cuda, t, n, k, dtype="bf16", residual=None, pad=0, seed=0, x=None, alpha=0.0123, pad_byte=0x7F,
+           **kw):
     import torch
 
     gen = _gen(cuda, seed + 7 * t + 31 * n + k)
@@ -41,7 +42,7 @@ def _check(gplk, cuda, t, n, k, dtype="bf16", residual=None, pad=0, seed=0, x=No
     if r is not None:
         want = want + r.double()
         err = err + 2.0 ** -24 * want.abs()
-    gplk.gemv_nvfp4(x, w, sf, y, al, residual=r)
+    gplk.gemv_nvfp4(x, w, sf, y, al, residual=r, **kw)
     torch.cuda.synchronize()
     got = y.double()
     assert torch.isfinite(got).all()
@@ -69,6 +70,32 @@ def test_odd_outputs(t, n, gplk, cuda):
 @pytest.mark.parametrize("t", [1, 9])
 def test_depths(t, k, gplk, cuda):
     _check(gplk, cuda, t, 200, k)
+
+
+@pytest.mark.parametrize("tnk", [(4, 700, 8192), (8, 129, 8256), (17, 1000, 4160), (25, 128, 16384), (26, 300, 8192),
+                                 (32, 130, 16448), (32, 9000, 1088), (7, 20000, 1600)])
+@pytest.mark.parametrize("workspace", ["auto", None])
+def test_converted_ahead_or_by_every_block(tnk, workspace, gplk, cuda):
+    """Sizes about and above where activations are converted ahead of the
+    products, and the same without the workspace that this takes."""
+    _check(gplk, cuda, *tnk, workspace=workspace, residual="apart", pad=3)
+
+
+def test_workspace_of_any_content_and_size(gplk, cuda):
+    """A workspace full of NaN serves; one a byte short is not used; both agree
+    with the automatic one's product."""
+    import torch
+
+    t, n, k = 9, 500, 8192
+    need = gplk.gemv_nvfp4_workspace_bytes(t, n, k)
+    auto = _check(gplk, cuda, t, n, k)
+    full = _check(gplk, cuda, t, n, k, workspace=torch.full((need,), 0xFF, dtype=torch.uint8, device=cuda))
+    short = torch.full((need,), 0xFF, dtype=torch.uint8, device=cuda)
+    without = _check(gplk, cuda, t, n, k, workspace=short[: need - 1])
+    none = _check(gplk, cuda, t, n, k, workspace=None)
+    assert bool((short == 0xFF).all())
+    assert torch.equal(auto.view(torch.int16), full.view(torch.int16))
+    assert torch.equal(without.view(torch.int16), none.view(torch.int16))
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
@@ -234,6 +261,38 @@ def test_empty(gplk, cuda):
     gplk.gemv_nvfp4(torch.empty(0, 64, dtype=torch.bfloat16, device=cuda), w, sf,
                     torch.empty(0, 8, dtype=torch.bfloat16, device=cuda), al)
     torch.cuda.synchronize()
+
+
+def test_two_calls_at_once_converting_ahead(gplk, cuda):
+    """Products of many tokens on two streams, replayed from two graphs that
+    were captured with automatic workspaces."""
+    import torch
+
+    gen = _gen(cuda, 21)
+    w, sf, _ = ref.random_weights(2000, 4096, gen, cuda)
+    al = torch.ones(1, device=cuda)
+    xs = [torch.zeros(16, 4096, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    ys = [torch.empty(16, 2000, dtype=torch.bfloat16, device=cuda) for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g, x, y in zip(graphs, xs, ys):
+        with torch.cuda.graph(g):
+            gplk.gemv_nvfp4(x, w, sf, y, al)
+            gplk.gemv_nvfp4(x, w, sf, y, al, residual=y)
+    streams = [torch.cuda.Stream(device=cuda) for _ in range(2)]
+    for _ in range(4):
+        for x in xs:
+            x.copy_(torch.randn(16, 4096, device=cuda, generator=gen))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(xs, ys):
+            e = torch.empty_like(y)
+            gplk.gemv_nvfp4(x, w, sf, e, al)
+            gplk.gemv_nvfp4(x, w, sf, e, al, residual=e)
+            torch.cuda.synchronize()
+            assert torch.equal(y.view(torch.int16), e.view(torch.int16))
 
 
 def test_python_refusals(gplk, cuda):

@@ -84,6 +84,39 @@ def test_widths(t, d, f, gplk, cuda):
     _case(gplk, cuda, t, 4, 2, d, f)
 
 
+@pytest.mark.parametrize("t,e,top,d,f", [
+    (8, 64, 8, 640, 1024),    # items for resident blocks, an odd number of down's tiles
+    (32, 40, 4, 320, 1088),   # the same, tiles cut short, some experts with several tokens
+    (32, 2, 2, 192, 128),     # every expert has all 32 tokens: three entries each
+    (32, 1, 1, 1024, 20480),  # resident gate / up of one expert in three entries
+    (32, 512, 16, 64, 64),    # the most experts, ranks and tokens
+    (3, 8, 2, 1024, 8192),    # down accumulates over long K
+    (12, 300, 3, 128, 192),   # more experts than four to a lane
+])
+def test_paths(t, e, top, d, f, gplk, cuda):
+    _case(gplk, cuda, t, e, top, d, f)
+
+
+def test_without_ids_and_weights(gplk, cuda):
+    """Through the C ABI with NULL for both: the same y."""
+    import ctypes
+
+    import torch
+
+    layer = Layer(6, 128, 192, torch.bfloat16, _gen(cuda, 10), cuda)
+    x = torch.randn(5, 128, device=cuda, generator=_gen(cuda, 11)).to(torch.bfloat16)
+    y, _, _ = layer.run(gplk, x, 2)
+    z = torch.empty_like(y)
+    ws = torch.empty(gplk.moe_nvfp4_workspace_bytes(5, 6, 2, 128, 192), dtype=torch.uint8, device=cuda)
+    p = lambda a: a.data_ptr()  # noqa: E731
+    g, u, d = layer.gate, layer.up, layer.down
+    c = gplk.MoeCfg(p(x), p(layer.router), p(g[0]), p(u[0]), p(d[0]), p(g[1]), p(u[1]), p(d[1]), p(g[2]), p(u[2]),
+                    p(d[2]), p(z), None, None, p(ws), ws.numel(), 5, 6, 2, 128, 192, 128, 128, 1, 0)
+    assert gplk.lib().gplk_moe_nvfp4(ctypes.byref(c), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y.view(torch.int16), z.view(torch.int16))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("renorm", [True, False])
 @pytest.mark.parametrize("pad", [0, 1, 8])
