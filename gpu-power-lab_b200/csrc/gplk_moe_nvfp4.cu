@@ -24,10 +24,9 @@
 // No atomics order a sum; the maxima that atomics find do not depend on it.
 // Measured, us, against the bytes at 6547 GB/s: 1 token 64/8 2048x1024 20 (4.4),
 // 8 tokens 128/8 4096x768 68 (41), 16 tokens 16/2 4096x4096 85 (61), 32 tokens
-// 64/6 4096x2048 172 (132). Small layers are the launches' latencies, 15.5 us at
+// 64/6 4096x2048 163 (132). Small layers are the launches' latencies, 15.5 us at
 // least; large ones what resident blocks do not overlap: routing before the first
-// weight (some 10 us), a last round of items that not all SMs have, and, at three
-// tokens an expert, the conversion (12 of the 172 us).
+// weight (some 10 us) and a last round of items that not all SMs have.
 #include "gplk_ptx.cuh"
 
 namespace gplk {
@@ -350,8 +349,11 @@ static bool few_experts(int T, int E, int D) { return T <= 4 && E <= 32 * kFewPe
 // (two sets) drain. stream_kernel starts a block per item instead, which costs
 // about 4 us of an SM's stream each; there K is split over a cluster, which is
 // what few items need.
-//   warp 0 copies, warp 1 MMAs, warps 2..9 convert, warps 10..13 epilogue
-constexpr int kItemThreads = 32 * 14;
+//   warp 0 copies, warp 1 MMAs, warps 2..17 convert, warps 18..21 epilogue
+// (8 / 12 / 16 converting warps, us: 32 tokens 32/8 4096x2048 156 / 137 / 128, 64/6
+// 4096x2048 173 / 165 / 163, 8 tokens 128/8 4096x768 67.5 / 67.3 / 68.8.)
+constexpr int kItemConvWarps = 16;
+constexpr int kItemThreads = 32 * (6 + kItemConvWarps);
 
 struct ItemControl {
     uint64_t full[kMaxSlots];
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     uint8_t* const b_ring = ring + (size_t)g.w_slots * kWSlot;
 
     if (threadIdx.x < kMaxSlots) {
-        mbar_init(&sm.full[threadIdx.x], 1 + kConvWarps);
+        mbar_init(&sm.full[threadIdx.x], 1 + kItemConvWarps);
         mbar_init(&sm.empty[threadIdx.x], 1);
         if (threadIdx.x < 2) {
             mbar_init(&sm.acc_full[threadIdx.x], 1);
@@ -517,9 +519,9 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         int dummy = 0;
         mbar_wait(&sm.drain, 0, &dummy, 0x0713, 100000000ull);
         __syncwarp();
-    } else if (warp < 2 + kConvWarps) {
+    } else if (warp < 2 + kItemConvWarps) {
         // ------------------------------------------------------------ activations
-        // Unit u = kb * tokens + t of an item is warp u % 8's.
+        // Unit u = kb * tokens + t of an item is warp u % 16's.
         const int w = (int)warp - 2;
         if constexpr (!GATE_UP) pdl_wait();
         struct Unit {
@@ -530,8 +532,8 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                 u.entry = u.it / groups;
                 u.ntok = p.route->head[u.entry] >> 16;
                 const uint32_t inverse = p.inverse[u.ntok];
-                u.step_kb = (int)(kConvWarps * inverse >> 16);
-                u.step_t = kConvWarps - u.step_kb * u.ntok;
+                u.step_kb = (int)(kItemConvWarps * inverse >> 16);
+                u.step_t = kItemConvWarps - u.step_kb * u.ntok;
                 u.kb = (int)((uint32_t)w * inverse >> 16);
                 u.t = w - u.kb * u.ntok;
                 if (u.kb < p.k_stages) return;

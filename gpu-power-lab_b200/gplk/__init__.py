@@ -281,19 +281,15 @@ def _fresh(nbytes: int, stream, like):
         return like.new_empty(nbytes)
 
 
-def _launch_on(index: int, stream, call) -> None:
-    """call(raw stream) with CUDA device `index` the current one. These calls
-    take microseconds: torch.cuda.current_stream() alone would take three."""
+def _raw_stream(fn: str, stream, index: int) -> int:
+    """The stream's handle, None: the current one of CUDA device `index`. These
+    calls take microseconds; torch.cuda.current_stream() alone would take three."""
     import torch
 
-    if torch._C._cuda_getDevice() != index:
-        with torch.cuda.device(index):
-            return _launch_on(index, stream, call)
     if stream is None:
-        return call(torch._C._cuda_getCurrentRawStream(index))
-    if stream.device_index != index:
-        raise GplkError("stream of another device", 1)
-    call(stream.cuda_stream)
+        return torch._C._cuda_getCurrentRawStream(index)
+    _need(fn, stream.device_index == index)
+    return stream.cuda_stream
 
 
 @functools.lru_cache(maxsize=4096)
@@ -311,9 +307,12 @@ def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None)
     or a uint8 CUDA tensor that no overlapping call uses."""
     import torch
 
-    fn, L = "gplk_gemv_nvfp4", lib()
+    fn, L = "gplk_gemv_nvfp4", _lib or lib()
     dt, u8, dev = _act_dtype(X), torch.uint8, X.get_device()
     _need(fn, dt >= 0 and dev >= 0 and X.dim() == Y.dim() == W.dim() == 2)
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return gemv_nvfp4(X, W, SF, Y, alpha, residual, workspace, stream)
     (T, K), (T2, N), (rows, row_bytes) = X.shape, Y.shape, W.shape
     (ldx, cx), (ldy, cy) = X.stride(), Y.stride()
     _need(fn, T2 == T and rows == N and row_bytes * 2 == K and (cx == 1 or K < 2) and (cy == 1 or N < 2)
@@ -335,9 +334,10 @@ def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None)
     if workspace is not None:
         _need(fn, workspace.get_device() == dev and workspace.is_contiguous())
         wp, wb = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _launch_on(dev, stream, lambda s: _check(fn, L.gplk_gemv_nvfp4(
-        X.data_ptr(), W.data_ptr(), SF.data_ptr(), Y.data_ptr(), rp, T, N, K, ldx, ldy, ldr, alpha.data_ptr(), dt, wp,
-        wb, s)))
+    st = L.gplk_gemv_nvfp4(X.data_ptr(), W.data_ptr(), SF.data_ptr(), Y.data_ptr(), rp, T, N, K, ldx, ldy, ldr,
+                           alpha.data_ptr(), dt, wp, wb, _raw_stream(fn, stream, dev))
+    if st:
+        raise GplkError(fn, st)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -358,10 +358,13 @@ def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = Tr
     call uses."""
     import torch
 
-    fn, L = "gplk_moe_nvfp4", lib()
+    fn, L = "gplk_moe_nvfp4", _lib or lib()
     dt, u8, f32, dev = _act_dtype(X), torch.uint8, torch.float32, X.get_device()
     (gw, gs, ga), (uw, us, ua), (dw, ds, da) = gate, up, down
     _need(fn, dt >= 0 and dev >= 0 and X.dim() == Y.dim() == router.dim() == ids.dim() == 2 and gw.dim() == 3)
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise, workspace, stream)
     T, D = X.shape
     E, top = router.shape[0], ids.shape[1]
     F = gw.shape[1]
@@ -371,11 +374,16 @@ def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = Tr
           and ids.is_contiguous() and weights.shape == ids.shape and weights.dtype == f32 and weights.is_contiguous()
           and router.get_device() == Y.get_device() == ids.get_device() == weights.get_device() == dev)
     up_shape, up_sf = (E, F, D // 2), E * -(-F // 128) * -(-D // 64) * 512
-    for w, sf, al, shape, n in ((gw, gs, ga, up_shape, up_sf), (uw, us, ua, up_shape, up_sf),
-                                (dw, ds, da, (E, D, F // 2), E * -(-D // 128) * -(-F // 64) * 512)):
-        _need(fn, w.shape == shape and w.dtype == u8 and sf.dtype == u8 and al.dtype == f32 and w.is_contiguous()
-              and sf.is_contiguous() and al.is_contiguous() and sf.numel() == n and al.numel() == E
-              and w.get_device() == sf.get_device() == al.get_device() == dev)
+    _need(fn, gw.shape == up_shape and uw.shape == up_shape and dw.shape == (E, D, F // 2)
+          and gs.numel() == up_sf and us.numel() == up_sf and ds.numel() == E * -(-D // 128) * -(-F // 64) * 512
+          and ga.numel() == E and ua.numel() == E and da.numel() == E
+          and gw.dtype == uw.dtype == dw.dtype == gs.dtype == us.dtype == ds.dtype == u8
+          and ga.dtype == ua.dtype == da.dtype == f32
+          and gw.is_contiguous() and uw.is_contiguous() and dw.is_contiguous() and gs.is_contiguous()
+          and us.is_contiguous() and ds.is_contiguous() and ga.is_contiguous() and ua.is_contiguous()
+          and da.is_contiguous()
+          and gw.get_device() == uw.get_device() == dw.get_device() == gs.get_device() == us.get_device()
+          == ds.get_device() == ga.get_device() == ua.get_device() == da.get_device() == dev)
     if T < 2:
         ldx = ldy = D
     if isinstance(workspace, str):
@@ -386,7 +394,9 @@ def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = Tr
                  us.data_ptr(), ds.data_ptr(), ga.data_ptr(), ua.data_ptr(), da.data_ptr(), Y.data_ptr(),
                  ids.data_ptr(), weights.data_ptr(), workspace.data_ptr(),
                  workspace.numel() * workspace.element_size(), T, E, top, D, F, ldx, ldy, bool(renormalise), dt)
-    _launch_on(dev, stream, lambda s: _check(fn, L.gplk_moe_nvfp4(c, s)))
+    st = L.gplk_moe_nvfp4(c, _raw_stream(fn, stream, dev))
+    if st:
+        raise GplkError(fn, st)
 
 
 # ------------------------------------------------------------ dense tensor-core GEMMs
