@@ -11,13 +11,16 @@ namespace fewtok {
 // Writes the B rows and scales of every stage as the ring holds them, a block
 // per token, so that the blocks of an Image kernel fetch them with one bulk
 // copy per stage instead of each converting all of the tokens again.
-constexpr int kImageThreads = 512;
+// (512 / 1024 threads, us of the product: 16x8192x8192 13.1 / 13.4, 32x16384x16384
+// 41.5 / 39.0: 512 up to K = 8192.)
+static int image_threads(int K) { return K <= 8192 ? 512 : 1024; }
 
 template <typename XT>
-__global__ void __launch_bounds__(kImageThreads)
+__global__ void __launch_bounds__(1024)
     image_kernel(const XT* X, uint8_t* image, uint32_t* amax, int K, int ldx, int x_vec, const Geometry g) {
-    __shared__ uint32_t top[kImageThreads / 32];
-    constexpr int kWarps = kImageThreads / 32, kHeld = 4;
+    __shared__ uint32_t top[32];
+    constexpr int kHeld = 4;
+    const int warps = (int)blockDim.x / 32;
     const int t = blockIdx.x, warp = (int)warp_id_uniform();
     const uint32_t lane = lane_id();
     const int stages = (K + kStageK - 1) / kStageK;
@@ -33,12 +36,12 @@ __global__ void __launch_bounds__(kImageThreads)
     };
     uint4 held[kHeld][2];  // the first stages stay in registers
     uint32_t m = 0;
-    for (int i0 = warp; i0 < stages; i0 += kHeld * kWarps) {
+    for (int i0 = warp; i0 < stages; i0 += kHeld * warps) {
         uint4 r[kHeld][2];
 #pragma unroll
         for (int c = 0; c < kHeld; ++c) {
             r[c][0] = r[c][1] = make_uint4(0, 0, 0, 0);
-            if (i0 + c * kWarps < stages) load(i0 + c * kWarps, r[c]);
+            if (i0 + c * warps < stages) load(i0 + c * warps, r[c]);
         }
 #pragma unroll
         for (int c = 0; c < kHeld; ++c) {
@@ -54,7 +57,7 @@ __global__ void __launch_bounds__(kImageThreads)
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) top[warp] = m;
     __syncthreads();
-    m = __reduce_max_sync(0xffffffffu, lane < kWarps ? top[lane] : 0u);
+    m = __reduce_max_sync(0xffffffffu, (int)lane < warps ? top[lane] : 0u);
     if (threadIdx.x == 0) amax[t] = m;
     const int anchor = anchor_of(m);
     auto emit = [&](int i, const uint4 (&r)[2]) {
@@ -65,8 +68,8 @@ __global__ void __launch_bounds__(kImageThreads)
     };
 #pragma unroll
     for (int c = 0; c < kHeld; ++c)
-        if (warp + c * kWarps < stages) emit(warp + c * kWarps, held[c]);
-    for (int i = warp + kHeld * kWarps; i < stages; i += kWarps) {
+        if (warp + c * warps < stages) emit(warp + c * warps, held[c]);
+    for (int i = warp + kHeld * warps; i < stages; i += warps) {
         uint4 r[2];
         load(i, r);
         emit(i, r);
@@ -105,7 +108,7 @@ static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* w
     if (!workspace) return launch_stream<Mode::Gemv, XT, XT>(tm, tm, p, s.smem, p.tiles, stream);
     uint8_t* image = static_cast<uint8_t*>(workspace);
     uint32_t* amax = reinterpret_cast<uint32_t*>(image + image_bytes(p.T, p.k_stages));
-    const int st = launch_status(launch_pdl(image_kernel<XT>, dim3((unsigned)p.T), dim3(kImageThreads), 0, stream,
+    const int st = launch_status(launch_pdl(image_kernel<XT>, dim3((unsigned)p.T), dim3(image_threads(p.K)), 0, stream,
                                             static_cast<const XT*>(p.X), image, amax, p.K, p.ldx, p.x_vec,
                                             p.geo[0]));
     if (st != GPLK_STATUS_OK) return st;
