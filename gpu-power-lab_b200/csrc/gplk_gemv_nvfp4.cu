@@ -142,7 +142,7 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     if (T == 0 || N == 0) return GPLK_STATUS_OK;
     if (K == 0 || K % 64 != 0 || ldx < K || ldy < N || (R && ldr < N)) return GPLK_STATUS_BAD_ARG;
     if (N > INT_MAX / 8 || K > INT_MAX / 8) return GPLK_STATUS_BAD_ARG;  // grids, sums of stages
-    if (!X || !W || !SF || !Y || !alpha) return GPLK_STATUS_BAD_ARG;
+    if (!X || !W || !SF || !Y || !alpha || X == Y) return GPLK_STATUS_BAD_ARG;
     if (!aligned16(W) || !aligned16(SF) || !aligned(X, 2) || !aligned(Y, 2) || !aligned(R, 2) || !aligned(alpha, 4) ||
         !aligned16(workspace))
         return GPLK_STATUS_BAD_ARG;

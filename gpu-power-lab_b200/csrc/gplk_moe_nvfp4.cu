@@ -405,6 +405,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     // pdl_wait() of the warps that read it.
     if constexpr (GATE_UP) pdl_wait();
     pdl_launch_dependents();
+    if constexpr (!GATE_UP) __threadfence();  // nothing older than the tables out of L1
     const uint32_t sfa_col0 = tmem + 4u * g.acc_cols, sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
     const int groups = GATE_UP ? p.tiles : (p.tiles + 1) / 2;
     const int items = p.route->n_entries * groups;

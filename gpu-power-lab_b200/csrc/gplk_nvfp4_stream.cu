@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     constexpr bool kEarly = IMAGE || M == Mode::Down;
     if constexpr (!kEarly) pdl_wait();
     pdl_launch_dependents();
+    if constexpr (M == Mode::Down) __threadfence();  // nothing older than the tables out of L1
 
     // This block's rows, tokens and stages.
     int tile = cid, expert = 0, ntok = p.T, total = p.k_stages;

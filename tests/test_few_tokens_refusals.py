@@ -11,7 +11,7 @@ PTR = 1 << 20  # never dereferenced: these calls end in an argument check
 
 
 def _gemv(gplk, **kw):
-    a = dict(X=PTR, W=PTR, SF=PTR, Y=PTR, R=None, T=1, N=128, K=256, ldx=256, ldy=128, ldr=0, alpha=PTR, dtype=0, workspace=None,
+    a = dict(X=PTR, W=PTR, SF=PTR, Y=2 * PTR, R=None, T=1, N=128, K=256, ldx=256, ldy=128, ldr=0, alpha=PTR, dtype=0, workspace=None,
              workspace_bytes=0)
     a.update(kw)
     return gplk.lib().gplk_gemv_nvfp4(*a.values(), None)
@@ -20,7 +20,7 @@ def _gemv(gplk, **kw):
 @pytest.mark.parametrize("kw", [
     dict(T=-1), dict(T=33), dict(N=-1), dict(K=-64), dict(K=0), dict(K=32), dict(K=100), dict(dtype=2), dict(dtype=-1),
     dict(ldx=255), dict(ldy=127), dict(R=PTR, ldr=127), dict(X=None), dict(W=None), dict(SF=None), dict(Y=None),
-    dict(alpha=None), dict(W=PTR + 8), dict(SF=PTR + 4), dict(X=PTR + 1), dict(Y=PTR + 1), dict(R=PTR + 1, ldr=128),
+    dict(alpha=None), dict(W=PTR + 8), dict(SF=PTR + 4), dict(X=PTR + 1), dict(Y=PTR + 1), dict(X=PTR, Y=PTR), dict(R=PTR + 1, ldr=128),
     dict(alpha=PTR + 2), dict(workspace=PTR + 8)])
 def test_gemv_refuses(kw, gplk):
     assert _gemv(gplk, **kw) == BAD_ARG
