@@ -170,23 +170,26 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 constexpr int kPer = kMaxExperts / 32;
 
 struct RouteShared {
-    int ids[kMaxTokens * kMaxTop];
-    uint32_t chosen_mask[kPer];
-    int active[kMaxExperts];
-    int chunks[kMaxExperts];
+    alignas(16) int16_t slot[kMaxExperts][kMaxTokens];  // token's slot with an expert, or -1
+    uint32_t chosen[kPer];         // experts, as bits
+    int active[kMaxExperts];       // the chosen ones, ascending
+    uint32_t tokens[kMaxExperts];  // theirs, as bits
 };
+
+// What does not wait for the logits.
+template <int WARPS>
+__device__ __forceinline__ void route_prepare(const RouteParams& p, RouteShared& sh) {
+    uint4* slots = reinterpret_cast<uint4*>(&sh.slot[0][0]);
+    for (int i = (int)threadIdx.x; i < p.E * kMaxTokens / 8; i += 32 * WARPS) slots[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+    if (threadIdx.x < kPer) sh.chosen[threadIdx.x] = 0;
+    __syncthreads();
+}
 
 template <int PER, int WARPS>
 __device__ __forceinline__ void route_body(const RouteParams& p, RouteShared& sh) {
     static_assert(32 * WARPS >= kMaxExperts, "a thread per expert");
     const int warp = (int)warp_id_uniform();
     const int lane = (int)lane_id();
-    int* const ids = sh.ids;
-    int* const active = sh.active;
-    int* const chunks = sh.chunks;
-    uint32_t* const chosen_mask = sh.chosen_mask;
-    if (threadIdx.x < kPer) chosen_mask[threadIdx.x] = 0;
-    __syncthreads();
     if (warp < p.T) {
         const float* l = p.logits + (size_t)warp * p.E;
         float v[PER];
@@ -205,9 +208,8 @@ __device__ __forceinline__ void route_body(const RouteParams& p, RouteShared& sh
         for (int i = 0; i < PER; ++i) sum += lane + 32 * i < p.E ? expf(v[i] - best) : 0.0f;
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        uint32_t taken = 0;
-        float chosen = 0.0f, top_sum = 0.0f;
-        int chosen_id = 0;
+        uint32_t taken = 0, my_key = 0;
+        int my_expert = 0;  // lane j: the expert of rank j
         for (int j = 0; j < p.top; ++j) {
             uint32_t k = 0;
 #pragma unroll
@@ -220,68 +222,72 @@ __device__ __forceinline__ void route_body(const RouteParams& p, RouteShared& sh
                 if (!(taken >> i & 1) && key[i] == m && lane + 32 * i < p.E) e = (uint32_t)(lane + 32 * i);
             e = __reduce_min_sync(0xffffffffu, e);  // top <= E: one is left
             if ((int)(e & 31) == lane) taken |= 1u << (e >> 5);
-            const float pr = expf(key_value(m) - best) / sum;
-            top_sum += pr;
             if (lane == j) {
-                chosen = pr;
-                chosen_id = (int)e;
+                my_key = m;
+                my_expert = (int)e;
             }
         }
+        const float mine = lane < p.top ? expf(key_value(my_key) - best) / sum : 0.0f;
+        float top_sum = mine;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top_sum += __shfl_xor_sync(0xffffffffu, top_sum, o);
         if (lane < p.top) {
             const int slot = warp * p.top + lane;
-            p.ids[slot] = chosen_id;
-            p.weights[slot] = p.renormalise ? chosen / top_sum : chosen;
-            ids[slot] = chosen_id;
-            atomicOr(&chosen_mask[chosen_id >> 5], 1u << (chosen_id & 31));
+            sh.slot[my_expert][warp] = (int16_t)slot;
+            atomicOr(&sh.chosen[my_expert >> 5], 1u << (my_expert & 31));
+            p.ids[slot] = my_expert;
+            p.weights[slot] = p.renormalise ? mine / top_sum : mine;
         }
     }
     __syncthreads();
-    // The chosen experts in ascending order, and how many tokens each has.
     int n_active = 0, before = 0;
     {
         const int e = (int)threadIdx.x;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            const uint32_t m = chosen_mask[i];
+            const uint32_t m = sh.chosen[i];
             if (i < (e >> 5)) before += __popc(m);
             n_active += __popc(m);
         }
-        if (e < p.E && (chosen_mask[e >> 5] >> (e & 31) & 1))
-            active[before + __popc(chosen_mask[e >> 5] & ((1u << (e & 31)) - 1))] = e;
+        if (e < p.E && (sh.chosen[e >> 5] >> (e & 31) & 1))
+            sh.active[before + __popc(sh.chosen[e >> 5] & ((1u << (e & 31)) - 1))] = e;
     }
     __syncthreads();
-    auto slot_of = [&](int e) {  // this lane's token's slot with expert e
-        int slot = -1;
-        if (lane < p.T)
-            for (int j = 0; j < p.top; ++j)
-                if (ids[lane * p.top + j] == e) slot = lane * p.top + j;
-        return slot;
+    auto entry = [&](int at, int expert, int slot, bool mine, int place, int tokens) {
+        if (mine) p.route->list[at][place] = (int16_t)slot;
+        p.route->slot[at][lane] = (int16_t)(mine ? slot : -1);
+        if (lane == 0) p.route->head[at] = expert | tokens << 16;
     };
+    // Up to kMaxEntryTokens tokens, an expert is one entry.
+    const bool one = p.T <= kMaxEntryTokens;
     for (int a = warp; a < n_active; a += WARPS) {
-        const uint32_t m = __ballot_sync(0xffffffffu, slot_of(active[a]) >= 0);
-        if (lane == 0) chunks[a] = (__popc(m) + kMaxEntryTokens - 1) / kMaxEntryTokens;
-    }
-    __syncthreads();
-    for (int a = warp; a < n_active; a += WARPS) {
-        // Entries of the experts before this one.
-        int base = 0;
-        for (int b = lane; b < a; b += 32) base += chunks[b];
-        base = __reduce_add_sync(0xffffffffu, base);
-        const int slot = slot_of(active[a]);
+        const int e = sh.active[a], slot = sh.slot[e][lane];
         const uint32_t m = __ballot_sync(0xffffffffu, slot >= 0);
-        const int n = __popc(m), place = __popc(m & ((1u << lane) - 1));
-        for (int c = 0; c < chunks[a]; ++c) {
-            const int in_chunk = place - c * kMaxEntryTokens;
-            const bool mine = slot >= 0 && in_chunk >= 0 && in_chunk < kMaxEntryTokens;
-            if (mine) p.route->list[base + c][in_chunk] = (int16_t)slot;
-            p.route->slot[base + c][lane] = (int16_t)(mine ? slot : -1);
-            if (lane == 0) p.route->head[base + c] = active[a] | min(kMaxEntryTokens, n - c * kMaxEntryTokens) << 16;
-        }
+        if (one) entry(a, e, slot, slot >= 0, __popc(m & ((1u << lane) - 1)), __popc(m));
+        else if (lane == 0) sh.tokens[a] = m;
     }
-    if (warp == 0) {
-        int entries = 0;
-        for (int b = lane; b < n_active; b += 32) entries += chunks[b];
-        entries = __reduce_add_sync(0xffffffffu, entries);
+    int entries = n_active;
+    if (!one) {
+        __syncthreads();
+        auto chunks = [&](int a) { return (__popc(sh.tokens[a]) + kMaxEntryTokens - 1) / kMaxEntryTokens; };
+        auto entries_before = [&](int a) {
+            int n = 0;
+            for (int b = lane; b < a; b += 32) n += chunks(b);
+            return __reduce_add_sync(0xffffffffu, n);
+        };
+        for (int a = warp; a < n_active; a += WARPS) {
+            const int e = sh.active[a], slot = sh.slot[e][lane], base = entries_before(a);
+            const uint32_t m = sh.tokens[a];
+            const int n = __popc(m), place = __popc(m & ((1u << lane) - 1));
+            for (int c = 0; c * kMaxEntryTokens < n; ++c) {
+                const int at = place - c * kMaxEntryTokens;
+                entry(base + c, e, slot, slot >= 0 && at >= 0 && at < kMaxEntryTokens, at,
+                      min(kMaxEntryTokens, n - c * kMaxEntryTokens));
+            }
+        }
+        if (warp == WARPS - 1) entries = entries_before(n_active);
+    }
+    if (warp == WARPS - 1) {
         for (int b = entries + lane; b < kMaxExperts; b += 32) p.route->head[b] = 0;
         if (lane == 0) p.route->n_entries = entries;
     }
@@ -290,6 +296,7 @@ __device__ __forceinline__ void route_body(const RouteParams& p, RouteShared& sh
 template <int PER>
 __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParams p) {
     __shared__ RouteShared sh;
+    route_prepare<kMaxTokens>(p, sh);
     pdl_wait();
     pdl_launch_dependents();
     route_body<PER, kMaxTokens>(p, sh);
@@ -310,6 +317,7 @@ __global__ void __cluster_dims__(kFewBlocks, 1, 1) __launch_bounds__(32 * (kFewW
     __shared__ RouteShared sh;
     __shared__ float part[kFewWarps][NX];
     const int rank = (int)cluster_ctarank(), warp = (int)warp_id_uniform(), lane = (int)lane_id();
+    if (rank == 0) route_prepare<kFewWarps + 1>(p, sh);
     pdl_wait();
     pdl_launch_dependents();
     // 2^sub_log2 warps share out an expert's K, so that a block's experts take
