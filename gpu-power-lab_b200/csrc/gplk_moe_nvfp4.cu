@@ -23,10 +23,10 @@
 //             blocks write a sum per slot, and a last launch adds a token's.
 // No atomics order a sum; the maxima that atomics find do not depend on it.
 // Measured, us, against the bytes at 6547 GB/s: 1 token 64/8 2048x1024 20 (4.4),
-// 8 tokens 128/8 4096x768 68 (41), 16 tokens 16/2 4096x4096 85 (61), 32 tokens
-// 64/6 4096x2048 163 (132). Small layers are the launches' latencies, 15.5 us at
+// 8 tokens 128/8 4096x768 66 (41), 16 tokens 16/2 4096x4096 85 (61), 32 tokens
+// 64/6 4096x2048 161 (132). Small layers are the launches' latencies, 15 us at
 // least; large ones what resident blocks do not overlap: routing before the first
-// weight (some 10 us) and a last round of items that not all SMs have.
+// weight (some 8 us) and a last round of items that not all SMs have.
 #include "gplk_ptx.cuh"
 
 namespace gplk {
@@ -304,9 +304,10 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
 
 // Router product and routing of few experts and tokens in one launch: a cluster of
 // eight blocks shares out the experts and the first block routes. On the device
-// it takes as long as two launches do (layer of 8 experts, 1024 x 512: 16.2 us
-// with it, 16.1 with two; of 32, 2048 x 704: 24.1 and 24.4; but of 64, 2048 x
-// 1024: 22.1 and 20.8, so it stops at 65536 weights); the host saves one.
+// it takes as long as two launches do (when both were measured: layer of 8
+// experts, 1024 x 512, 16.2 us with it and 16.1 with two; of 32, 2048 x 704, 24.1
+// and 24.4; but of 64, 2048 x 1024, 22.1 and 20.8, so it stops at 65536 weights);
+// the host saves one.
 constexpr int kFewBlocks = 8;
 constexpr int kFewWarps = 16;
 constexpr int kFewPer = 4;  // at most 128 experts
@@ -735,24 +736,24 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* part, XT* y, 
 }
 
 // Whether gate and up run as resident blocks over `items`: from two for every SM.
-// Measured, us of the layer, a block per item / resident: 310 items (8 tokens,
-// 128/8, 4096x768) 85 / 71, 976 (32, 64/6, 4096x2048) 183 / 174, but 256 (8, 8/2,
-// 4096x4096) 51.6 / 52.1 and (32, 8/2, 4096x4096) 75 / 88, 64 (16, 8/2, 2048x1024)
-// 23.3 / 26.9.
+// Measured, us of the layer, a block per item / resident: 976 items (32 tokens,
+// 64/6, 4096x2048) 175 / 162, 310 (8, 128/8, 4096x768) 78 / 66, but 256 (8, 8/2,
+// 4096x4096) 50.0 / 50.8 and (32, 8/2, 4096x4096) 69 / 72, 200 (16, 64/6, 2048x512)
+// 35 / 37, 64 (16, 8/2, 2048x1024) 23.1 / 25.5; 168 (4, 64/8, 4096x768) 52 / 51.
 static bool use_gate_items(double items, int sm_count) { return items >= 2.0 * sm_count; }
 
 // Whether down runs as resident blocks with a sum per slot, or accumulates over the
 // experts, which splits K further but converts and multiplies for every token in
 // every stage: by the tiles an SM streams, the second's weighed by its tokens.
 // Measured, us of the layer, accumulating / resident: 1 token 8/2 4096x14336
-// 47 / 68, 64/8 2048x1024 20.4 / 21.6; 2 tokens 16/4 4096x2048 32.5 / 33.2; 4 tokens
-// 32/4 2048x704 23.2 / 22.6; 8 tokens 8/2 4096x4096 59 / 52; 16 tokens 8/2
-// 2048x1024 27.2 / 23.3; 32 tokens 8/2 4096x4096 132 / 75.
+// 47 / 68, 64/8 2048x1024 20.1 / 21.2; 2 tokens 16/4 4096x2048 31.6 / 32.5; 4 tokens
+// 32/4 2048x704 22.2 / 22.6, 8/1 1024x14336 42 / 58; 8 tokens 8/2 4096x4096 58 / 50;
+// 16 tokens 8/2 2048x1024 27.4 / 22.3; 32 tokens 8/2 4096x4096 131 / 69.
 static bool use_down_items(int T, double active, int tiles, int k_stages, int split, int sm_count) {
     const int pairs = (tiles + 1) / 2;
     const double resident = 2.0 * k_stages * ceil(active * pairs / sm_count);
     const double accumulated = ceil(active * k_stages / split) * ceil((double)tiles * split / sm_count);
-    return resident <= accumulated * (T < 4 ? 0.8 : 1.0 + T / 8.0);
+    return resident <= accumulated * (T <= 4 ? 0.8 : 1.0 + T / 8.0);
 }
 
 template <typename XT>

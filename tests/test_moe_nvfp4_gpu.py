@@ -242,6 +242,31 @@ def test_two_captured_graphs(gplk, cuda):
             layer.check(x, 2, True, y, ids, w)
 
 
+@pytest.mark.parametrize("t,e,top,d,f", [(8, 64, 8, 640, 1024), (3, 32, 4, 512, 320)])
+def test_replays_on_other_experts(t, e, top, d, f, gplk, cuda):
+    """A captured layer (resident blocks; clusters) replayed back to back on
+    inputs that choose other experts each time: the eager call's bits."""
+    import torch
+
+    gen = _gen(cuda, 12)
+    layer = Layer(e, d, f, torch.bfloat16, gen, cuda)
+    x = torch.zeros(t, d, dtype=torch.bfloat16, device=cuda)
+    xs = [torch.randn(t, d, device=cuda, generator=gen).to(torch.bfloat16) for _ in range(5)]
+    eager = [layer.run(gplk, v, top) for v in xs]
+    outs = [torch.empty_like(x) for _ in xs]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y, ids, w = layer.run(gplk, x, top)
+    for v, o in zip(xs, outs):  # nothing waits between the replays
+        x.copy_(v)
+        g.replay()
+        o.copy_(y)
+    torch.cuda.synchronize()
+    assert len({tuple(i.flatten().tolist()) for _, i, _ in eager}) == len(xs)
+    for (want, _, _), got in zip(eager, outs):
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
 def test_decoding_block(gplk, cuda):
     """The operators in a row as a decoding block has them: a projection that
     adds the residual stream, the mixture of experts on its output, a
