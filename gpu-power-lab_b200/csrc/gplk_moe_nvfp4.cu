@@ -53,6 +53,14 @@ static Layout layout(int T, int E, int top, int D, int F) {
     return l;
 }
 
+// Sizes the layer takes.
+static bool takes(int T, int E, int top, int D, int F) {
+    if (T < 0 || T > kMaxTokens || E < 1 || E > kMaxExperts || top < 1 || top > kMaxTop || top > E) return false;
+    if (D < 64 || D % 64 != 0 || F < 64 || F % 64 != 0) return false;
+    // Rows of the expert stacks are TMA coordinates; grids stay below 2^31.
+    return (long long)E * F <= INT_MAX / 8 && (long long)E * D <= INT_MAX / 8;
+}
+
 struct RouteParams {
     const void* x;
     const void* router;
@@ -877,10 +885,7 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
 
 extern "C" size_t gplk_moe_nvfp4_workspace_bytes(int T, int E, int top, int D, int F) {
     using namespace gplk;
-    if (T <= 0 || E <= 0 || top <= 0 || D <= 0 || F <= 0 || T > fewtok::kMaxTokens || E > fewtok::kMaxExperts ||
-        top > fewtok::kMaxTop || top > E)
-        return 0;
-    return moe::layout(T, E, top, D, F).total;
+    return T > 0 && moe::takes(T, E, top, D, F) ? moe::layout(T, E, top, D, F).total : 0;
 }
 
 extern "C" int gplk_moe_nvfp4(const gplk_moe_cfg* cfg, cudaStream_t stream) {
@@ -888,12 +893,8 @@ extern "C" int gplk_moe_nvfp4(const gplk_moe_cfg* cfg, cudaStream_t stream) {
     using namespace gplk::fewtok;
     if (!cfg) return GPLK_STATUS_BAD_ARG;
     const gplk_moe_cfg& c = *cfg;
-    if (c.T < 0 || c.T > kMaxTokens || c.E < 1 || c.E > kMaxExperts || c.top < 1 || c.top > kMaxTop || c.top > c.E)
-        return GPLK_STATUS_BAD_ARG;
+    if (!moe::takes(c.T, c.E, c.top, c.D, c.F)) return GPLK_STATUS_BAD_ARG;
     if (c.dtype != GPLK_DTYPE_BF16 && c.dtype != GPLK_DTYPE_F16) return GPLK_STATUS_BAD_ARG;
-    if (c.D < 64 || c.D % 64 != 0 || c.F < 64 || c.F % 64 != 0) return GPLK_STATUS_BAD_ARG;
-    // Rows of the expert stacks are TMA coordinates; grids stay below 2^31.
-    if ((long long)c.E * c.F > INT_MAX / 8 || (long long)c.E * c.D > INT_MAX / 8) return GPLK_STATUS_BAD_ARG;
     if (c.T == 0) return GPLK_STATUS_OK;
     if (c.ldx < c.D || c.ldy < c.D) return GPLK_STATUS_BAD_ARG;
     if (!c.x || !c.router || !c.gate || !c.up || !c.down || !c.sf_gate || !c.sf_up || !c.sf_down || !c.alpha_gate ||

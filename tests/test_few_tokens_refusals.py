@@ -74,6 +74,15 @@ def test_moe_workspace_bytes(gplk):
     assert ws(32, 64, 8, 4096, 2048) >= 32 * 8 * 2048 * 4
 
 
+@pytest.mark.parametrize("sizes", [
+    (2, 8, 2, 100, 128), (2, 8, 2, 128, 100), (2, 8, 2, 32, 64), (2, 8, 2, 64, 32), (2, 512, 2, 1 << 20, 64),
+    (2, 512, 2, 64, 1 << 20), (-1, 8, 2, 64, 64), (2, 8, 17, 64, 64)])
+def test_moe_workspace_is_zero_where_the_call_refuses(sizes, gplk):
+    T, E, top, D, F = sizes
+    assert _moe(gplk, T=T, E=E, top=top, D=D, F=F, ldx=D, ldy=D, workspace_bytes=1 << 60) == BAD_ARG
+    assert gplk.moe_nvfp4_workspace_bytes(*sizes) == 0
+
+
 def test_python_wrappers_refuse_cpu_tensors(gplk):
     import torch
 
