@@ -704,14 +704,12 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     }
 }
 
-// Shared memory and TMEM of such a block: all of an SM's.
 static size_t set_item_shape(Params& p, int entry_tokens) {
-    const size_t overhead = 1024 + ((sizeof(ItemControl) + 127) & ~(size_t)127);
-    p.ring_bytes = (uint32_t)((227 * 1024 - overhead) & ~(size_t)1023);
-    p.tmem_cols = 512;
     for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
-    p.geo[0] = geometry(entry_tokens, 2, Fill::Convert, p.ring_bytes, p.tmem_cols, 2);
-    return p.ring_bytes + overhead;
+    const Shape s = item_shape(p.geo, entry_tokens, sizeof(ItemControl));
+    p.ring_bytes = s.ring_bytes;
+    p.tmem_cols = s.tmem_cols;
+    return s.smem;
 }
 
 template <bool GATE_UP, typename XT>
