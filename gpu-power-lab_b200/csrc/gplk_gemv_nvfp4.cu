@@ -59,12 +59,14 @@ __global__ void __launch_bounds__(1024)
     __syncthreads();
     m = __reduce_max_sync(0xffffffffu, (int)lane < warps ? top[lane] : 0u);
     if (threadIdx.x == 0) amax[t] = m;
-    const int anchor = anchor_of(m);
+    constexpr int kPlanes = kPlanesOf<XT>;
+    const int anchor = anchor_of<kPlanes>(m);
     auto emit = [&](int i, const uint4 (&r)[2]) {
         float v[8];
         widen<XT>(r, v);
         uint8_t* b_rows = image + (size_t)i * g.image;
-        convert(v, anchor, t, i * kStageK + (int)lane * 8 < K, b_rows, b_rows + (size_t)g.nb * 128, g.sfb_step, lane);
+        const bool inside = i * kStageK + (int)lane * 8 < K;
+        convert<kPlanes>(v, anchor, t, inside, b_rows, b_rows + (size_t)g.nb * 128, g.sfb_step, lane);
     };
 #pragma unroll
     for (int c = 0; c < kHeld; ++c)
@@ -79,14 +81,14 @@ __global__ void __launch_bounds__(1024)
 constexpr int kSms = 148;
 
 // Sizes and slices of a product of T tokens.
-static void plan(Params& p, int T, int N, int K) {
+static void plan(Params& p, int planes, int T, int N, int K) {
     p.T = T;
     p.N = N;
     p.K = K;
     p.tiles = (N + kTileRows - 1) / kTileRows;
     p.k_stages = (K + kStageK - 1) / kStageK;
     p.kblocks = K / 64;
-    const int per_sm = kPlanes * T > 128 ? 1 : 2;
+    const int per_sm = planes * T > 128 ? 1 : 2;
     p.split_log2 = choose_split_log2(p.tiles, p.k_stages, kSms, per_sm);
 }
 static int block_stages(const Params& p) { return ((p.k_stages - 1) >> p.split_log2) + 1; }
@@ -100,8 +102,10 @@ static int block_stages(const Params& p) { return ((p.k_stages - 1) >> p.split_l
 static bool use_image(const Params& p) { return p.T >= 4 && p.T * block_stages(p) >= 24; }
 
 // Workspace of the converted activations: the stages' images, then the
-// tokens' largest magnitudes.
-static size_t image_bytes(int T, int k_stages) { return (size_t)k_stages * geometry(T, 1, Fill::Image, 0, 0).image; }
+// tokens' largest magnitudes. One size for both types.
+static size_t image_bytes(int T, int k_stages) {
+    return (size_t)k_stages * geometry(kMaxPlanes, T, 1, Fill::Image, 0, 0).image;
+}
 
 template <typename XT>
 static int launch_gemv(Params& p, const Shape& s, const CUtensorMap& tm, void* workspace, cudaStream_t stream) {
@@ -127,8 +131,12 @@ extern "C" size_t gplk_gemv_nvfp4_workspace_bytes(int T, int N, int K) {
         return 0;
     Params p;
     memset(&p, 0, sizeof(p));
-    plan(p, T, N, K);
-    if (!use_image(p)) return 0;
+    bool any = false;
+    for (int planes : {kPlanesBF16, kPlanesF16}) {
+        plan(p, planes, T, N, K);
+        any = any || use_image(p);
+    }
+    if (!any) return 0;
     return image_bytes(T, (K + kStageK - 1) / kStageK) + sizeof(uint32_t) * kMaxTokens;
 }
 
@@ -160,10 +168,11 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     p.ldy = ldy;
     p.ldr = ldr;
     p.x_vec = aligned16(X) && (T == 1 || ldx % 8 == 0);
-    plan(p, T, N, K);
+    const int planes = dtype == GPLK_DTYPE_BF16 ? kPlanesBF16 : kPlanesF16;
+    plan(p, planes, T, N, K);
     const size_t need = use_image(p) ? image_bytes(T, p.k_stages) + sizeof(uint32_t) * kMaxTokens : 0;
     void* ws = need > 0 && workspace_bytes >= need ? workspace : nullptr;
-    const Shape s = set_shape(p, T, false, 1, ws ? Fill::Image : Fill::Convert, block_stages(p));
+    const Shape s = set_shape(p, planes, T, false, 1, ws ? Fill::Image : Fill::Convert, block_stages(p));
     if (s.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
     CUtensorMap tm;
     st = encode_weights(&tm, W, (uint64_t)N, K);

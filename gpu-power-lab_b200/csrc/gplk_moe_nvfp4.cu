@@ -382,10 +382,12 @@ struct ItemControl {
     int abort;
 };
 
-template <bool GATE_UP, typename XT>
+template <bool GATE_UP, typename T>
 __global__ void __launch_bounds__(kItemThreads, 1)
     item_kernel(const __grid_constant__ CUtensorMap tm0, const __grid_constant__ CUtensorMap tm1,
                 const __grid_constant__ Params p) {
+    using XT = std::conditional_t<GATE_UP, T, float>;
+    constexpr int kPlanes = kPlanesOf<T>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     ItemControl& sm = *reinterpret_cast<ItemControl*>(ring + p.ring_bytes);
@@ -578,7 +580,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
             const int row = GATE_UP ? slot / p.top : slot;
             const int k = u.kb * kStageK + (int)lane * 8;
             if (k < p.K) load_raw(static_cast<const XT*>(p.X) + (size_t)row * p.ldx + k, p.x_vec != 0, r);
-            anchor = anchor_of(p.amax[slot / p.top]);
+            anchor = anchor_of<kPlanes>(p.amax[slot / p.top]);
         };
         Unit cur;
         cur.it = (int)blockIdx.x;
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                         next_unit(cur);
                         if (ahead.it < items) next_unit(ahead);
                         load(ahead, r1, a1);
-                        convert(v, anchor, t, inside, b_rows, sfb, g.sfb_step, lane);
+                        convert<kPlanes>(v, anchor, t, inside, b_rows, sfb, g.sfb_step, lane);
                     } while (cur.it == it && cur.kb == kb);
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -651,27 +653,29 @@ __global__ void __launch_bounds__(kItemThreads, 1)
             __syncwarp();
             tc_fence_after();
             const uint32_t acc0 = tmem + ((quarter * 32u) << 16) + (uint32_t)(2 * acc.slot) * g.acc_cols;
-            for (int t0 = 0; t0 < ntok; t0 += 4) {  // 20 columns of each tile
-                uint32_t c0[3][8], c1[3][8];
+            // Four tokens' columns of both tiles fit a thread's registers up to six planes.
+            constexpr int kAtOnce = kPlanes < 7 ? 4 : 2, kLoads = (kPlanes * kAtOnce + 7) / 8;
+            for (int t0 = 0; t0 < ntok; t0 += kAtOnce) {
+                uint32_t c0[kLoads][8], c1[kLoads][8];
 #pragma unroll
-                for (int i = 0; i < 3; ++i) {
+                for (int i = 0; i < kLoads; ++i) {
                     tmem_ld_32x32b_x8(acc0 + (uint32_t)(kPlanes * t0 + 8 * i), c0[i]);
                     tmem_ld_32x32b_x8(acc0 + g.acc_cols + (uint32_t)(kPlanes * t0 + 8 * i), c1[i]);
                 }
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < kAtOnce; ++i) {
                     if (t0 + i >= ntok) continue;
-                    float s = __uint_as_float(c0[(5 * i + 4) >> 3][(5 * i + 4) & 7]);
-                    float u = __uint_as_float(c1[(5 * i + 4) >> 3][(5 * i + 4) & 7]);
+                    auto col = [&](const uint32_t (&c)[kLoads][8], int n) { return __uint_as_float(c[n >> 3][n & 7]); };
+                    float s = col(c0, kPlanes * i + kPlanes - 1), u = col(c1, kPlanes * i + kPlanes - 1);
 #pragma unroll
-                    for (int q = 3; q >= 0; --q) {
-                        s = __fmaf_rn(s, 0.125f, __uint_as_float(c0[(5 * i + q) >> 3][(5 * i + q) & 7]));
-                        u = __fmaf_rn(u, 0.125f, __uint_as_float(c1[(5 * i + q) >> 3][(5 * i + q) & 7]));
+                    for (int q = kPlanes - 2; q >= 0; --q) {
+                        s = __fmaf_rn(s, 0.125f, col(c0, kPlanes * i + q));
+                        u = __fmaf_rn(u, 0.125f, col(c1, kPlanes * i + q));
                     }
                     const uint32_t mb = __shfl_sync(0xffffffffu, my_max, t0 + i);
                     const int slot = __shfl_sync(0xffffffffu, my_slot, t0 + i);
-                    const float unit = __uint_as_float((uint32_t)(anchor_of(mb) - 8 + 127) << 23);
+                    const float unit = __uint_as_float((uint32_t)(anchor_of<kPlanes>(mb) - 8 + 127) << 23);
                     s = s * ag * unit;
                     u = u * au * unit;
                     if (mb >= kInfBits) s = u = __uint_as_float(0x7FC00000u);
@@ -704,19 +708,19 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     }
 }
 
-static size_t set_item_shape(Params& p, int entry_tokens) {
+static size_t set_item_shape(Params& p, int planes, int entry_tokens) {
     for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
-    const Shape s = item_shape(p.geo, entry_tokens, sizeof(ItemControl));
+    const Shape s = item_shape(p.geo, planes, entry_tokens, sizeof(ItemControl));
     p.ring_bytes = s.ring_bytes;
     p.tmem_cols = s.tmem_cols;
     return s.smem;
 }
 
-template <bool GATE_UP, typename XT>
+template <bool GATE_UP, typename T>
 static int launch_items(const CUtensorMap& tm0, const CUtensorMap& tm1, const Params& p, size_t smem, int blocks,
                         cudaStream_t stream) {
     static thread_local uint64_t configured = 0;  // bit per device
-    return launch_clusters(item_kernel<GATE_UP, XT>, &configured, blocks, kItemThreads, 1, smem, stream, tm0, tm1, p);
+    return launch_clusters(item_kernel<GATE_UP, T>, &configured, blocks, kItemThreads, 1, smem, stream, tm0, tm1, p);
 }
 
 // y[t] = the sum of a token's slots, in the order of their ranks.
@@ -831,16 +835,16 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     size_t g_smem, o_smem;
     const bool g_items = use_gate_items(active * g.tiles, d.sm_count);
     if (g_items) {
-        g_smem = set_item_shape(g, entry_tokens);
+        g_smem = set_item_shape(g, kPlanesOf<XT>, entry_tokens);
     } else {
-        const Shape s = set_shape(g, entry_tokens, true, 2, Fill::Convert, g.k_stages);
+        const Shape s = set_shape(g, kPlanesOf<XT>, entry_tokens, true, 2, Fill::Convert, g.k_stages);
         g_smem = s.smem;
         g.split_log2 = choose_split_log2(g.tiles * active, 2.0 * g.k_stages, d.sm_count, s.per_sm);
     }
-    const Shape os = set_shape(o, c.T, false, 1, Fill::Convert, o.k_stages * max_entries);
+    const Shape os = set_shape(o, kPlanesOf<XT>, c.T, false, 1, Fill::Convert, o.k_stages * max_entries);
     o.split_log2 = choose_split_log2(o.tiles, o.k_stages * active, d.sm_count, os.per_sm);
     const bool o_items = use_down_items(c.T, active, o.tiles, o.k_stages, 1 << o.split_log2, d.sm_count);
-    o_smem = o_items ? set_item_shape(o, entry_tokens) : os.smem;
+    o_smem = o_items ? set_item_shape(o, kPlanesOf<XT>, entry_tokens) : os.smem;
     o.Y = o_items ? static_cast<void*>(ws + l.part) : c.y;
     o.ldy = o_items ? c.D : c.ldy;
     if (g_smem > (size_t)d.max_smem_optin || o_smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
@@ -872,7 +876,7 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
                      : launch_stream<Mode::GateUp, XT, float>(tg, tu, g, g_smem, max_entries * g.tiles, stream);
     if (st != GPLK_STATUS_OK) return st;
     if (!o_items) return launch_stream<Mode::Down, float, XT>(td, td, o, o_smem, o.tiles, stream);
-    st = launch_items<false, float>(td, td, o, o_smem, d.sm_count, stream);
+    st = launch_items<false, XT>(td, td, o, o_smem, d.sm_count, stream);
     if (st != GPLK_STATUS_OK) return st;
     return launch_status(launch_pdl(combine_kernel<XT>, dim3((c.D + 1023) / 1024, c.T), dim3(256), 0, stream,
                                     static_cast<const float*>(o.Y), static_cast<XT*>(c.y), c.top, c.D, c.ldy));

@@ -11,7 +11,7 @@ namespace fewtok {
 
 constexpr int kMaxTokens = 32;
 constexpr int kMaxEntryTokens = 12;             // tokens of one expert that a block takes
-constexpr int kPlanes = 5;
+constexpr int kMaxPlanes = 7;                   // digit planes of an activation, see gplk_nvfp4_stream.cu
 constexpr int kTileRows = 128;
 constexpr int kStageK = 256;                    // elements of K per slot
 constexpr uint32_t kWBytes = kTileRows * 128;   // codes of a weights' slot
@@ -24,7 +24,7 @@ constexpr int kMaxSlots = 10;
 // weights' scale columns per slot, the activations'. Worked out by the host: a
 // division takes the device as long as a stage's MMA.
 struct Geometry {
-    int nb;              // accumulator columns, 5 per token padded to 8
+    int nb;              // accumulator columns, one per token and plane, padded to 8
     int w_slots, b_slots;
     uint32_t sfb_step;   // bytes from one 64-element block of B scales to the next
     uint32_t image;      // bytes of B rows and scales
@@ -53,10 +53,10 @@ static uint32_t columns_of(const Geometry& g, int accs) {
 
 enum class Fill { Convert, Image };
 
-static Geometry geometry(int ntok, int tiles, Fill fill, uint32_t ring_bytes, uint32_t tmem_cols, int accs = 1,
-                         int most_slots = kMaxSlots) {
+static Geometry geometry(int planes, int ntok, int tiles, Fill fill, uint32_t ring_bytes, uint32_t tmem_cols,
+                         int accs = 1, int most_slots = kMaxSlots) {
     Geometry g;
-    g.nb = (kPlanes * ntok + 7) & ~7;
+    g.nb = (planes * ntok + 7) & ~7;
     const bool wide = g.nb > 128;  // a second 128 rows of B scales
     // Four blocks of B scales, one per 64 elements of K: 32 lanes of 16 bytes, the
     // scales of rows r, r + 32, r + 64 and r + 96 (and four more for a second 128
@@ -103,7 +103,8 @@ static size_t overhead_of(size_t control) { return 1024 + ((control + 127) & ~(s
 // 2 tiles and of at most `stages` stages, with `control` bytes behind its rings:
 // half of an SM, or all of it where half holds fewer than three tiles' slots, with no
 // more slots than the stages want.
-static Shape block_shape(Geometry* geo, int tokens, bool each, int tiles, Fill fill, int stages, size_t control) {
+static Shape block_shape(Geometry* geo, int planes, int tokens, bool each, int tiles, Fill fill, int stages,
+                         size_t control) {
     const size_t overhead = overhead_of(control);
     const int want = stages < kMaxSlots ? (stages * tiles < kMaxSlots ? stages * tiles : kMaxSlots) : kMaxSlots;
     Shape s;
@@ -112,7 +113,8 @@ static Shape block_shape(Geometry* geo, int tokens, bool each, int tiles, Fill f
         ring = cols = 0;
         bool enough = true;
         for (int t = each ? 1 : tokens; t <= tokens; ++t) {
-            const Geometry g = geometry(t, tiles, fill, (uint32_t)(share_of_smem(most) - overhead), most, 1, want);
+            const Geometry g =
+                geometry(planes, t, tiles, fill, (uint32_t)(share_of_smem(most) - overhead), most, 1, want);
             enough = enough && columns_of(g, tiles) <= most && g.w_slots >= (want < 3 ? want : 3);
             ring = ring_of(g) > ring ? ring_of(g) : ring;
             cols = columns_of(g, tiles) > cols ? columns_of(g, tiles) : cols;
@@ -132,13 +134,13 @@ static Shape block_shape(Geometry* geo, int tokens, bool each, int tiles, Fill f
 
 // A resident block of the experts' products, for entries of up to `tokens` tokens: two
 // tiles, two sets of accumulators, all of an SM.
-static Shape item_shape(Geometry* geo, int tokens, size_t control) {
+static Shape item_shape(Geometry* geo, int planes, int tokens, size_t control) {
     Shape s;
     s.ring_bytes = (uint32_t)((share_of_smem(512) - overhead_of(control)) & ~(size_t)1023);
     s.tmem_cols = 512;
     s.smem = share_of_smem(512);
     s.per_sm = 1;
-    geo[0] = geometry(tokens, 2, Fill::Convert, s.ring_bytes, s.tmem_cols, 2);
+    geo[0] = geometry(planes, tokens, 2, Fill::Convert, s.ring_bytes, s.tmem_cols, 2);
     return s;
 }
 

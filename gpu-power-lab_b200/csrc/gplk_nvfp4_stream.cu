@@ -10,21 +10,26 @@
 // 0.56 TB/s at one token, 16384 x 8192). So the weights are not decoded at all:
 // they go from HBM through TMA to the block-scaled tensor-core MMA
 // (kind::mxf4nvf4), codes and scales as they lie, and the activations are
-// brought to its operand format instead, exactly enough to count as 16-bit:
+// brought to its operand format instead:
 //
 //   Within a 16-group of a token, 2^b the power of two at or below its largest
-//   magnitude, x is rounded to a multiple of 2^b / 8192 and written in
-//   balanced base-8 digits  x = 2^b * sum_p d_p / 2 * 8^-p,  p = 0..4,
+//   magnitude, x is rounded to a multiple of 2^b * 2^-(3 P - 2) and written in P
+//   balanced base-8 digits  x = 2^b * sum_p d_p / 2 * 8^-p,  p = 0..P - 1,
 //   d_0 in -4..4, the others in -4..3. Every d / 2 is an E2M1 value, so digit p
 //   of all of k is one E2M1 row ("plane") of the MMA's B operand, and 2^b,
 //   relative to the token's largest magnitude 2^A, is the group's UE4M3 scale.
-//   Five planes keep 15 bits: an activation is off by at most 2^-14 of its
-//   group's largest magnitude (2^-28 of the token's, in groups 2^14 below
-//   it), where BF16 itself is off by 2^-9 of each value. The accumulator
-//   column of each (token, plane) is exact products in FP32 sums; the epilogue
-//   adds 8^-p times the planes' columns.
+//   P is 6 for BF16 and 7 for FP16: with either, a value down to 2^-9 of its
+//   group's 2^b keeps all of its bits (8 and 11), and a smaller one is off by at
+//   most 2^-17 and 2^-20 of 2^b, half a step. (In groups 2^14 and more below the
+//   token's largest magnitude: 2^-31 and 2^-34 of that.) An MoE layer's h, FP32,
+//   is taken to the planes of the layer's type. With one plane less, values next
+//   to an outlier lose bits that their type has; it takes as long for a few
+//   tokens, and for many of them 32x16384x16384 38.7 instead of 40.2 us, a layer
+//   of 32 tokens 8/2 4096x4096 70 instead of 80. The accumulator column of each
+//   (token, plane) is exact products in FP32 sums; the epilogue adds 8^-p times
+//   the planes' columns.
 //
-// So T tokens are an MMA of N = 5 T columns (padded to 8), at most 160 of the
+// So T tokens are an MMA of N = P T columns (padded to 8), at most 224 of the
 // 256 an instruction takes.
 //
 // Layout of the work. A block owns 128 weight rows (the MMA's M), or two such
@@ -46,7 +51,7 @@
 // addresses and descriptors in uniform registers, 65536 x 8192 at one token
 // takes 51 us; issued from a lane of a diverged warp 76 us. At one token that is
 // 5.9 TB/s, with 4.5 us of start and end in smaller calls; at 32 tokens what counts
-// is the weights on their way (16384 x 16384: 42 us; 37 without any MMA, scale
+// is the weights on their way (16384 x 16384: 40 us; 37 without any MMA, scale
 // copy or activation), since activations take half of the shared memory.
 // Every mbarrier wait is bounded, as everywhere in this library.
 #include <cuda_bf16.h>
@@ -66,12 +71,16 @@ namespace fewtok {
 constexpr int kMaxExperts = 512;
 constexpr int kMaxTop = 16;
 constexpr int kConvWarps = 8;
-constexpr uint32_t kDigitBias = 4u * (1u + 8u + 64u + 512u + 4096u);
+constexpr int kPlanesBF16 = 6, kPlanesF16 = 7;
 
 // Gemv: all tokens against one matrix. GateUp: tokens of a chosen expert against
 // its gate and up matrices. Down: all tokens against every chosen expert's down
 // matrix, accumulated over the experts.
 enum class Mode { Gemv, GateUp, Down };
+
+// Planes of the activations in a product of type T.
+template <typename T>
+constexpr int kPlanesOf = std::is_same<T, __half>::value ? kPlanesF16 : kPlanesBF16;
 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
@@ -243,9 +252,13 @@ __device__ __forceinline__ uint32_t max_bits(const float (&v)[8]) {
 
 constexpr uint32_t kInfBits = 0x7F800000u;
 
-// Exponent A of a token's largest magnitude. Below 2^-100 the anchor stays
-// there: what is then lost is below 2^-127, FP32's own subnormal range.
-__device__ __forceinline__ int anchor_of(uint32_t amax_bits) { return max((int)(amax_bits >> 23) - 127, -100); }
+// Exponent A of a token's largest magnitude. The anchor stays where a group 2^14
+// below it is still a multiple of 2^-127: what is lost there is at most 2^-128,
+// in FP32's own subnormal range.
+template <int PLANES>
+__device__ __forceinline__ int anchor_of(uint32_t amax_bits) {
+    return max((int)(amax_bits >> 23) - 127, 3 * PLANES - 115);
+}
 
 // Eight nibbles of biased digits (0..7 for -4..3; 8 for the top digit's 4) to
 // E2M1 codes of d / 2: magnitude |d| in the low three bits, sign above.
@@ -265,34 +278,44 @@ __device__ __forceinline__ uint32_t sfb_offset(uint32_t r, uint32_t lane, uint32
     return (r >> 7) * 2048 + (lane >> 3) * step + (r & 31) * 16 + ((r & 127) >> 5) * 4 + ((lane >> 1) & 3);
 }
 
-// One token's 256 elements of a stage, eight per lane: planes 5 t .. 5 t + 4
+// One token's 256 elements of a stage, eight per lane: planes PLANES t and on
 // of the stage's B rows (128-byte swizzled, K-major) and the 16 groups'
 // scales. `on` is false for lanes beyond K, whose blocks no MMA reads.
+template <int PLANES>
 __device__ __forceinline__ void convert(const float (&v)[8], int anchor, int t, bool on, uint8_t* b_rows,
                                         uint8_t* sfb, uint32_t sfb_step, uint32_t lane) {
+    static_assert(PLANES >= 5 && PLANES <= kMaxPlanes, "digits in 22 bits of a word");
     uint32_t m = max_bits(v);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));  // the other half of the 16-group
     const int b = max((int)(m >> 23) - 127, anchor - 14);
-    const float scale = __uint_as_float((uint32_t)(13 - b + 127) << 23);
-    // x * scale is at most 2^14 in magnitude; adding 1.5 * 2^23 rounds it to an
-    // integer, and the bias makes every digit non-negative.
+    const float scale = __uint_as_float((uint32_t)(3 * PLANES - 2 - b + 127) << 23);
+    // x * scale is at most 2^(3 PLANES - 1) in magnitude; adding 1.5 * 2^23 rounds
+    // it to an integer, and the bias, a 4 in every digit, makes all of them
+    // non-negative.
+    constexpr uint32_t kDigitBias = 4u * (((1u << 3 * PLANES) - 1) / 7);
     constexpr float kMagic = 12582912.0f + (float)kDigitBias;
     uint32_t u[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__fmaf_rn(v[i], scale, kMagic));
-    uint32_t q[4];  // elements i and i + 4: nibbles i and i + 4 of a word are 16 bits apart
+    // Elements i and i + 4 (nibbles i and i + 4 of a word are 16 bits apart): bits 0
+    // to 15, and 8 to 23 for the digits above.
+    uint32_t low[4], high[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = __byte_perm(u[i], u[i + 4], 0x5410);
+    for (int i = 0; i < 4; ++i) {
+        low[i] = __byte_perm(u[i], u[i + 4], 0x5410);
+        high[i] = __byte_perm(u[i], u[i + 4], 0x6521);
+    }
     if (!on) return;
 #pragma unroll
-    for (int p = 0; p < kPlanes; ++p) {
-        const int sh = 3 * (kPlanes - 1 - p);
+    for (int p = 0; p < PLANES; ++p) {
+        const int sh = 3 * (PLANES - 1 - p);
+        const bool upper = sh + (p == 0 ? 4 : 3) > 16;
         const uint32_t mask = p == 0 ? 0x000F000Fu : 0x00070007u;
         uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= ((q[i] >> sh) & mask) << (4 * i);
+        for (int i = 0; i < 4; ++i) w |= ((upper ? high[i] >> (sh - 8) : low[i] >> sh) & mask) << (4 * i);
         w = p == 0 ? digit_codes<true>(w) : digit_codes<false>(w);
-        const uint32_t r = (uint32_t)(kPlanes * t + p);
+        const uint32_t r = (uint32_t)(PLANES * t + p);
         *reinterpret_cast<uint32_t*>(b_rows + (r >> 3) * 1024 + (r & 7) * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
                                      (lane & 3) * 4) = w;
         if ((lane & 1) == (uint32_t)(p & 1))
@@ -301,11 +324,12 @@ __device__ __forceinline__ void convert(const float (&v)[8], int anchor, int t, 
 }
 
 // A token without a part in the stage's expert: zero digits, scale 1.
+template <int PLANES>
 __device__ __forceinline__ void convert_zero(int t, uint8_t* b_rows, uint8_t* sfb, uint32_t sfb_step,
                                              uint32_t lane) {
 #pragma unroll
-    for (int p = 0; p < kPlanes; ++p) {
-        const uint32_t r = (uint32_t)(kPlanes * t + p);
+    for (int p = 0; p < PLANES; ++p) {
+        const uint32_t r = (uint32_t)(PLANES * t + p);
         *reinterpret_cast<uint32_t*>(b_rows + (r >> 3) * 1024 + (r & 7) * 128 + lane * 4) = 0u;
         if ((lane & 1) == (uint32_t)(p & 1))
             sfb[sfb_offset(r, lane, sfb_step)] = 0x38;
@@ -328,6 +352,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     const int split = 1 << p.split_log2;
     const int cid = (int)(blockIdx.x >> p.split_log2);
     constexpr bool kPerExpert = M == Mode::GateUp;
+    constexpr int kPlanes = kPlanesOf<std::conditional_t<M == Mode::Down, YT, XT>>;
 
     // Barriers and TMEM. A slot is full when the copies have landed and the warps
     // with tokens in the stage have converted them (where the tokens are not
@@ -634,8 +659,8 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     float v[8];
                     widen<XT>(r[c], v);
                     uint8_t* b_rows = b_ring + (size_t)u.i * g.b_slot;
-                    convert(v, anchor_of(sm.amax[u.t]), u.t, in_k(u), b_rows, b_rows + (size_t)g.nb * 128, g.sfb_step,
-                            lane);
+                    convert<kPlanes>(v, anchor_of<kPlanes>(sm.amax[u.t]), u.t, in_k(u), b_rows,
+                                     b_rows + (size_t)g.nb * 128, g.sfb_step, lane);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -712,10 +737,11 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                         next_unit(ahead);
                         if (ahead.i < nst) on1 = load(ahead, r1);
                         if (M != Mode::Down || on) {
-                            convert(v, anchor_of(sm.amax[t]), t, inside, b_rows, sfb, g.sfb_step, lane);
+                            convert<kPlanes>(v, anchor_of<kPlanes>(sm.amax[t]), t, inside, b_rows, sfb, g.sfb_step,
+                                             lane);
                             if (M == Mode::Down && lane == 0) sm.dirty[b.slot][t] = 1;
                         } else if (sm.dirty[b.slot][t]) {
-                            convert_zero(t, b_rows, sfb, g.sfb_step, lane);
+                            convert_zero<kPlanes>(t, b_rows, sfb, g.sfb_step, lane);
                             __syncwarp();
                             if (lane == 0) sm.dirty[b.slot][t] = 0;
                         }
@@ -755,19 +781,21 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                                     : M == Mode::GateUp ? (h ? p.alpha1 : p.alpha0)[expert]
                                                         : 1.0f;
                 const uint32_t acc = tmem + ((quarter * 32u) << 16) + (uint32_t)h * g.acc_cols;
-                for (int t0 = 0; t0 < ntok; t0 += 8) {
+                constexpr int kAtOnce = 4;  // tokens
+                for (int t0 = 0; t0 < ntok; t0 += kAtOnce) {
                     if (nst == 0) {
-                        for (int t = t0; t < min(t0 + 8, ntok); ++t) part[t * kTileRows + row] = 0.0f;
+                        for (int t = t0; t < min(t0 + kAtOnce, ntok); ++t) part[t * kTileRows + row] = 0.0f;
                         continue;
                     }
-                    uint32_t c[5][8];
+                    constexpr int kLoads = (kPlanes * kAtOnce + 7) / 8;
+                    uint32_t c[kLoads][8];
 #pragma unroll
-                    for (int i = 0; i < 5; ++i) tmem_ld_32x32b_x8(acc + (uint32_t)(kPlanes * t0 + 8 * i), c[i]);
+                    for (int i = 0; i < kLoads; ++i) tmem_ld_32x32b_x8(acc + (uint32_t)(kPlanes * t0 + 8 * i), c[i]);
                     // With one slice the sums are final: no other block has a part.
                     const int n = tile * kTileRows + row;
-                    float r[8];
+                    float r[kAtOnce];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < kAtOnce; ++i) {
                         r[i] = 0.0f;
                         if constexpr (M == Mode::Gemv)
                             if (direct && p.R && t0 + i < ntok && n < p.N)
@@ -775,14 +803,14 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     }
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < kAtOnce; ++i) {
                         if (t0 + i >= ntok) continue;
                         auto col = [&](int n) { return __uint_as_float(c[n >> 3][n & 7]); };
-                        float s = col(5 * i + 4);
+                        float s = col(kPlanes * i + kPlanes - 1);
 #pragma unroll
-                        for (int q = 3; q >= 0; --q) s = __fmaf_rn(s, 0.125f, col(5 * i + q));
+                        for (int q = kPlanes - 2; q >= 0; --q) s = __fmaf_rn(s, 0.125f, col(kPlanes * i + q));
                         const uint32_t mb = sm.amax[t0 + i];
-                        s = s * alpha * __uint_as_float((uint32_t)(anchor_of(mb) - 8 + 127) << 23);
+                        s = s * alpha * __uint_as_float((uint32_t)(anchor_of<kPlanes>(mb) - 8 + 127) << 23);
                         if (mb >= kInfBits) s = __uint_as_float(0x7FC00000u);
                         if (!direct) part[(t0 + i) * kTileRows + row] = s;
                         else if (n < p.N) static_cast<YT*>(p.Y)[(size_t)(t0 + i) * p.ldy + n] = from_f32<YT>(s + r[i]);
@@ -869,9 +897,9 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
 static inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // The shape of a stream_kernel's blocks, see block_shape().
-static Shape set_shape(Params& p, int tokens, bool each, int tiles, Fill fill, int stages) {
+static Shape set_shape(Params& p, int planes, int tokens, bool each, int tiles, Fill fill, int stages) {
     for (int t = 1; t <= kMaxTokens; ++t) p.inverse[t] = 65536u / (uint32_t)t + 1;
-    const Shape s = block_shape(p.geo, tokens, each, tiles, fill, stages, sizeof(Control));
+    const Shape s = block_shape(p.geo, planes, tokens, each, tiles, fill, stages, sizeof(Control));
     p.ring_bytes = s.ring_bytes;
     p.tmem_cols = s.tmem_cols;
     return s;

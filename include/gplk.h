@@ -148,14 +148,15 @@ size_t gplk_nvfp4_sf_bytes(int rows, int k);
  * ldr >= N in elements. R may be NULL, and may be Y itself (Y is then
  * updated in place); X must not overlap Y. Sums are FP32; each output is
  * rounded once. alpha is a device pointer to the weights' per-tensor scale.
- * Activations enter the products as multiples of 2^b / 8192 within a group of
- * 16, 2^b being the power of two at or below the group's largest magnitude
- * (so off by at most 2^-14 of it; 2^-28 of the token's largest magnitude in
- * groups that lie more than 2^14 below that). A token with an infinity or a
- * NaN in X gets NaN in all of its outputs; other tokens are not affected.
- * Requires K % 64 == 0, N and K below 2^28 and 16-byte aligned W and SF; X, Y and R may have any
- * alignment and leading dimension (rows of X on 16-byte boundaries load
- * fastest). The result does not depend on other calls or on timing: equal
+ * Activations enter the products as multiples of 2^b / 2^16 (BF16) or
+ * 2^b / 2^19 (FP16) within a group of 16, 2^b being the power of two at or
+ * below the group's largest magnitude: a value down to 2^b / 2^9 enters with
+ * all of its bits, a smaller one is off by at most half such a step. (b is at
+ * least A - 14, 2^A being the token's largest magnitude taken the same way.) A
+ * token with an infinity or a NaN in X gets NaN in all of its outputs; other
+ * tokens are not affected. Requires K % 64 == 0, N and K below 2^28 and 16-byte
+ * aligned W and SF; X, Y and R may have any alignment and leading dimension
+ * (rows of X on 16-byte boundaries load fastest). The result does not depend on other calls or on timing: equal
  * inputs give equal bits. */
 int gplk_gemv_nvfp4(const void *X, const uint8_t *W, const uint8_t *SF, void *Y, const void *R, int T,
                     int N, int K, int ldx, int ldy, int ldr, const float *alpha, int dtype,
@@ -182,7 +183,7 @@ size_t gplk_gemv_nvfp4_workspace_bytes(int T, int N, int K);
  * FP32. Requires D % 64 == 0, F % 64 == 0, E <= 512, top <= min(E, 16),
  * E * F and E * D below 2^28; x, y and router in any alignment.
  * x must not overlap y. x and h enter the products as the activations of
- * gplk_gemv_nvfp4 do. A token with an infinity or a NaN in x gets NaN in y, and
+ * gplk_gemv_nvfp4 do, h by the type of x. A token with an infinity or a NaN in x gets NaN in y, and
  * experts that are in range and distinct but otherwise unspecified. The last
  * bits of a token's y may depend on which experts the other tokens choose
  * (sums are split accordingly); equal inputs give equal bits.

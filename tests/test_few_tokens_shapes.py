@@ -23,7 +23,7 @@ def shapes(tmp_path_factory):
     exe = tmp_path_factory.mktemp("shapes") / "shapes"
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wno-unused-function", f"-I{CSRC}", "-o", str(exe),
                     str(REPO / "tests/csrc/few_token_shapes.cpp")], check=True)
-    names = ("kind", "tokens", "tiles", "stages", "tmem", "smem", "per_sm", "ring", "w", "b", "cols", "ring_used",
+    names = ("kind", "planes", "tokens", "tiles", "stages", "tmem", "smem", "per_sm", "ring", "w", "b", "cols", "ring_used",
              "image", "nb")
     rows = [line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()]
     out = [dict(zip(names, [r[0], *map(int, r[1:])])) for r in rows]
