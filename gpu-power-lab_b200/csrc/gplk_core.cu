@@ -110,6 +110,22 @@ static int encode_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t row_by
     return r == CUDA_SUCCESS ? GPLK_STATUS_OK : GPLK_STATUS_BAD_ARG;
 }
 
+// 3-D byte tensor with the given sizes, strides of its outer two dimensions in bytes
+// and box (innermost first, box[0] <= 128), 128-byte swizzle.
+static int encode_tmap_3d_u8(CUtensorMap* map, const void* base, const uint64_t (&sizes)[3],
+                             const uint64_t (&pitches)[2], const uint32_t (&boxes)[3]) {
+    auto enc = tensor_map_encoder();
+    if (!enc) return GPLK_STATUS_UNSUPPORTED;
+    cuuint64_t dims[3] = {sizes[0], sizes[1], sizes[2]};
+    cuuint64_t strides[2] = {pitches[0], pitches[1]};
+    cuuint32_t box[3] = {boxes[0], boxes[1], boxes[2]};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? GPLK_STATUS_OK : GPLK_STATUS_BAD_ARG;
+}
+
 // 2-D 16-bit tensor, row length `inner` elements, `outer` rows, row pitch
 // `pitch_bytes`; box inner x outer, no swizzle (for TMA stores of BF16 tiles).
 static int encode_tmap_2d_u16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,

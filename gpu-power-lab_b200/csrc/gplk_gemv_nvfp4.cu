@@ -175,7 +175,7 @@ extern "C" int gplk_gemv_nvfp4(const void* X, const uint8_t* W, const uint8_t* S
     const Shape s = set_shape(p, planes, T, false, 1, ws ? Fill::Image : Fill::Convert, block_stages(p));
     if (s.smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
     CUtensorMap tm;
-    st = encode_weights(&tm, W, (uint64_t)N, K);
+    st = encode_weights(&tm, W, N, 1, K);
     if (st != GPLK_STATUS_OK) return st;
     return dtype == GPLK_DTYPE_BF16 ? launch_gemv<__nv_bfloat16>(p, s, tm, ws, stream)
                                     : launch_gemv<__half>(p, s, tm, ws, stream);

@@ -57,7 +57,7 @@ static Layout layout(int T, int E, int top, int D, int F) {
 static bool takes(int T, int E, int top, int D, int F) {
     if (T < 0 || T > kMaxTokens || E < 1 || E > kMaxExperts || top < 1 || top > kMaxTop || top > E) return false;
     if (D < 64 || D % 64 != 0 || F < 64 || F % 64 != 0) return false;
-    // Rows of the expert stacks are TMA coordinates; grids stay below 2^31.
+    // Rows of a stack, numbers of stages and grids stay below 2^31.
     return (long long)E * F <= INT_MAX / 8 && (long long)E * D <= INT_MAX / 8;
 }
 
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(kItemThreads, 1)
                             const uint8_t* sf = (up ? p.sf1 : p.sf0) + (size_t)expert * sf_matrix +
                                                 ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
                             mbar_arrive_expect_tx(full, kWBytes + sf_bytes);
-                            tma_load_2d(st, up ? &tm1 : &tm0, full, kb * 128, expert * p.N + tile * kTileRows);
+                            tma_load_3d(st, up ? &tm1 : &tm0, full, kb * 128, tile * kTileRows, expert);
                             bulk_load(st + kWBytes, sf, sf_bytes, full);
                         } else {
                             mbar_arrive(full);  // an odd last tile: its neighbour's slot stays as it is
@@ -850,9 +850,9 @@ static int launch(const gplk_moe_cfg& c, const DeviceInfo& d, cudaStream_t strea
     if (g_smem > (size_t)d.max_smem_optin || o_smem > (size_t)d.max_smem_optin) return GPLK_STATUS_UNSUPPORTED;
 
     CUtensorMap tg, tu, td;
-    int st = encode_weights(&tg, c.gate, (uint64_t)c.E * c.F, c.D);
-    if (st == GPLK_STATUS_OK) st = encode_weights(&tu, c.up, (uint64_t)c.E * c.F, c.D);
-    if (st == GPLK_STATUS_OK) st = encode_weights(&td, c.down, (uint64_t)c.E * c.D, c.F);
+    int st = encode_weights(&tg, c.gate, c.F, c.E, c.D);
+    if (st == GPLK_STATUS_OK) st = encode_weights(&tu, c.up, c.F, c.E, c.D);
+    if (st == GPLK_STATUS_OK) st = encode_weights(&td, c.down, c.D, c.E, c.F);
     if (st != GPLK_STATUS_OK) return st;
 
     auto router = [&](auto kernel, int nx) {

@@ -77,6 +77,19 @@ static Geometry geometry(int planes, int ntok, int tiles, Fill fill, uint32_t ri
     return g;
 }
 
+// Tensor map of a stack of weight matrices, `rows` rows of k / 2 bytes each: boxes of
+// 128 bytes of a tile's rows. The matrices are a dimension of their own, so that a box
+// over a matrix's last rows ends with it (zeros) instead of reading the next matrix,
+// which may be an expert that no token chose.
+struct WeightMap {
+    uint64_t sizes[3], pitches[2];
+    uint32_t box[3];
+};
+
+static WeightMap weight_map(uint64_t rows, uint64_t matrices, uint64_t k) {
+    return {{k / 2, rows, matrices}, {k / 2, rows * (k / 2)}, {128, (uint32_t)kTileRows, 1}};
+}
+
 // Shared memory and TMEM of a block.
 struct Shape {
     uint32_t ring_bytes;  // shared memory of the two rings

@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                                         ((size_t)tile * p.kblocks + (size_t)kb * 4) * 512;
                     uint64_t* full = &sm.full[c.slot];
                     mbar_arrive_expect_tx(full, kWBytes + sf_bytes);
-                    tma_load_2d(st, up ? &tm1 : &tm0, full, kb * 128, expert * p.N + tile * kTileRows);
+                    tma_load_3d(st, up ? &tm1 : &tm0, full, kb * 128, tile * kTileRows, expert);
                     bulk_load(st + kWBytes, sf, sf_bytes, full);
                     ++issued;
                     if constexpr (IMAGE) {
@@ -972,9 +972,10 @@ static int launch_stream(const CUtensorMap& tm0, const CUtensorMap& tm1, const P
                            1 << p.split_log2, smem, stream, tm0, tm1, p);
 }
 
-// Tensor map of `rows` weight rows of K / 2 bytes, boxes of 128 rows x 128 bytes.
-static int encode_weights(CUtensorMap* map, const uint8_t* W, uint64_t rows, int K) {
-    return encode_tmap_2d_u8(map, W, (uint64_t)K / 2, rows, (uint64_t)K / 2, 128, kTileRows);
+// Tensor map of `matrices` weight matrices of `rows` rows of K / 2 bytes.
+static int encode_weights(CUtensorMap* map, const uint8_t* W, int rows, int matrices, int K) {
+    const WeightMap m = weight_map((uint64_t)rows, (uint64_t)matrices, (uint64_t)K);
+    return encode_tmap_3d_u8(map, W, m.sizes, m.pitches, m.box);
 }
 
 }  // namespace fewtok

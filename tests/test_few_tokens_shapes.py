@@ -19,14 +19,18 @@ pytestmark = pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not ava
 
 
 @pytest.fixture(scope="module")
-def shapes(tmp_path_factory):
+def lines(tmp_path_factory):
     exe = tmp_path_factory.mktemp("shapes") / "shapes"
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wno-unused-function", f"-I{CSRC}", "-o", str(exe),
                     str(REPO / "tests/csrc/few_token_shapes.cpp")], check=True)
+    return [line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()]
+
+
+@pytest.fixture(scope="module")
+def shapes(lines):
     names = ("kind", "planes", "tokens", "tiles", "stages", "tmem", "smem", "per_sm", "ring", "w", "b", "cols", "ring_used",
              "image", "nb")
-    rows = [line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()]
-    out = [dict(zip(names, [r[0], *map(int, r[1:])])) for r in rows]
+    out = [dict(zip(names, [r[0], *map(int, r[1:])])) for r in lines if r[0] != "map"]
     assert {s["kind"] for s in out} == {"convert", "image", "gateup", "item"}
     return out
 
@@ -54,3 +58,12 @@ def test_rings_and_columns_fit(shapes):
         if s["tiles"] == 2:  # pairs: a stage's slot is free once both its tiles' slots are
             assert 2 * s["b"] >= s["w"], s
 
+
+def test_boxes_of_a_matrix_stay_in_it(lines):
+    """An expert's weights are read to their end and no other expert's are:
+    those may be on their way in or out of memory while a layer runs."""
+    maps = [tuple(map(int, r[1:])) for r in lines if r[0] == "map"]
+    assert len(maps) == 15
+    for rows, matrices, k, outside, covered in maps:
+        assert outside == 0, (rows, k, outside)
+        assert covered == matrices * rows * k // 2
