@@ -361,7 +361,8 @@ def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = Tr
     fn, L = "gplk_moe_nvfp4", _lib or lib()
     dt, u8, f32, dev = _act_dtype(X), torch.uint8, torch.float32, X.get_device()
     (gw, gs, ga), (uw, us, ua), (dw, ds, da) = gate, up, down
-    _need(fn, dt >= 0 and dev >= 0 and X.dim() == Y.dim() == router.dim() == ids.dim() == 2 and gw.dim() == 3)
+    _need(fn, workspace is not None and dt >= 0 and dev >= 0 and gw.dim() == 3
+          and X.dim() == Y.dim() == router.dim() == ids.dim() == 2)
     if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
             return moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise, workspace, stream)
