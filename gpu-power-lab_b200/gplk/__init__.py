@@ -70,7 +70,8 @@ class MoeCfg(ctypes.Structure):
     ]
 
 
-_moe_cfg = struct.Struct("@15PN9i4x").pack
+# The bytes of a MoeCfg from its values ("0P" pads the end as the compiler does).
+_moe_cfg = struct.Struct("@" + "".join({_p: "P", _sz: "N", _i: "i"}[t] for _, t in MoeCfg._fields_) + "0P").pack
 
 
 def lib() -> ctypes.CDLL:
