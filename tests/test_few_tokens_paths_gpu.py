@@ -7,7 +7,9 @@ from __future__ import annotations
 import pytest
 
 import nvfp4_reference as ref
+from test_gemv_nvfp4_gpu import _check as product
 from test_moe_nvfp4_gpu import Layer
+from test_moe_nvfp4_gpu import _case as layer_case
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +29,122 @@ def test_layer_without_a_workspace_is_refused(gplk, cuda):
     x = torch.zeros(2, 128, dtype=torch.bfloat16, device=cuda)
     with pytest.raises(gplk.GplkError):
         layer.run(gplk, x, 2, workspace=None)
+
+@pytest.mark.parametrize("t", [1, 2, 3, 4, 7, 12, 16, 18, 19, 24, 27, 32])
+def test_product_f16_tokens(t, gplk, cuda):
+    product(gplk, cuda, t, 300, 1088, dtype="f16", pad=1)
+
+
+@pytest.mark.parametrize("tnk", [(4, 700, 8192), (9, 500, 8192), (17, 1000, 4160), (25, 128, 16384), (32, 130, 16448)])
+@pytest.mark.parametrize("pad", [0, 1, 3, 8])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_product_converted_ahead(dtype, pad, tnk, gplk, cuda):
+    product(gplk, cuda, *tnk, dtype=dtype, pad=pad, residual="inplace")
+
+
+@pytest.mark.parametrize("tnk", [(1, 200, 512), (4, 300, 1088), (3, 200, 16384), (9, 500, 8192), (17, 1000, 4160),
+                                 (32, 130, 16448)])
+@pytest.mark.parametrize("bad", ["inf", "-inf", "nan"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_product_token_that_is_not_finite(dtype, bad, tnk, gplk, cuda):
+    """All of its outputs are NaN, whatever the weights; the others keep their bits."""
+    import torch
+
+    t, n, k = tnk
+    gen = _gen(cuda, 61 + t + n + k)
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float16
+    w, sf, _ = ref.random_weights(n, k, gen, cuda)
+    w[::2, (k - 1) // 2] &= 0x0F  # zero weights on the bad element in every other row
+    al = torch.full((1,), 1e-3, device=cuda)
+    x = torch.randn(t, k, device=cuda, generator=gen).to(dt)
+    clean, y = (torch.empty(t, n, dtype=dt, device=cuda) for _ in range(2))
+    gplk.gemv_nvfp4(x, w, sf, clean, al)
+    at = t // 2
+    x[at, k - 1] = float(bad)
+    gplk.gemv_nvfp4(x, w, sf, y, al)
+    torch.cuda.synchronize()
+    keep = [i for i in range(t) if i != at]
+    assert bool(torch.isnan(y[at]).all())
+    assert torch.equal(y[keep].view(torch.int16), clean[keep].view(torch.int16))
+
+
+# Resident blocks (strided x, several entries an expert, an odd last tile); clusters with the router of many
+# tokens; more experts than four to a lane.
+LAYERS = [(8, 64, 8, 640, 1024), (32, 40, 4, 320, 1088), (32, 2, 2, 192, 128), (7, 9, 3, 256, 192), (12, 300, 3, 128, 192)]
+
+
+@pytest.mark.parametrize("size", LAYERS)
+@pytest.mark.parametrize("pad", [0, 1, 3])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_layer_types_and_strides(dtype, pad, size, gplk, cuda):
+    layer_case(gplk, cuda, *size, dtype=dtype, pad=pad)
+
+
+@pytest.mark.parametrize("size", LAYERS)
+@pytest.mark.parametrize("bad", ["inf", "-inf", "nan"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_layer_token_that_is_not_finite(dtype, bad, size, gplk, cuda):
+    import torch
+
+    t, e, top, d, f = size
+    gen = _gen(cuda, 67 + sum(size))
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float16
+    layer = Layer(e, d, f, dt, gen, cuda)
+    x = torch.randn(t, d, device=cuda, generator=gen).to(dt)
+    at = t // 2
+    x[at, d - 1] = float(bad)
+    y, ids, w = layer.run(gplk, x, top)
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(y[at]).all())
+    assert bool(((ids[at] >= 0) & (ids[at] < e)).all()) and len(set(ids[at].tolist())) == top
+    keep = [i for i in range(t) if i != at]
+    layer.check(x[keep], top, True, y[keep], ids[keep], w[keep])
+
+
+def test_products_layers_and_gemms_at_once(gplk, cuda):
+    """Streams of products, of layers and of GEMMs side by side, whose blocks
+    want different parts of an SM: every call ends, with the bits it has alone."""
+    import torch
+
+    gen = _gen(cuda, 71)
+    bf = dict(dtype=torch.bfloat16, device=cuda)
+    sizes = [(1, 2048, 2048), (3, 1000, 4096), (12, 2000, 4096), (32, 4000, 1024)]
+    products = []
+    for t, n, k in sizes:
+        w, sf, _ = ref.random_weights(n, k, gen, cuda)
+        products.append((torch.randn(t, k, device=cuda, generator=gen).to(torch.bfloat16), w, sf))
+    al = torch.full((1,), 1e-3, device=cuda)
+    layers = [(Layer(e, d, f, torch.bfloat16, gen, cuda), torch.randn(t, d, device=cuda, generator=gen).to(**bf), top)
+              for t, e, top, d, f in ((2, 8, 2, 512, 256), (8, 64, 8, 640, 1024))]
+    p, q = torch.randn(1024, 1024, device=cuda, generator=gen).to(torch.bfloat16), torch.empty(1024, 1024, **bf)
+
+    def product_run(i, stream=None):
+        x, w, sf = products[i]
+        y = torch.empty(x.shape[0], w.shape[0], **bf)
+        gplk.gemv_nvfp4(x, w, sf, y, al, stream=stream)
+        return y
+
+    want = [product_run(i) for i in range(len(products))]
+    want_layers = [layer.run(gplk, x, top)[0] for layer, x, top in layers]
+    gplk.gemm_nn("bf16", p, p, q, 1024, 1024, 1024)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=cuda) for _ in range(4)]
+    got, got_layers, got_gemm = [], [], []
+    for r in range(12):
+        for s, i in zip(streams[:2], (r % 4, (r + 2) % 4)):
+            with torch.cuda.stream(s):
+                got.append((i, product_run(i)))
+        with torch.cuda.stream(streams[2]):
+            layer, x, top = layers[r % 2]
+            got_layers.append((r % 2, layer.run(gplk, x, top)[0]))
+        with torch.cuda.stream(streams[3]):
+            g = torch.empty_like(q)
+            gplk.gemm_nn("bf16", p, p, g, 1024, 1024, 1024)
+            got_gemm.append(g)
+    torch.cuda.synchronize()
+    for i, y in got:
+        assert torch.equal(y.view(torch.int16), want[i].view(torch.int16))
+    for i, y in got_layers:
+        assert torch.equal(y.view(torch.int16), want_layers[i].view(torch.int16))
+    for g in got_gemm:
+        assert torch.equal(g.view(torch.int16), q.view(torch.int16))
