@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
         bool done = false;
         if constexpr (M == Mode::Gemv) {
             constexpr int kHeld = 4;
-            if (nst * nw <= g.w_slots && units <= kHeld * kConvWarps) {
+            if (nst <= g.w_slots && units <= kHeld * kConvWarps) {
                 uint4 r[kHeld][2];
                 Unit u = first_unit;
 #pragma unroll
@@ -667,8 +667,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                 // One arrival for each stage in which the warp had a token.
                 if (lane == 0)
                     for (int i = 0; i < nst; ++i)
-                        if (((w - i * ntok) & (kConvWarps - 1)) < ntok)
-                            for (int h = 0; h < nw; ++h) mbar_arrive(&sm.full[i * nw + h]);
+                        if (((w - i * ntok) & (kConvWarps - 1)) < ntok) mbar_arrive(&sm.full[i]);
                 done = true;
             }
         }
@@ -748,10 +747,7 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
                     } while (cur.i == i);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (!kPerExpert && lane == 0) {
-                        mbar_arrive(&sm.full[slot0]);
-                        if (nw == 2) mbar_arrive(&sm.full[slot1]);
-                    }
+                    if (!kPerExpert && lane == 0) mbar_arrive(&sm.full[slot0]);
                 }
                 if (kPerExpert && lane == 0) {
                     mbar_arrive(&sm.full[slot0]);
