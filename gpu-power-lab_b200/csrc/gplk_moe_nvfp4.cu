@@ -419,12 +419,8 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
-    // The down products follow a gate / up kernel that itself waited for the
-    // routing tables: those and weights may be read at once, h behind a
-    // pdl_wait() of the warps that read it.
-    if constexpr (GATE_UP) pdl_wait();
+    pdl_wait();
     pdl_launch_dependents();
-    if constexpr (!GATE_UP) __threadfence();  // nothing older than the tables out of L1
     const uint32_t sfa_col0 = tmem + 4u * g.acc_cols, sfb_col0 = sfa_col0 + (uint32_t)g.w_slots * 16;
     const int groups = GATE_UP ? p.tiles : (p.tiles + 1) / 2;
     const int items = p.route->n_entries * groups;
@@ -543,7 +539,6 @@ __global__ void __launch_bounds__(kItemThreads, 1)
         // ------------------------------------------------------------ activations
         // Unit u = kb * tokens + t of an item is warp u % 16's.
         const int w = (int)warp - 2;
-        if constexpr (!GATE_UP) pdl_wait();
         struct Unit {
             int it, kb, t, ntok, step_kb, step_t, entry;
         };
@@ -633,7 +628,6 @@ __global__ void __launch_bounds__(kItemThreads, 1)
     } else {
         // ------------------------------------------------------------ epilogue
         // A thread has one row of both tiles.
-        if constexpr (!GATE_UP) pdl_wait();
         const uint32_t quarter = warp & 3u;
         const int row = (int)(quarter * 32 + lane);
         Cursor acc;

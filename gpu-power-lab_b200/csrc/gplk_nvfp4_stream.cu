@@ -382,15 +382,12 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
     set_up(p.T);
     // What is above may overlap the previous kernel's tail. The conversion
     // kernel that an Image kernel follows let it start only once every kernel
-    // before the two had completed, so weights may be read at once, and what that
-    // kernel wrote is read behind a pdl_wait() of its own. A Down kernel follows
-    // a gate / up kernel that itself waited for the routing tables, so it may
-    // read those and weights at once. Elsewhere nothing below touches global
-    // memory before the previous kernel has completed.
-    constexpr bool kEarly = IMAGE || M == Mode::Down;
-    if constexpr (!kEarly) pdl_wait();
+    // before the two had completed, with its results in global memory, so weights
+    // (which TMA fetches from L2) may be read at once, and what that kernel wrote
+    // is read behind a pdl_wait() of the warps that read it. Elsewhere nothing
+    // below touches global memory before the previous kernel has completed.
+    if constexpr (!IMAGE) pdl_wait();
     pdl_launch_dependents();
-    if constexpr (M == Mode::Down) __threadfence();  // nothing older than the tables out of L1
 
     // This block's rows, tokens and stages.
     int tile = cid, expert = 0, ntok = p.T, total = p.k_stages;
@@ -592,15 +589,14 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             if constexpr (M == Mode::GateUp) return sm.slot[n.t] / p.top;
             return n.t;
         };
-        auto load_row = [&](const Unit& n, int row, uint4 (&r)[2]) -> bool {
-            const int kb = M == Mode::Down ? n.kb : first + n.i;
+        auto load = [&](const Unit& n, uint4 (&r)[2]) -> bool {
+            const int row = row_of(n), kb = M == Mode::Down ? n.kb : first + n.i;
             const int k = kb * kStageK + (int)lane * 8;
             r[0] = r[1] = make_uint4(0, 0, 0, 0);
             if (row < 0) return false;
             if (k < p.K) load_raw(static_cast<const XT*>(p.X) + (size_t)row * p.ldx + k, p.x_vec != 0, r);
             return true;
         };
-        auto load = [&](const Unit& n, uint4 (&r)[2]) { return load_row(n, row_of(n), r); };
         // x / ntok for x <= 8, exactly.
         const uint32_t inverse = p.inverse[ntok];
         const int step_i = (int)(kConvWarps * inverse >> 16), step_t = kConvWarps - step_i * ntok;
@@ -672,17 +668,13 @@ __global__ void __launch_bounds__(kThreads<IMAGE>, 2)
             }
         }
         if (!done) {
-            // Two units' elements are on their way while one is converted. A Down
-            // block looks its first rows up before it waits for h.
+            // Two units' elements are on their way while one is converted.
             Unit cur = first_unit, ahead = first_unit;
             uint4 r0[2], r1[2];
             bool on0 = false, on1 = false;
-            const int row0 = ahead.i < nst ? row_of(ahead) : 0;
+            if (cur.i < nst) on0 = load(cur, r0);
             next_unit(ahead);
-            const int row1 = ahead.i < nst ? row_of(ahead) : 0;
-            if constexpr (kEarly) pdl_wait();
-            if (cur.i < nst) on0 = load_row(cur, row0, r0);
-            if (ahead.i < nst) on1 = load_row(ahead, row1, r1);
+            if (ahead.i < nst) on1 = load(ahead, r1);
             if (p.amax) {
                 if (w == 0 && (int)lane < ntok)
                     sm.amax[lane] = p.amax[kPerExpert ? sm.slot[lane] / p.top : (int)lane];

@@ -148,3 +148,56 @@ def test_products_layers_and_gemms_at_once(gplk, cuda):
         assert torch.equal(y.view(torch.int16), want_layers[i].view(torch.int16))
     for g in got_gemm:
         assert torch.equal(g.view(torch.int16), q.view(torch.int16))
+
+
+def test_weights_written_by_the_kernel_before(gplk, cuda):
+    """Weights and scales that a kernel writes right before each call, in
+    streams and in a captured graph: no product or layer starts on older ones."""
+    import torch
+
+    gen = _gen(cuda, 73)
+    t, n, k = 16, 3000, 4096  # converted ahead: weights are read while that runs
+    sets = [ref.random_weights(n, k, gen, cuda)[:2] for _ in range(3)]
+    layer, other = (Layer(8, 512, 320, torch.bfloat16, gen, cuda) for _ in range(2))
+    al = torch.full((1,), 1e-3, device=cuda)
+    x = torch.randn(t, k, device=cuda, generator=gen).to(torch.bfloat16)
+    v = torch.randn(3, 512, device=cuda, generator=gen).to(torch.bfloat16)
+    stacks = [torch.cat([a.flatten() for op in (q.gate, q.up, q.down) for a in op[:2]]) for q in (layer, other)]
+
+    def product(w, sf):
+        y = torch.empty(t, n, dtype=torch.bfloat16, device=cuda)
+        gplk.gemv_nvfp4(x, w, sf, y, al)
+        return y
+
+    want = [product(*s) for s in sets]
+    other.gate, other.up, other.down = ((b[0], b[1], a[2]) for a, b in zip((layer.gate, layer.up, layer.down),
+                                                                           (other.gate, other.up, other.down)))
+    other.router = layer.router
+    want_layers = [q.run(gplk, v, 2)[0] for q in (layer, other)]
+    parts = [a for op in (layer.gate, layer.up, layer.down) for a in op[:2]]
+    torch.cuda.synchronize()
+    w, sf = sets[0][0].clone(), sets[0][1].clone()
+
+    def write(i):
+        at = 0
+        for a in parts:
+            a.view(-1).copy_(stacks[i][at : at + a.numel()])
+            at += a.numel()
+
+    def both(i):
+        w.copy_(sets[i % 3][0])
+        sf.copy_(sets[i % 3][1])
+        y = product(w, sf)
+        write(i % 2)
+        return y, layer.run(gplk, v, 2)[0]
+
+    got = [both(i) for i in range(12)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [both(i) for i in range(6)]
+    graph.replay()
+    torch.cuda.synchronize()
+    for outs in (got, captured):
+        for i, (y, z) in enumerate(outs):
+            assert torch.equal(y.view(torch.int16), want[i % 3].view(torch.int16))
+            assert torch.equal(z.view(torch.int16), want_layers[i % 2].view(torch.int16))
