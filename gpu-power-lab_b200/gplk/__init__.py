@@ -250,6 +250,7 @@ def gemm_nvfp4_tn(A, B, SFA, SFB, D, K: int, alpha, stream=None) -> None:
 # ------------------------------------------------------------ a few tokens with NVFP4 weights
 
 MAX_TOKENS = 32
+_INT_MAX = 2**31 - 1  # ctypes cuts a larger C int without a word
 
 
 _act_dtypes: dict = {}
@@ -295,7 +296,7 @@ def _raw_stream(fn: str, stream, index: int) -> int:
 
 @functools.lru_cache(maxsize=4096)
 def gemv_nvfp4_workspace_bytes(T: int, N: int, K: int) -> int:
-    return int(lib().gplk_gemv_nvfp4_workspace_bytes(T, N, K))
+    return int(lib().gplk_gemv_nvfp4_workspace_bytes(T, N, K)) if max(T, N, K) <= _INT_MAX else 0
 
 
 def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None) -> None:
@@ -329,6 +330,7 @@ def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None)
         rp = residual.data_ptr()
     if T < 2:  # one row has no distance to the next
         ldx, ldy, ldr = K, N, N
+    _need(fn, max(T, N, K, ldx, ldy, ldr) <= _INT_MAX)
     if isinstance(workspace, str):
         need = gemv_nvfp4_workspace_bytes(T, N, K)
         workspace = _fresh(need, stream, W) if need else None
@@ -343,7 +345,7 @@ def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None)
 
 @functools.lru_cache(maxsize=4096)
 def moe_nvfp4_workspace_bytes(T: int, E: int, top: int, D: int, F: int) -> int:
-    return int(lib().gplk_moe_nvfp4_workspace_bytes(T, E, top, D, F))
+    return int(lib().gplk_moe_nvfp4_workspace_bytes(T, E, top, D, F)) if max(T, E, top, D, F) <= _INT_MAX else 0
 
 
 def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = True, workspace="auto",
@@ -388,6 +390,7 @@ def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = Tr
           == ds.get_device() == ga.get_device() == ua.get_device() == da.get_device() == dev)
     if T < 2:
         ldx = ldy = D
+    _need(fn, max(T, E, D, F, ldx, ldy) <= _INT_MAX)
     if isinstance(workspace, str):
         workspace = _fresh(max(1, moe_nvfp4_workspace_bytes(T, E, top, D, F)), stream, gw)
     _need(fn, workspace.get_device() == dev and workspace.is_contiguous())

@@ -201,3 +201,24 @@ def test_weights_written_by_the_kernel_before(gplk, cuda):
         for i, (y, z) in enumerate(outs):
             assert torch.equal(y.view(torch.int16), want[i % 3].view(torch.int16))
             assert torch.equal(z.view(torch.int16), want_layers[i % 2].view(torch.int16))
+
+
+def test_row_distances_beyond_32_bits_are_refused(gplk, cuda):
+    """A C int carries them: 2^32 + 64 would arrive as 64, a row distance in bounds
+    that is not the tensor's."""
+    import torch
+
+    k, n = 64, 128
+    w, sf, _ = ref.random_weights(n, k, _gen(cuda, 79), cuda)
+    al = torch.ones(1, device=cuda)
+    far = torch.empty((1 << 32) + 2 * n, dtype=torch.bfloat16, device=cuda)
+    x, y = (far.as_strided((2, width), ((1 << 32) + width, 1)) for width in (k, n))
+    x_near, y_near = x.contiguous(), torch.zeros(2, n, dtype=torch.bfloat16, device=cuda)
+    for args in ((x, y_near, None), (x_near, y, None), (x_near, y_near, y)):
+        with pytest.raises(gplk.GplkError):
+            gplk.gemv_nvfp4(args[0], w, sf, args[1], al, residual=args[2])
+    layer = Layer(4, 64, 128, torch.bfloat16, _gen(cuda, 80), cuda)
+    y_near = torch.zeros_like(x_near)
+    for args in ((x, y_near), (x_near, x)):
+        with pytest.raises(gplk.GplkError):
+            layer.run(gplk, args[0], 2, y=args[1])

@@ -32,3 +32,9 @@ def test_structure_is_the_header_s(gplk, tmp_path):
     for name, line in zip(names, fields, strict=True):
         field = getattr(gplk.MoeCfg, name)
         assert [int(v) for v in line.split()] == [field.offset, field.size], name
+
+
+def test_workspace_sizes_beyond_32_bits(gplk):
+    """ctypes cuts what a C int cannot hold: such sizes are refused, not cut."""
+    assert gplk.gemv_nvfp4_workspace_bytes(16, (1 << 32) + 8192, 8192) == 0
+    assert gplk.moe_nvfp4_workspace_bytes(2, 8, 2, (1 << 32) + 256, 128) == 0
