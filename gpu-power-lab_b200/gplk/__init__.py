@@ -273,8 +273,9 @@ def _need(fn: str, cond: bool) -> None:
 
 def _fresh(nbytes: int, stream, like):
     """A block of the caching allocator in the stream's own pool, on the device
-    of `like`, a uint8 tensor: calls that overlap, and captured graphs, never
-    share it."""
+    of `like`, a uint8 tensor: calls that overlap never share it, nor do captured
+    graphs, unless they were given one memory pool (whose graphs must not overlap
+    anyway)."""
     if stream is None:
         return like.new_empty(nbytes)
     import torch
@@ -302,7 +303,8 @@ def gemv_nvfp4_workspace_bytes(T: int, N: int, K: int) -> int:
 def gemv_nvfp4(X, W, SF, Y, alpha, residual=None, workspace="auto", stream=None) -> None:
     """Y = alpha * X @ w.T (+ residual) for up to 32 rows of activations.
     X: (T, K), Y and residual: (T, N), all bf16 or all f16, rows contiguous and
-    any distance apart; residual may be Y. W: (N, K/2) packed E2M1 and SF its
+    any distance (below 2^31 elements) apart; residual may be Y, and nothing else
+    may overlap Y. W: (N, K/2) packed E2M1 and SF its
     scale bytes, as gemm_nvfp4_tn and operands.quantize_nvfp4 have them;
     alpha: 1-element float32 tensor, the matrix scale. workspace: "auto" (from
     torch's allocator, on the call's stream), None (none: slower at most sizes),
@@ -351,8 +353,8 @@ def moe_nvfp4_workspace_bytes(T: int, E: int, top: int, D: int, F: int) -> int:
 def moe_nvfp4(X, router, gate, up, down, Y, ids, weights, renormalise: bool = True, workspace="auto",
               stream=None) -> None:
     """A mixture-of-experts layer (gplk_moe_nvfp4) for up to 32 tokens.
-    X, Y: (T, D), bf16 or f16, rows contiguous and any distance apart;
-    router: (E, D) of the same type. gate, up, down: (W, SF, alpha) with W
+    X, Y: (T, D), bf16 or f16, rows contiguous and any distance (below 2^31
+    elements) apart; nothing may overlap Y; router: (E, D) of the same type. gate, up, down: (W, SF, alpha) with W
     (E, F, D/2), (E, F, D/2), (E, D, F/2) packed E2M1, SF (E, bytes) the scale
     bytes of each expert's matrix and alpha (E,) float32. ids: (T, top) int32
     and weights: (T, top) float32 receive each token's experts and their

@@ -146,7 +146,7 @@ size_t gplk_nvfp4_sf_bytes(int rows, int k);
  * affect the result. X, Y and R are
  * row-major, of type `dtype`, with leading dimensions ldx >= K, ldy >= N and
  * ldr >= N in elements. R may be NULL, and may be Y itself (Y is then
- * updated in place); X must not overlap Y. Sums are FP32; each output is
+ * updated in place); nothing else that is read may overlap Y. Sums are FP32; each output is
  * rounded once. alpha is a device pointer to the weights' per-tensor scale.
  * Activations enter the products as multiples of 2^b / 2^16 (BF16) or
  * 2^b / 2^19 (FP16) within a group of 16, 2^b being the power of two at or
@@ -182,9 +182,11 @@ size_t gplk_gemv_nvfp4_workspace_bytes(int T, int N, int K);
  * that no token chose are not read. Logits, softmax, h and every sum are
  * FP32. Requires D % 64 == 0, F % 64 == 0, E <= 512, top <= min(E, 16),
  * E * F and E * D below 2^28; x, y and router in any alignment.
- * x must not overlap y. x and h enter the products as the activations of
+ * Nothing that is read may overlap y. x and h enter the products as the activations of
  * gplk_gemv_nvfp4 do, h by the type of x. A token with an infinity or a NaN in x gets NaN in y, and
- * experts that are in range and distinct but otherwise unspecified. The last
+ * experts that are in range and distinct but otherwise unspecified; other tokens
+ * are not affected. Scale bytes are numbers: a NaN among the down scales of an
+ * expert that some token chose may reach every token's y. The last
  * bits of a token's y may depend on which experts the other tokens choose
  * (sums are split accordingly); equal inputs give equal bits.
  * The workspace (gplk_moe_nvfp4_workspace_bytes, 16-byte aligned, any
