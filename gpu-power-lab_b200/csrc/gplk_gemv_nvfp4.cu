@@ -11,8 +11,9 @@ namespace fewtok {
 // Writes the B rows and scales of every stage as the ring holds them, a block
 // per token, so that the blocks of an Image kernel fetch them with one bulk
 // copy per stage instead of each converting all of the tokens again.
-// (512 / 1024 threads, us of the product: 16x8192x8192 13.1 / 13.4, 32x16384x16384
-// 41.5 / 39.0: 512 up to K = 8192.)
+// (512 / 1024 threads, us of the product: 32x8192x4096 12.2 / 12.6, 4x8192x8192 10.9 /
+// 11.1, 16x8192x8192 13.8 / 13.5, 32x8192x8192 17.5 / 16.9, 4x8192x12288 15.0 / 14.6,
+// 32x8192x12288 22.5 / 20.6, 32x16384x16384 43.6 / 39.6: 512 up to K = 8192.)
 static int image_threads(int K) { return K <= 8192 ? 512 : 1024; }
 
 template <typename XT>
@@ -96,9 +97,10 @@ static int block_stages(const Params& p) { return ((p.k_stages - 1) >> p.split_l
 // Whether the activations are converted once, by a kernel of their own, or by
 // every block for itself: that keeps up with the weights up to about four tokens
 // a stage, and a launch costs as much as some 20 units (a token's stage) of it.
-// Measured, fused / image, us: 4x16384x8192 19.1 / 18.8 (64 units in a block),
-// 8x16384x4096 17.1 / 12.2 (64), 8x16384x2048 10.7 / 9.8 (32), 8x8192x2048
-// 7.2 / 7.5 (16), 6x4096x4096 7.4 / 8.0 (12), 2x16384x8192 16.3 / 18.8 (32).
+// Measured, fused / image, us: 2x16384x16384 29.2 / 29.8, 3x16384x16384 29.4 / 30.0
+// (192 units in a block), 3x16384x4096 10.8 / 10.8, 4x16384x16384 33.5 / 30.1 (256),
+// 4x16384x8192 19.6 / 18.4 (128), 4x4096x4096 6.2 / 6.7 (16), 6x4096x4096 7.2 / 7.0
+// (24), 8x8192x2048 8.1 / 6.8, 8x16384x8192 30.6 / 18.6.
 static bool use_image(const Params& p) { return p.T >= 4 && p.T * block_stages(p) >= 24; }
 
 // Workspace of the converted activations: the stages' images, then the

@@ -22,11 +22,13 @@
 //             experts happens in the accumulator (stream_kernel). Else resident
 //             blocks write a sum per slot, and a last launch adds a token's.
 // No atomics order a sum; the maxima that atomics find do not depend on it.
-// Measured, us, against the bytes at 6547 GB/s: 1 token 64/8 2048x1024 20 (4.4),
-// 8 tokens 128/8 4096x768 66 (41), 16 tokens 16/2 4096x4096 85 (61), 32 tokens
-// 64/6 4096x2048 161 (132). Small layers are the launches' latencies, 15 us at
-// least; large ones what resident blocks do not overlap: routing before the first
-// weight (some 8 us) and a last round of items that not all SMs have.
+// Measured, us, against the bytes at 6547 GB/s: 1 token 64/8 2048x1024 19 (4.4),
+// 8 tokens 128/8 4096x768 69 (42), 16 tokens 16/2 4096x4096 88 (61; FP16 92), 32
+// tokens 64/6 4096x2048 165 (133), 32/8 4096x2048 136 (69). Small layers are the
+// launches' latencies, 15 us at least; large ones what resident blocks do not
+// overlap: routing before the first weight (some 8 us), a last round of items
+// that not all SMs have, and with many tokens an expert their conversion, which
+// every item repeats.
 #include "gplk_ptx.cuh"
 
 namespace gplk {
@@ -311,11 +313,13 @@ __global__ void __launch_bounds__(32 * kMaxTokens) route_kernel(const RouteParam
 }
 
 // Router product and routing of few experts and tokens in one launch: a cluster of
-// eight blocks shares out the experts and the first block routes. On the device
-// it takes as long as two launches do (when both were measured: layer of 8
-// experts, 1024 x 512, 16.2 us with it and 16.1 with two; of 32, 2048 x 704, 24.1
-// and 24.4; but of 64, 2048 x 1024, 22.1 and 20.8, so it stops at 65536 weights);
-// the host saves one.
+// eight blocks shares out the experts and the first block routes. It saves the host
+// a launch, which decides small layers that are called one by one, and costs the
+// device a little. Called / replayed, us, in one launch and in two: 1 token 8/2
+// 1024x512 18.3 and 20.1 / 15.2 and 15.2, 2 tokens 18.3 and 20.1 / 16.4 and 16.0,
+// 1 token 32/4 2048x704 18.7 and 20.0 / 17.2 and 17.1; 4 tokens 32/4 2048x704 24.2
+// and 23.7 / 22.8 and 22.1; but 1 token 64/8 2048x1024 21.9 and 20.8 / 21.3 and 19.4,
+// 4 tokens 64/8 38.1 and 35.2 replayed, so it stops at 65536 weights.
 constexpr int kFewBlocks = 8;
 constexpr int kFewWarps = 16;
 constexpr int kFewPer = 4;  // at most 128 experts
@@ -367,8 +371,9 @@ static bool few_experts(int T, int E, int D) { return T <= 4 && E <= 32 * kFewPe
 // about 4 us of an SM's stream each; there K is split over a cluster, which is
 // what few items need.
 //   warp 0 copies, warp 1 MMAs, warps 2..17 convert, warps 18..21 epilogue
-// (8 / 12 / 16 converting warps, us: 32 tokens 32/8 4096x2048 156 / 137 / 128, 64/6
-// 4096x2048 173 / 165 / 163, 8 tokens 128/8 4096x768 67.5 / 67.3 / 68.8.)
+// (8 / 12 / 16 converting warps, us: 32 tokens 32/8 4096x2048 165 / 145 / 137, 64/6
+// 4096x2048 176 / 167 / 166, 16 tokens 16/2 4096x4096 FP16 90.2 / 90.1 / 91.8, 8 tokens
+// 128/8 4096x768 66.6 / 67.0 / 68.2.)
 constexpr int kItemConvWarps = 16;
 constexpr int kItemThreads = 32 * (6 + kItemConvWarps);
 
@@ -741,18 +746,24 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* part, XT* y, 
 
 // Whether gate and up run as resident blocks over `items`: from two for every SM.
 // Measured, us of the layer, a block per item / resident: 976 items (32 tokens,
-// 64/6, 4096x2048) 175 / 162, 310 (8, 128/8, 4096x768) 78 / 66, but 256 (8, 8/2,
-// 4096x4096) 50.0 / 50.8 and (32, 8/2, 4096x4096) 69 / 72, 200 (16, 64/6, 2048x512)
-// 35 / 37, 64 (16, 8/2, 2048x1024) 23.1 / 25.5; 168 (4, 64/8, 4096x768) 52 / 51.
+// 64/6, 4096x2048) 177 / 165, 448 (16, 16/2, 4096x4096) 89 / 89, 390 (8, 64/6,
+// 2048x1408) 57 / 49, 310 (8, 128/8, 4096x768) 80 / 68, but 256 (8, 8/2, 4096x4096)
+// 53 / 53 and (32, 8/2, 4096x4096) 82 / 79, 200 (16, 64/6, 2048x512) 36 / 39, 168 (4,
+// 64/8, 4096x768) 50 / 56, 145 (4, 32/4, 4096x1408) 44 / 50, 64 (16, 8/2, 2048x1024)
+// 24 / 27.
 static bool use_gate_items(double items, int sm_count) { return items >= 2.0 * sm_count; }
 
 // Whether down runs as resident blocks with a sum per slot, or accumulates over the
 // experts, which splits K further but converts and multiplies for every token in
 // every stage: by the tiles an SM streams, the second's weighed by its tokens.
 // Measured, us of the layer, accumulating / resident: 1 token 8/2 4096x14336
-// 47 / 68, 64/8 2048x1024 20.1 / 21.2; 2 tokens 16/4 4096x2048 31.6 / 32.5; 4 tokens
-// 32/4 2048x704 22.2 / 22.6, 8/1 1024x14336 42 / 58; 8 tokens 8/2 4096x4096 58 / 50;
-// 16 tokens 8/2 2048x1024 27.4 / 22.3; 32 tokens 8/2 4096x4096 131 / 69.
+// 48 / 71, 64/8 2048x1024 19.3 / 20.8; 2 tokens 16/4 4096x2048 31.4 / 32.2; 3 tokens
+// 39 / 42, 4 tokens 52 / 57, 5 tokens 56 / 60, 6 tokens 59 / 62; 4 tokens 32/4 2048x704
+// 22.8 / 21.6, 5 tokens 23.9 / 22.3, 6 tokens 26.6 / 25.3; 64/8 2048x1024 5 tokens
+// 39.5 / 38.0, 7 tokens 52 / 47; 8/2 4096x4096 5 tokens 54 / 56, 6 tokens 63 / 60, 8
+// tokens 66 / 53, 32 tokens 147 / 82; 8 tokens 8/1 1024x14336 70 / 63; 16 tokens 8/2
+// 2048x1024 28.5 / 23.1. Where the two are within a tenth, some sizes have the
+// slower one (3, 5 and 6 tokens 16/4; 8 tokens 8/1).
 static bool use_down_items(int T, double active, int tiles, int k_stages, int split, int sm_count) {
     const int pairs = (tiles + 1) / 2;
     const double resident = 2.0 * k_stages * ceil(active * pairs / sm_count);

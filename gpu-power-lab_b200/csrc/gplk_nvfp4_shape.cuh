@@ -39,9 +39,9 @@ struct Geometry {
 // fill the activations' slot of stage i then, which has to be free too: b = w
 // slots for single tiles, b = w / 2 + 1 for pairs. An Image block copies stage
 // i - w + b's then: its activations come out of L2, sooner than the weights, so
-// that it holds four stages of them and the more of weights. (Weights on their
-// way are what counts: with as many slots of both, 28 x 8192 x 8192 takes 18.6
-// instead of 16.8 us, 8 x 16384 x 8192 18.5 instead of 17.9.)
+// that it holds four stages of them and the more of weights. (With as many slots
+// of both, us: 28 x 8192 x 8192 17.1 instead of 16.9, 8 x 16384 x 8192 17.9 and 32 x
+// 16384 x 16384 40 as with four.)
 constexpr int kImageSlots = 4;
 
 static uint32_t ring_of(const Geometry& g) {

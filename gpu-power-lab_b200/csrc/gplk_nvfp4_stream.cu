@@ -49,10 +49,12 @@
 //               warps 2..5 only.
 // The MMA warp runs its loop converged and elects the issuing lane: with
 // addresses and descriptors in uniform registers, 65536 x 8192 at one token
-// takes 51 us; issued from a lane of a diverged warp 76 us. At one token that is
-// 5.9 TB/s, with 4.5 us of start and end in smaller calls; at 32 tokens what counts
-// is the weights on their way (16384 x 16384: 40 us; 37 without any MMA, scale
-// copy or activation), since activations take half of the shared memory.
+// takes 49 us (6.2 TB/s); issued from a lane of a diverged warp it took 76 us.
+// Smaller calls have some 4 us of start and end. At 32 tokens what counts is the
+// weights on their way, since activations take half of the shared memory (16384 x
+// 16384: 40 us; an earlier build's 42 were 37 without any MMA, scale copy or
+// activation), and, with more tiles than SMs, the rounds of blocks, each with a
+// start and an end (65536 x 8192: 102 us against 47 at HBM's rate).
 // Every mbarrier wait is bounded, as everywhere in this library.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -900,9 +902,9 @@ static Shape set_shape(Params& p, int planes, int tokens, bool each, int tiles, 
 //   way), two stages' time for start and end, half a one for each doubling of the
 //   cluster;
 //   else waves of blocks, each with that start and end.
-// Measured at one token, us, for 1 / 2 / 4 / 8 slices: 2048 x 2048 6.4 / 4.9 / 4.4 /
-// 4.4, 4096 x 4096 8.9 / 6.6 / 5.4 / 5.7, 8192 x 2048 6.4 / 5.3 / 5.5 / 10.6, 8192 x
-// 8192 14.3 / 10.4 / 9.8 / 14.0, 28672 x 8192 24.0 / 27.3 / 33.3 / 43.1.
+// Measured at one token, us, for 1 / 2 / 4 / 8 slices: 2048 x 2048 6.2 / 4.8 / 4.3 /
+// 4.4, 4096 x 4096 8.9 / 6.5 / 5.1 / 5.5, 8192 x 2048 6.3 / 5.0 / 5.1 / 10.0, 8192 x
+// 8192 14.5 / 10.3 / 8.9 / 13.3, 28672 x 8192 24.0 / 27.1 / 33.1 / 43.0.
 static int choose_split_log2(double units, double stages, int sms, int per_sm) {
     int best = 0;
     double best_cost = 0;
