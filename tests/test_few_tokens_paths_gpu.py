@@ -222,3 +222,69 @@ def test_row_distances_beyond_32_bits_are_refused(gplk, cuda):
     for args in ((x, y_near), (x_near, x)):
         with pytest.raises(gplk.GplkError):
             layer.run(gplk, args[0], 2, y=args[1])
+
+
+def _rows(w, sf, at, k):
+    """float64 values of rows `at` of one matrix."""
+    import torch
+
+    r, g = at.view(-1, 1), torch.arange(k // 16, device=w.device).view(1, -1)
+    return ref.decode(w[at], sf[(r // 128 * -(-k // 64) + g // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + g % 4])
+
+
+def test_product_offsets_beyond_32_bits(gplk, cuda):
+    """8 GiB of codes: rows on both sides of 2^32 bytes, and the last ones."""
+    import torch
+
+    n, k = 131072 + 40, 131072
+    gen = _gen(cuda, 83)
+    w = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=cuda, generator=gen)
+    sf = torch.randint(0x28, 0x48, (ref.sf_bytes(n, k),), dtype=torch.uint8, device=cuda, generator=gen)
+    x = torch.randn(4, k, device=cuda, generator=gen).to(torch.bfloat16)
+    al = torch.full((1,), 1e-3, device=cuda)
+    at = torch.cat([torch.arange(65536 - 64, 65536 + 64), torch.arange(n - 100, n)]).to(cuda)
+    wd = _rows(w, sf, at, k)
+    for workspace in ("auto", None):
+        y = torch.empty(4, n, dtype=torch.bfloat16, device=cuda)
+        gplk.gemv_nvfp4(x, w, sf, y, al, workspace=workspace)
+        want = float(al) * (x.double() @ wd.T)
+        err = ref.product_error(wd, x, float(al)) + 2 * 2.0 ** -24 * want.abs()
+        assert ref.off(y[:, at], want, err, torch.bfloat16) <= 1
+
+
+def test_layer_offsets_beyond_32_bits(gplk, cuda):
+    """Stacks of 4 GiB and more, of which the last experts are chosen."""
+    import torch
+
+    e, d, f, t, top = 512, 4096, 4160, 3, 2
+    gen = _gen(cuda, 89)
+
+    def stack(rows, k):
+        w = torch.randint(0, 256, (e, rows, k // 2), dtype=torch.uint8, device=cuda, generator=gen)
+        sf = torch.randint(0x28, 0x40, (e, ref.sf_bytes(rows, k)), dtype=torch.uint8, device=cuda, generator=gen)
+        return w, sf, torch.full((e,), 0.3 / k ** 0.5, device=cuda)
+
+    gate, up, down = stack(f, d), stack(f, d), stack(d, f)
+    assert gate[0].numel() > 1 << 32
+    x = torch.randn(t, d, device=cuda, generator=gen).to(torch.bfloat16)
+    router = torch.randn(e, d, device=cuda, generator=gen) / d ** 0.5
+    for i in range(t):  # token i's experts are among the last
+        router[e - 1 - i] += x[i].float() / 64
+        router[e - 4 - i] += x[i].float() / 128
+    router = router.to(torch.bfloat16)
+    y, ids, w = torch.empty_like(x), torch.empty(t, top, dtype=torch.int32, device=cuda), torch.empty(t, top, device=cuda)
+    gplk.moe_nvfp4(x, router, gate, up, down, y, ids, w)
+    assert int(ids.min()) >= e - 8
+
+    class Decoded:
+        def __init__(self, op, rows, k):
+            self.op, self.rows, self.k = op, rows, k
+
+        def __getitem__(self, i):
+            at = torch.arange(self.rows, device=cuda)
+            return _rows(self.op[0][i], self.op[1][i], at, self.k), float(self.op[2][i])
+
+    want, err, wids, ww, dw = ref.moe(x, router, Decoded(gate, f, d), Decoded(up, f, d), Decoded(down, d, f), top, True)
+    assert torch.equal(ids, wids)
+    assert bool(((w.double() - ww).abs() <= dw * ww + 2.0 ** -140).all())
+    assert ref.off(y, want, err, x.dtype) <= 1
